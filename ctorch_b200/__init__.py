@@ -124,6 +124,36 @@ class Experts(C.Structure):
                 ("gated", C.c_int32), ("weigh_results", C.c_int32), ("identity", C.c_int32), ("after", C.POINTER(Sandwich))]
 
 
+class KvPages(C.Structure):
+    """Paged keys and values whose pages may be shared: b200_kv_pages."""
+    _fields_ = [("dtype", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("sequences", C.c_int32),
+                ("pages_per_sequence", C.c_int32), ("pages", C.c_int64), ("key", C.c_void_p), ("value", C.c_void_p), ("table", C.c_void_p)]
+
+
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_PARTS = 0, 1, 2, 3
+
+
+class RotaryScaling(C.Structure):
+    """How the angles of long contexts are stretched: b200_rotary_scaling."""
+    _fields_ = [("kind", C.c_int32), ("base", C.c_double), ("factor", C.c_double), ("original", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class RotaryAppendArgs(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("rot_dims", C.c_int32), ("rotate_pairs", C.c_int32), ("cosine", C.c_void_p), ("sine", C.c_void_p), ("positions", C.c_int32),
+                ("offset", C.c_void_p), ("projected", C.c_void_p), ("stride", C.c_int64), ("query_dtype", C.c_int32), ("query", C.c_void_p), ("cache", KvPages)]
+
+
+class PrefixArgs(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("scale", C.c_float), ("query", C.c_void_p), ("cache", KvPages), ("prefix", KvPages), ("groups", C.c_int32),
+                ("group_first", C.c_void_p), ("group_prefix", C.c_void_p), ("prefix_length", C.c_void_p)]
+
+
+class VerifyArgs(C.Structure):
+    _fields_ = [("vocab", C.c_int64), ("stride", C.c_int64), ("logits", C.c_void_p), ("draft_logits", C.c_void_p), ("ids", C.c_void_p), ("temperature", C.c_double),
+                ("accept", C.c_void_p), ("draw", C.c_void_p), ("accepted", C.c_void_p), ("next", C.c_void_p), ("advance", C.c_int32)]
+
+
 class PassEntry(C.Structure):
     _fields_ = [("slot", C.c_int64), ("tokens", C.POINTER(C.c_int64)), ("token_count", C.c_size_t), ("want", C.POINTER(C.c_int64)),
                 ("want_count", C.c_size_t)]
@@ -278,6 +308,13 @@ def _declare(l: C.CDLL) -> None:
         "b200_experts_grouped": (C.c_int, [C.POINTER(Experts), vp, vp, vp, sz, vp]),
         "b200_experts_takes_grouped": (i32, [C.POINTER(Experts)]),
         "b200_latent_attention_kernel": (C.c_char_p, [C.POINTER(LatentArgs)]),
+        "b200_kv_cache_pages": (C.c_int, [vp, C.POINTER(KvPages)]),
+        "b200_rotary_tables": (C.c_int, [C.POINTER(RotaryScaling), i32, i64, i64, vp, vp, vp]),
+        "b200_rotary_append": (C.c_int, [C.POINTER(RotaryAppendArgs), C.POINTER(Rows), vp]),
+        "b200_prefix_scratch_bytes": (sz, [C.POINTER(PrefixArgs), C.POINTER(Rows), i32, i32]),
+        "b200_prefix_attention": (C.c_int, [C.POINTER(PrefixArgs), C.POINTER(Rows), i32, i32, vp, sz, vp, vp, vp, i64, vp]),
+        "b200_verify_scratch_bytes": (sz, [C.POINTER(VerifyArgs), C.POINTER(Rows)]),
+        "b200_verify_drafts": (C.c_int, [C.POINTER(VerifyArgs), C.POINTER(Rows), vp, sz, vp]),
         "b200_take_device_status": (C.c_int, [i32, vp, C.POINTER(i32)]),
     }
     for name, (restype, argtypes) in sig.items():

@@ -213,6 +213,12 @@ void* b200_kv_cache_pool(b200_kv_cache* c, int32_t which) { return c->pool[which
 int32_t b200_kv_cache_pages_per_sequence(const b200_kv_cache* c) { return c->pages_per_seq; }
 int32_t b200_kv_cache_page_size(const b200_kv_cache* c) { return c->page_size; }
 size_t b200_kv_cache_pool_bytes(const b200_kv_cache* c) { return c->pool_bytes; }
+int b200_kv_cache_pages(const b200_kv_cache* c, b200_kv_pages* out) {
+    if (!c || !out) { set_error("b200_kv_cache_pages: bad pointer"); return B200_BAD_ARGUMENT; }
+    if (!c->pool[1]) { set_error("b200_kv_cache_pages: a latent cache holds no keys and values of heads"); return B200_UNSUPPORTED; }
+    *out = b200_kv_pages{c->dtype, c->kv_heads, c->head_dim, c->page_size, c->sequences, c->pages_per_seq, c->num_pages, c->pool[0], c->pool[1], c->page_table};
+    return B200_OK;
+}
 
 int b200_kv_cache_advance(b200_kv_cache* const* caches, int32_t count, int32_t delta, void* stream) {
     if (!caches || count < 0) return B200_BAD_ARGUMENT;

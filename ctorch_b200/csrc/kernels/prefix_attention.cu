@@ -1,0 +1,685 @@
+// Grouped-query attention of packed sequences over a prefix that groups of them share and over their own tokens (b200_prefix_attention).
+//
+// With G = heads / kv_heads, the rows of a group times the G heads of one KV head are the M side of the products with the prefix: every key and
+// value of the prefix enters an SM once per tile of rows instead of once per sequence.  A sequence's own tokens are the same work with the rows
+// of that sequence.  Items are (prefix tile or sequence tile, KV head, split of the keys); each leaves an unnormalised partial result (maximum,
+// sum, accumulator) per row and head, and the merge kernel joins them under one softmax:
+//   m = max m_i,  out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i      (scores in units of log2 e).
+#include "mma.cuh"
+#include "paged.cuh"
+#include "rows.cuh"
+
+#include <cmath>
+
+namespace b200 {
+namespace {
+
+constexpr int kUnit = 64;   // keys of a step; splits are whole steps
+
+struct PrefixParams {
+    RowsView rows;
+    PagesView own, prefix;
+    int heads, group, dim, groups;
+    const int32_t *group_first, *group_prefix, *prefix_length;
+    const void* query;
+    float scale;               // times log2(e)
+    int prefix_splits, own_splits;
+    int prefix_tiles;          // row tiles of all groups, at most
+    int own_tiles;             // row tiles per sequence, at most
+    float* part_o;             // [rows * heads][splits][dim]
+    float* part_ml;            // [rows * heads][splits][2]
+    float* out;
+    __nv_bfloat16 *out_hi, *out_lo;
+    int64_t out_stride;
+};
+
+struct KeySpan { int begin, end; };
+// Split `index` of `total` keys.
+__device__ __forceinline__ KeySpan split_span(int total, int splits, int index) {
+    const int steps = (total + kUnit - 1) / kUnit, per = (steps + splits - 1) / splits;
+    const int begin = min(total, index * per * kUnit);
+    return {begin, min(total, begin + per * kUnit)};
+}
+__device__ __forceinline__ int used_splits(int total, int splits) {
+    const int steps = (total + kUnit - 1) / kUnit;
+    if (steps == 0) return 0;
+    const int per = (steps + splits - 1) / splits;
+    return (steps + per - 1) / per;
+}
+
+__device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
+    const int slot = __ldg(p.group_prefix + g);
+    if (slot < 0 || slot >= p.prefix.sequences) return 0;
+    return max(0, min(__ldg(p.prefix_length + slot), p.prefix.capacity()));
+}
+__device__ __forceinline__ int own_keys(const PrefixParams& p, int slot, int count) {
+    if (slot < 0 || slot >= p.own.sequences) return 0;
+    return max(0, min(p.rows.lengths[slot] + count, p.own.capacity()));
+}
+
+// The group that owns sequence s, -1 if none does.
+__device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
+    int low = 0, high = p.groups;   // the last group that begins at or before s
+    while (low < high) {
+        const int middle = (low + high) / 2;
+        if (__ldg(p.group_first + middle) <= s) low = middle + 1;
+        else high = middle;
+    }
+    return low > 0 && s < __ldg(p.group_first + low) ? low - 1 : -1;
+}
+
+// One item: the rows m_begin .. m_count - 1 of (row, head of the group) pairs from `row` on, and a span of keys.
+struct Item {
+    bool live, causal;
+    int row, m_begin, m_count;   // first row of the group or sequence; pair m is row + m / group, head kv_head * group + m % group
+    int kv_head, slot, split;    // split: which partial result
+    int visible;                 // keys that pair 0 sees (causal: pair m sees m / group more)
+    KeySpan keys;
+};
+
+// Items are numbered split-major inside a kind; the prefix's, which are longer, come first.  Every warp works this out for itself.
+__device__ __forceinline__ Item find_item(const PrefixParams& p, int index, int tile_rows) {
+    Item it{};
+    const int kv_heads = p.own.kv_heads, prefix_items = p.prefix_tiles * kv_heads * p.prefix_splits;
+    const int lane = threadIdx.x & 31;
+    if (index < prefix_items) {
+        it.kv_head = index % kv_heads;
+        const int rest = index / kv_heads;
+        int tile = rest % p.prefix_tiles;
+        it.split = rest / p.prefix_tiles;
+        // tile -> group: the groups' tile counts are added up 32 at a time
+        for (int base = 0; base < p.groups; base += 32) {
+            const int g = base + lane;
+            int begin = 0, rows = 0, tiles = 0;
+            if (g < p.groups) {
+                begin = __ldg(p.rows.first + __ldg(p.group_first + g));
+                rows = max(0, __ldg(p.rows.first + __ldg(p.group_first + g + 1)) - begin);
+                tiles = (rows * p.group + tile_rows - 1) / tile_rows;
+            }
+            int up_to = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, up_to, o);
+                if (lane >= o) up_to += other;
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, up_to > tile);
+            if (found) {
+                const int from = __ffs(found) - 1;
+                it.row = __shfl_sync(0xffffffffu, begin, from);
+                it.m_count = __shfl_sync(0xffffffffu, rows, from) * p.group;
+                it.m_begin = (tile - __shfl_sync(0xffffffffu, up_to - tiles, from)) * tile_rows;
+                const int group = base + from, keys = prefix_keys(p, group);
+                it.slot = __ldg(p.group_prefix + group);
+                it.keys = split_span(keys, p.prefix_splits, it.split);
+                it.visible = keys;
+                it.live = it.keys.begin < it.keys.end;
+                return it;
+            }
+            tile -= __shfl_sync(0xffffffffu, up_to, 31);
+        }
+        return it;
+    }
+    index -= prefix_items;
+    it.kv_head = index % kv_heads;
+    int rest = index / kv_heads;
+    const int tile = rest % p.own_tiles;
+    rest /= p.own_tiles;
+    const int s = rest % p.rows.sequences, split = rest / p.rows.sequences;
+    it.split = p.prefix_splits + split;
+    it.row = __ldg(p.rows.first + s);
+    const int count = max(0, __ldg(p.rows.first + s + 1) - it.row);
+    it.m_count = count * p.group;
+    it.m_begin = tile * tile_rows;
+    it.slot = __ldg(p.rows.slot + s);
+    const int keys = own_keys(p, it.slot, count);
+    it.keys = split_span(keys, p.own_splits, split);
+    it.causal = true;
+    it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
+    if (it.live) it.visible = p.rows.lengths[it.slot] + 1;
+    return it;
+}
+
+// Where pair m of an item leaves its partial result: row of [rows * heads][splits].
+__device__ __forceinline__ int64_t partial_row(const PrefixParams& p, const Item& it, int m) {
+    return ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * (p.prefix_splits + p.own_splits) + it.split;
+}
+
+// ---- any type and head size: f32 products on the CUDA cores --------------------------------------------------------------------------------
+constexpr int kPlainRows = 32, kPlainKeys = 32, kPlainThreads = 128;
+
+__host__ __device__ constexpr int plain_width(int dim) { return (dim + 3) / 4 * 4; }
+__host__ __device__ constexpr int plain_smem(int dim) {
+    return (kPlainRows * plain_width(dim) + 2 * kPlainKeys * (plain_width(dim) + 4) + kPlainRows * (kPlainKeys + 1)) * static_cast<int>(sizeof(float));
+}
+
+// A tile of 32 pairs x 32 keys: thread (ty, tx) has the scores of rows 2 ty, 2 ty + 1 with the keys tx + 8 j, and the columns 4 tx + 32 c of their
+// accumulators.
+template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) prefix_plain_kernel(const PrefixParams p) {
+    extern __shared__ __align__(16) float plain_shared[];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const Item it = find_item(p, blockIdx.x, kPlainRows);
+    if (!it.live) return;
+    const int width = plain_width(p.dim), pitch = width + 4;
+    float* query = plain_shared;
+    float* key = query + kPlainRows * width;
+    float* value = key + kPlainKeys * pitch;
+    float* weight = value + kPlainKeys * pitch;
+    const int thread = threadIdx.x, ty = thread / 8, tx = thread % 8;
+    const PagesView& view = it.causal ? p.own : p.prefix;
+    for (int i = thread; i < kPlainRows * width; i += kPlainThreads) {
+        const int m = it.m_begin + i / width, d = i % width;
+        query[i] = m < it.m_count && d < p.dim
+                       ? load_as_f32(static_cast<const T*>(p.query), ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * p.dim + d)
+                       : 0.0f;
+    }
+    float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, acc[2][BLOCKS][4] = {};
+    int limit[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) limit[r] = it.causal ? min(it.keys.end, it.visible + (it.m_begin + 2 * ty + r) / p.group) : it.keys.end;
+    for (int begin = it.keys.begin; begin < it.keys.end; begin += kPlainKeys) {
+        __syncthreads();
+        for (int i = thread; i < kPlainKeys * width; i += kPlainThreads) {
+            const int r = i / width, d = i % width, position = begin + r;
+            float k = 0.0f, v = 0.0f;
+            if (position < it.keys.end && d < p.dim) {
+                const int page = page_of(view, it.slot, position / view.page_size);
+                if (page >= 0) {
+                    const int64_t at = page_row(view, page, it.kv_head, position % view.page_size) + d;
+                    k = load_as_f32(static_cast<const T*>(view.pool[0]), at);
+                    v = load_as_f32(static_cast<const T*>(view.pool[1]), at);
+                }
+            }
+            key[r * pitch + d] = k;
+            value[r * pitch + d] = v;
+        }
+        __syncthreads();
+        float score[2][4] = {};
+        for (int d = 0; d < width; d += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(query + 2 * ty * width + d), b = *reinterpret_cast<const float4*>(query + (2 * ty + 1) * width + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 k = *reinterpret_cast<const float4*>(key + (tx + 8 * j) * pitch + d);
+                score[0][j] += a.x * k.x + a.y * k.y + a.z * k.z + a.w * k.w;
+                score[1][j] += b.x * k.x + b.y * k.y + b.z * k.z + b.w * k.w;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float top = most[r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                score[r][j] = begin + tx + 8 * j < limit[r] ? score[r][j] * p.scale : -INFINITY;
+                top = fmaxf(top, score[r][j]);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float base = top == -INFINITY ? 0.0f : top, shrink = exp2f(most[r] - base);
+            float here = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w = exp2f(score[r][j] - base);
+                here += w;
+                weight[(2 * ty + r) * (kPlainKeys + 1) + tx + 8 * j] = w;
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) here += __shfl_xor_sync(0xffffffffu, here, o);
+            sum[r] = sum[r] * shrink + here;
+            most[r] = top;
+#pragma unroll
+            for (int c = 0; c < BLOCKS; ++c)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc[r][c][u] *= shrink;
+        }
+        __syncwarp();   // the weights of two rows are written and read by the same eight lanes
+        // row 2 ty sees no more than row 2 ty + 1; what a row does not see is not multiplied, since it may be no number
+        const int both = min(kPlainKeys, limit[0] - begin), one = min(kPlainKeys, limit[1] - begin);
+        for (int k = 0; k < one; ++k) {
+            const float a = weight[2 * ty * (kPlainKeys + 1) + k], b = weight[(2 * ty + 1) * (kPlainKeys + 1) + k];
+#pragma unroll
+            for (int c = 0; c < BLOCKS; ++c) {
+                if (32 * c + 4 * tx >= width) continue;
+                const float4 v = *reinterpret_cast<const float4*>(value + k * pitch + 32 * c + 4 * tx);
+                if (k < both) { acc[0][c][0] += a * v.x; acc[0][c][1] += a * v.y; acc[0][c][2] += a * v.z; acc[0][c][3] += a * v.w; }
+                acc[1][c][0] += b * v.x; acc[1][c][1] += b * v.y; acc[1][c][2] += b * v.z; acc[1][c][3] += b * v.w;
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int m = it.m_begin + 2 * ty + r;
+        if (m >= it.m_count) continue;
+        const int64_t at = partial_row(p, it, m);
+        if (tx == 0) {
+            p.part_ml[2 * at] = most[r];
+            p.part_ml[2 * at + 1] = sum[r];
+        }
+#pragma unroll
+        for (int c = 0; c < BLOCKS; ++c)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (32 * c + 4 * tx + u < p.dim) p.part_o[at * p.dim + 32 * c + 4 * tx + u] = acc[r][c][u];
+    }
+}
+
+// ---- bf16, heads of 8 n <= 128 values: mma.sync ---------------------------------------------------------------------------------------------
+constexpr int kMmaThreads = 128, kMmaStages = 3;
+
+template <int HD> struct MmaShape {                              // HD: the head size rounded up to 64, 96 or 128
+    static constexpr int row_bytes = HD <= 64 ? 128 : 256;
+    static constexpr int tile_bytes = kUnit * row_bytes;         // K or V of one step
+    static constexpr int stage_bytes = 2 * tile_bytes;
+    static constexpr int smem_bytes = kMmaStages * stage_bytes;
+    static constexpr int slots = row_bytes / 16;                 // 16-byte pieces of a row
+    static constexpr int rows_per_pass = kMmaThreads / slots;
+    static constexpr int passes = kUnit / rows_per_pass;
+};
+// Byte offset of 16-byte piece c of row r: pieces are permuted inside groups of eight, so that ldmatrix and the copies are free of conflicts.
+template <int HD> __device__ __forceinline__ uint32_t piece_offset(int r, int c) {
+    return static_cast<uint32_t>(r * MmaShape<HD>::row_bytes + (((c & ~7) | ((c ^ r) & 7)) << 4));
+}
+
+// Steps with keys that some pairs of the tile do not see: a weight of 0 does not cancel a value that is no number, so such values leave the tile
+// before the products, and are added here to the accumulators of the pairs that do see them.
+template <int HD> __device__ __noinline__ void move_values_out(unsigned char* value, int pieces, int begin, int warp_key, int keys, const int (&seen)[2], float (&acc)[HD / 8][4]) {
+    const int lane = threadIdx.x & 31, quad = lane & 3;
+    for (int k = warp_key; k < warp_key + keys; ++k)
+        for (int n = 0; n < pieces; ++n) {
+            const uint32_t two = *reinterpret_cast<const uint32_t*>(value + piece_offset<HD>(k, n) + 4 * quad);
+            const float v[2] = {bf16_lo(two), bf16_hi(two)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!isfinite(v[e & 1]) && begin + k < seen[e >> 1]) {
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i)
+                        if (i == n) acc[i][e] += v[e & 1];
+                }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kUnit * pieces * 8; i += kMmaThreads) {
+        uint16_t* x = reinterpret_cast<uint16_t*>(value + piece_offset<HD>(i / (pieces * 8), i / 8 % pieces)) + i % 8;
+        if ((*x & 0x7f80) == 0x7f80) *x = 0;
+    }
+    __syncthreads();
+}
+template <int HD> __device__ __forceinline__ void guard_values(const PrefixParams& p, const Item& it, unsigned char* value, int begin, int warp_key, int keys,
+                                                               const int (&seen)[2], float (&acc)[HD / 8][4]) {
+    const int pieces = p.dim / 8;
+    bool odd = false;
+    for (int i = threadIdx.x; i < kUnit * pieces; i += kMmaThreads) {
+        const uint4 x = *reinterpret_cast<const uint4*>(value + piece_offset<HD>(i / pieces, i % pieces));
+        const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) odd |= (words[u] & 0x7f80u) == 0x7f80u || (words[u] & 0x7f800000u) == 0x7f800000u;
+    }
+    if (__syncthreads_or(odd)) move_values_out<HD>(value, pieces, begin, warp_key, keys, seen, acc);
+}
+
+// SPLIT: a tile of 16 pairs, each warp takes 16 of the 64 keys of a step and the warps' results are joined at the end; otherwise a tile of 64 pairs,
+// 16 per warp, all of which use the same keys.
+template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) prefix_mma_kernel(const PrefixParams p) {
+    using S = MmaShape<HD>;
+    extern __shared__ __align__(128) unsigned char mma_shared[];
+    constexpr int kKeys = SPLIT ? 16 : 64;       // keys per warp and step
+    constexpr int kTiles = kKeys / 8, kSteps = HD / 16, kColumns = HD / 8;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const Item it = find_item(p, blockIdx.x, SPLIT ? 16 : 64);
+    if (!it.live) return;
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    const PagesView& view = it.causal ? p.own : p.prefix;
+    const uint32_t shared = smem_u32(mma_shared);
+    const int pieces = p.dim / 8;
+    if (pieces < S::slots && pieces < HD / 8) {   // the columns past the head's size stay zero
+        for (int i = thread; i < kMmaStages * 2 * kUnit * S::slots; i += kMmaThreads) {
+            const int r = i / S::slots, c = i % S::slots;
+            if (c >= pieces) *reinterpret_cast<uint4*>(mma_shared + r / kUnit * S::tile_bytes + piece_offset<HD>(r % kUnit, c)) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    // Every thread copies piece `c` of the rows r0, r0 + rows_per_pass, ...; the page numbers of a step are fetched one step ahead of its copies.
+    const int c = thread % S::slots, r0 = thread / S::slots;
+    const int steps = (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+    const int64_t piece = static_cast<int64_t>(it.kv_head) * view.page_size * view.head_dim + c * 8;
+    int64_t at[S::passes];   // of the row in the pools, -1: zeros
+    auto fetch = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < S::passes; ++i) {
+            const int position = it.keys.begin + step * kUnit + r0 + i * S::rows_per_pass;
+            at[i] = -1;
+            if (c < pieces && position < it.keys.end) {
+                const int page = page_of(view, it.slot, position / view.page_size);
+                if (page >= 0) at[i] = (static_cast<int64_t>(page) * view.kv_heads * view.page_size + position % view.page_size) * view.head_dim + piece;
+            }
+        }
+    };
+    auto copy = [&](int step) {
+        const uint32_t stage = shared + step % kMmaStages * S::stage_bytes;
+        if (c < pieces) {
+#pragma unroll
+            for (int i = 0; i < S::passes; ++i) {
+                const uint32_t to = stage + piece_offset<HD>(r0 + i * S::rows_per_pass, c);
+                const bool live = at[i] >= 0;
+                const int64_t from = live ? at[i] : 0;
+                copy_async_16(to, static_cast<const __nv_bfloat16*>(view.pool[0]) + from, live);
+                copy_async_16(to + S::tile_bytes, static_cast<const __nv_bfloat16*>(view.pool[1]) + from, live);
+            }
+        }
+    };
+    fetch(0);
+    for (int step = 0; step < kMmaStages - 1; ++step) {
+        if (step < steps) {
+            copy(step);
+            fetch(step + 1);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // query fragments
+    const int quad = lane & 3, m0 = it.m_begin + (SPLIT ? 0 : warp * 16) + (lane >> 2);
+    uint32_t q[kSteps][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int m = m0 + 8 * r;
+        const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.query)
+                                   + ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * p.dim;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int d = 16 * k + 8 * h + 2 * quad;
+                q[k][2 * h + r] = m < it.m_count && d < p.dim ? __ldg(reinterpret_cast<const uint32_t*>(row + d)) : 0u;
+            }
+    }
+    int seen[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) seen[r] = it.causal ? min(it.keys.end, it.visible + (m0 + 8 * r) / p.group) : it.keys.end;
+    float acc[kColumns][4] = {}, most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    const int warp_key = SPLIT ? warp * 16 : 0;
+    const int first_limit = it.causal ? it.visible + it.m_begin / p.group : it.keys.end;   // keys that the tile's first pair sees
+    for (int step = 0; step < steps; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMmaStages - 2) : "memory");
+        __syncthreads();
+        if (step + kMmaStages - 1 < steps) {
+            copy(step + kMmaStages - 1);
+            fetch(step + kMmaStages);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const uint32_t key = shared + step % kMmaStages * S::stage_bytes, value = key + S::tile_bytes;
+        float score[kTiles][4] = {};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int n = 0; n < kTiles; n += 2) {
+                uint32_t b[4];   // keys n*8 .. +7 and +8 .. +15, both halves of the 16 values
+                ldsm_x4(b, key + piece_offset<HD>(warp_key + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                mma_16816(score[n], q[k], b[0], b[1]);
+                mma_16816(score[n + 1], q[k], b[2], b[3]);
+            }
+        const int first_key = it.keys.begin + step * kUnit + warp_key + 2 * quad;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float top = most[r];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float& x = score[n][2 * r + u];
+                    x = first_key + n * 8 + u < seen[r] ? x * p.scale : -INFINITY;
+                    top = fmaxf(top, x);
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(most[r] - base);
+            float here = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float& x = score[n][2 * r + u];
+                    x = exp2_fast(x - base);
+                    here += x;
+                }
+            sum[r] = sum[r] * shrink + here;   // of this lane's keys; the quad's are added at the end
+            most[r] = top;
+#pragma unroll
+            for (int n = 0; n < kColumns; ++n) {
+                acc[n][2 * r] *= shrink;
+                acc[n][2 * r + 1] *= shrink;
+            }
+        }
+        if (min(it.keys.end, it.keys.begin + (step + 1) * kUnit) > first_limit)
+            guard_values<HD>(p, it, mma_shared + (value - shared), it.keys.begin + step * kUnit, warp_key, kKeys, seen, acc);
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k) {
+            const uint32_t a[4] = {pack_bf16(score[2 * k][0], score[2 * k][1]), pack_bf16(score[2 * k][2], score[2 * k][3]),
+                                   pack_bf16(score[2 * k + 1][0], score[2 * k + 1][1]), pack_bf16(score[2 * k + 1][2], score[2 * k + 1][3])};
+#pragma unroll
+            for (int n = 0; n < kColumns; n += 2) {
+                uint32_t b[4];
+                ldsm_x4_trans(b, value + piece_offset<HD>(warp_key + 16 * k + (lane & 15), n + (lane >> 4)));
+                mma_16816(acc[n], a, b[0], b[1]);
+                mma_16816(acc[n + 1], a, b[2], b[3]);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    }
+    if constexpr (SPLIT) {
+        // join the warps: [warp][16 rows][HD] accumulators behind [warp][16][2] maxima and sums
+        __syncthreads();
+        float* joined = reinterpret_cast<float*>(mma_shared);
+        float* rows_of = joined + 4 * 16 * 2;
+        constexpr int kPitch = HD + 4;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int m = (lane >> 2) + 8 * r;
+            if (quad == 0) {
+                joined[(warp * 16 + m) * 2] = most[r];
+                joined[(warp * 16 + m) * 2 + 1] = sum[r];
+            }
+#pragma unroll
+            for (int n = 0; n < kColumns; ++n)
+                *reinterpret_cast<float2*>(rows_of + (warp * 16 + m) * kPitch + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+        }
+        __syncthreads();
+        const int live = min(16, it.m_count - it.m_begin);
+        for (int i = thread; i < live * (HD / 4); i += kMmaThreads) {
+            const int m = i / (HD / 4), d = i % (HD / 4) * 4;
+            float top = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, joined[(w * 16 + m) * 2]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = exp2_fast(joined[(w * 16 + m) * 2] - base);
+                const float4 v = *reinterpret_cast<const float4*>(rows_of + (w * 16 + m) * kPitch + d);
+                total += f * joined[(w * 16 + m) * 2 + 1];
+                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+            }
+            const int64_t to = partial_row(p, it, it.m_begin + m);
+            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(top, total);
+            if (d < p.dim) *reinterpret_cast<float4*>(p.part_o + to * p.dim + d) = o;
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int m = m0 + 8 * r;
+            if (m >= it.m_count) continue;
+            const int64_t to = partial_row(p, it, m);
+            if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most[r], sum[r]);
+#pragma unroll
+            for (int n = 0; n < kColumns; ++n)
+                if (8 * n < p.dim) *reinterpret_cast<float2*>(p.part_o + to * p.dim + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+        }
+    }
+}
+
+// ---- merge ------------------------------------------------------------------------------------------------------------------------------
+// A warp per row and head.
+__global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int64_t index = blockIdx.x * 4 + static_cast<int64_t>(threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int row = static_cast<int>(index / p.heads);
+    if (row >= min(p.rows.rows, __ldg(p.rows.first + p.rows.sequences))) return;
+    const int s = __ldg(p.rows.sequence + row), g = group_of(p, s);
+    const int from_prefix = g < 0 ? 0 : used_splits(prefix_keys(p, g), p.prefix_splits);
+    const int from_own = used_splits(own_keys(p, __ldg(p.rows.slot + s), __ldg(p.rows.first + s + 1) - __ldg(p.rows.first + s)), p.own_splits);
+    const int parts = from_prefix + from_own;
+    const int64_t base = index * (p.prefix_splits + p.own_splits);
+    auto place = [&](int i) { return base + (i < from_prefix ? i : p.prefix_splits + i - from_prefix); };
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[2 * place(i)]);
+    top = warp_max(top);
+    float total = 0.0f;
+    if (top > -INFINITY)
+        for (int i = lane; i < parts; i += 32) total += exp2f(p.part_ml[2 * place(i)] - top) * p.part_ml[2 * place(i) + 1];
+    total = warp_sum(total);
+    const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+    const int64_t to = row * p.out_stride + index % p.heads * p.dim;
+    for (int d = lane; d < p.dim; d += 32) {
+        float o = 0.0f;
+        if (top > -INFINITY)
+            for (int i = 0; i < parts; ++i) {
+                const float f = exp2f(p.part_ml[2 * place(i)] - top);
+                if (f > 0.0f) o += f * p.part_o[place(i) * p.dim + d];
+            }
+        store_forms(o * inverse, to + d, p.out, p.out_hi, p.out_lo);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------------
+constexpr int kMostDim = 256;
+
+enum class Form { plain, mma_split, mma_rows };
+struct Plan {
+    Form form;
+    int tile_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
+};
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length, int max_prefix) {
+    Plan plan{};
+    const int kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
+    uintptr_t bits = reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.cache.key) | reinterpret_cast<uintptr_t>(a.cache.value);
+    if (a.groups) bits |= reinterpret_cast<uintptr_t>(a.prefix.key) | reinterpret_cast<uintptr_t>(a.prefix.value);
+    const bool mma = a.cache.dtype == B200_BF16 && a.cache.head_dim % 8 == 0 && a.cache.head_dim <= 128 && bits % 16 == 0;
+    const int64_t pairs = pass.rows * group;
+    const int groups = a.groups < pass.sequences ? a.groups : pass.sequences;
+    plan.form = !mma ? Form::plain : pairs <= 16 * static_cast<int64_t>(pass.sequences) ? Form::mma_split : Form::mma_rows;
+    if (mma && a.groups && pairs > 16 * static_cast<int64_t>(a.groups)) plan.form = Form::mma_rows;
+    plan.tile_rows = plan.form == Form::plain ? kPlainRows : plan.form == Form::mma_split ? 16 : 64;
+    const bool prefix = a.groups > 0 && max_prefix > 0;
+    plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.tile_rows) + groups : 0;
+    plan.own_tiles = ceil_div(static_cast<int64_t>(pass.max_count) * group, plan.tile_rows);
+    auto splits = [&](int64_t items, int keys) {
+        const int most = ceil_div(keys, 4 * kUnit);
+        int n = static_cast<int>(2 * 148 / (items > 0 ? items : 1));
+        if (n > most) n = most;
+        if (n > 64) n = 64;
+        return n < 1 ? 1 : n;
+    };
+    plan.prefix_splits = prefix ? splits(static_cast<int64_t>(plan.prefix_tiles) * kv_heads, max_prefix) : 0;
+    plan.own_splits = splits(static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads, max_length);
+    return plan;
+}
+
+bool same_heads(const b200_kv_pages& a, const b200_kv_pages& b) { return a.dtype == b.dtype && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim; }
+
+int check_prefix(const b200_prefix_args* a, const b200_rows* pass, PrefixParams& p) {
+    if (!rows_view(pass, p.rows)) return B200_BAD_ARGUMENT;
+    if (!a) { set_error("b200_prefix_attention: no arguments"); return B200_BAD_ARGUMENT; }
+    if (!pages_view(a->cache, "b200_prefix_attention", p.own)) return B200_BAD_ARGUMENT;
+    if (a->groups < 0 || a->heads <= 0 || a->heads % a->cache.kv_heads || !a->query || !std::isfinite(a->scale)
+        || (a->groups && (!a->group_first || !a->group_prefix || !a->prefix_length))) {
+        set_error("b200_prefix_attention: bad pointer, size, scale or head grouping");
+        return B200_BAD_ARGUMENT;
+    }
+    if (a->groups) {
+        if (!pages_view(a->prefix, "b200_prefix_attention", p.prefix)) return B200_BAD_ARGUMENT;
+        if (!same_heads(a->cache, a->prefix)) { set_error("b200_prefix_attention: prefix and cache differ in type or heads"); return B200_BAD_ARGUMENT; }
+    }
+    if (a->cache.head_dim > kMostDim) { set_error("b200_prefix_attention: head_dim above %d is not supported", kMostDim); return B200_UNSUPPORTED; }
+    return B200_OK;
+}
+
+template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned items, cudaStream_t stream) {
+    auto kernel = p.dim <= 64 ? prefix_plain_kernel<T, 2> : p.dim <= 128 ? prefix_plain_kernel<T, 4> : prefix_plain_kernel<T, 8>;
+    const int smem = plain_smem(p.dim);
+    if (smem > 48 * 1024) {
+        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (status != cudaSuccess) return status;
+    }
+    return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p);
+}
+
+template <int HD> cudaError_t launch_mma(const PrefixParams& p, bool split, unsigned items, cudaStream_t stream) {
+    auto kernel = split ? prefix_mma_kernel<HD, true> : prefix_mma_kernel<HD, false>;
+    constexpr int smem = MmaShape<HD>::smem_bytes;
+    const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (status != cudaSuccess) return status;
+    return launch_dependent(kernel, dim3(items), dim3(kMmaThreads), static_cast<size_t>(smem), stream, p);
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" size_t b200_prefix_scratch_bytes(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix) {
+    PrefixParams p{};
+    if (check_prefix(a, pass, p) != B200_OK || max_length <= 0 || max_prefix < 0) return 0;
+    const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
+    return static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * (a->cache.head_dim + 2) * sizeof(float) + 256;
+}
+
+extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch, size_t scratch_bytes,
+                                     float* out, void* out_hi, void* out_lo, int64_t out_stride, void* stream) {
+    PrefixParams p{};
+    const int checked = check_prefix(a, pass, p);
+    if (checked != B200_OK) return checked;
+    const int64_t width = static_cast<int64_t>(a->heads) * a->cache.head_dim;
+    if ((!out && !out_hi) || (out_lo && !out_hi) || max_length <= 0 || max_prefix < 0 || (out_stride && out_stride < width)) {
+        set_error("b200_prefix_attention: bad result, stride or length");
+        return B200_BAD_ARGUMENT;
+    }
+    const size_t need = b200_prefix_scratch_bytes(a, pass, max_length, max_prefix);
+    if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16) {
+        set_error("b200_prefix_attention: scratch of %zu bytes on a 16-byte boundary needed, %zu given", need, scratch_bytes);
+        return B200_BAD_ARGUMENT;
+    }
+    const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
+    p.heads = a->heads; p.group = a->heads / a->cache.kv_heads; p.dim = a->cache.head_dim;
+    p.groups = plan.prefix_splits ? a->groups : 0;
+    p.group_first = a->group_first; p.group_prefix = a->group_prefix; p.prefix_length = a->prefix_length;
+    p.query = a->query;
+    p.scale = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
+    p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits; p.prefix_tiles = plan.prefix_tiles; p.own_tiles = plan.own_tiles;
+    p.part_o = static_cast<float*>(scratch);
+    p.part_ml = p.part_o + static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * p.dim;
+    p.out = out; p.out_hi = static_cast<__nv_bfloat16*>(out_hi); p.out_lo = static_cast<__nv_bfloat16*>(out_lo);
+    p.out_stride = out_stride ? out_stride : width;
+    const int64_t items = (static_cast<int64_t>(plan.prefix_tiles) * plan.prefix_splits + static_cast<int64_t>(pass->sequences) * plan.own_tiles * plan.own_splits)
+                          * a->cache.kv_heads;
+    const int64_t merges = (pass->rows * a->heads + 3) / 4;
+    if (items > INT32_MAX || merges > INT32_MAX || static_cast<int64_t>(pass->rows) * p.group > INT32_MAX / 2) {
+        set_error("b200_prefix_attention: too many rows");
+        return B200_UNSUPPORTED;
+    }
+    cudaStream_t s = as_stream(stream);
+    cudaError_t launched;
+    if (plan.form == Form::plain)
+        launched = a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, static_cast<unsigned>(items), s) : launch_plain<float>(p, static_cast<unsigned>(items), s);
+    else if (p.dim <= 64) launched = launch_mma<64>(p, plan.form == Form::mma_split, static_cast<unsigned>(items), s);
+    else if (p.dim <= 96) launched = launch_mma<96>(p, plan.form == Form::mma_split, static_cast<unsigned>(items), s);
+    else launched = launch_mma<128>(p, plan.form == Form::mma_split, static_cast<unsigned>(items), s);
+    const int status = cuda_status(launched, "b200_prefix_attention launch");
+    if (status != B200_OK) return status;
+    return cuda_status(launch_dependent(prefix_merge_kernel, dim3(static_cast<unsigned>(merges)), dim3(128), 0, s, p), "prefix_merge_kernel launch");
+}

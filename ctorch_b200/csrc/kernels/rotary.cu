@@ -1,0 +1,208 @@
+// Rotary positions: tables of cosines and sines, scaled for long contexts, and the rotation of the queries and keys of a packed pass with
+// the append of its keys and values to paged caches.
+#include "paged.cuh"
+#include "rows.cuh"
+
+#include <cmath>
+
+namespace b200 {
+
+bool pages_view(const b200_kv_pages& p, const char* who, PagesView& view) {
+    if ((p.dtype != B200_F32 && p.dtype != B200_BF16) || p.kv_heads <= 0 || p.head_dim <= 0 || p.page_size <= 0 || p.sequences <= 0 || p.pages_per_sequence <= 0
+        || p.pages <= 0 || p.pages > INT32_MAX || !p.key || !p.value || !p.table || static_cast<int64_t>(p.pages_per_sequence) * p.page_size > INT32_MAX / 2) {
+        set_error("%s: inconsistent pages (b200_kv_pages)", who);
+        return false;
+    }
+    view = PagesView{{p.key, p.value}, p.table, p.pages, p.sequences, p.pages_per_sequence, p.page_size, p.kv_heads, p.head_dim, p.dtype};
+    return true;
+}
+
+namespace {
+
+// ---- tables -----------------------------------------------------------------------------------------------------------------------------
+struct TableParams {
+    double log_base, factor, original, low, high, magnitude;
+    int kind, half, run;
+    int64_t first, positions;
+    float *cosine, *sine;
+};
+
+// A thread owns one frequency and `run` consecutive positions.
+__global__ void __launch_bounds__(256) rotary_tables_kernel(const TableParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int64_t at = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+    const int i = static_cast<int>(at % p.half);
+    const int64_t begin = at / p.half * p.run, end = min(begin + p.run, p.positions);
+    if (begin >= end) return;
+    double frequency = exp(-static_cast<double>(i) / p.half * p.log_base);
+    if (p.kind == B200_ROTARY_LINEAR) frequency /= p.factor;
+    if (p.kind == B200_ROTARY_PARTS) {
+        const double turns = p.original * frequency * 0.15915494309189535;
+        const double kept = fmin(1.0, fmax(0.0, (turns - p.low) / (p.high - p.low)));
+        frequency *= kept + (1.0 - kept) / p.factor;
+    }
+    for (int64_t q = begin; q < end; ++q) {
+        double s, c;
+        sincos(static_cast<double>(p.first + q) * frequency, &s, &c);
+        p.cosine[q * p.half + i] = static_cast<float>(p.magnitude * c);
+        p.sine[q * p.half + i] = static_cast<float>(p.magnitude * s);
+    }
+}
+
+// ---- rotation and append ----------------------------------------------------------------------------------------------------------------
+struct AppendParams {
+    RowsView rows;
+    PagesView cache;
+    int heads, rot, pairs, positions;
+    const float *cosine, *sine, *projected;
+    const int32_t* offset;
+    int64_t stride;
+    int query_bf16;
+    void* query;
+};
+
+template <int V> __device__ __forceinline__ void store_values(void* base, int bf16, int64_t at, const Lanes<V>& v) {
+    if (!bf16) {
+        store_lanes<V>(static_cast<float*>(base) + at, v);
+    } else if constexpr (V == 4) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.v[0], v.v[1]), b = __floats2bfloat162_rn(v.v[2], v.v[3]);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(base) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(v.v[0]);
+    }
+}
+
+// An item is 2 V values of one head of one row: entries d .. d + V - 1 and e .. e + V - 1, which turn together in the rotating part.  grid
+// (rows, blocks of items).
+template <int V> __global__ void __launch_bounds__(256) rotary_append_kernel(const AppendParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int row = blockIdx.x;
+    if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
+    const int dim = p.cache.head_dim, per_head = dim / (2 * V), kv_heads = p.cache.kv_heads;
+    const int items = (p.heads + 2 * kv_heads) * per_head;
+    const RowPlace place = row_place(p.rows, row);
+    const int64_t turn = static_cast<int64_t>(place.position) + (p.offset ? __ldg(p.offset + place.sequence) : 0);
+    const bool turns = p.rot > 0 && turn >= 0 && turn < p.positions;
+    int page = -1, entry = 0;
+    if (place.slot >= 0 && place.slot < p.cache.sequences && place.position >= 0 && place.position < p.cache.capacity()) {
+        page = page_of(p.cache, place.slot, place.position / p.cache.page_size);
+        entry = place.position % p.cache.page_size;
+    }
+    const float* source = p.projected + row * p.stride;
+    const int half = p.rot / 2;
+    const float* cosine = p.cosine + turn * half;
+    const float* sine = p.sine + turn * half;
+    for (int item = blockIdx.y * blockDim.x + threadIdx.x; item < items; item += gridDim.y * blockDim.x) {
+        const int head = item / per_head, j = item % per_head;
+        const bool rotates = turns && head < p.heads + kv_heads && j * 2 * V < p.rot;
+        int d, e;
+        if (!p.pairs && j * 2 * V < p.rot) {
+            d = j * V;
+            e = d + half;
+        } else {
+            d = j * 2 * V;
+            e = d + V;
+        }
+        Lanes<V> a = load_lanes<V>(source + head * dim + d), b = load_lanes<V>(source + head * dim + e);
+        if (rotates) {
+            if (!p.pairs) {
+                const Lanes<V> c = load_lanes<V>(cosine + d), s = load_lanes<V>(sine + d);
+#pragma unroll
+                for (int u = 0; u < V; ++u) {
+                    const float x = a.v[u], y = b.v[u];
+                    a.v[u] = x * c.v[u] - y * s.v[u];
+                    b.v[u] = y * c.v[u] + x * s.v[u];
+                }
+            } else if constexpr (V == 4) {
+                const Lanes<4> c = load_lanes<4>(cosine + d / 2), s = load_lanes<4>(sine + d / 2);
+                const float x[4] = {a.v[0], a.v[2], b.v[0], b.v[2]}, y[4] = {a.v[1], a.v[3], b.v[1], b.v[3]};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    Lanes<4>& to = u < 2 ? a : b;
+                    to.v[(u & 1) * 2] = x[u] * c.v[u] - y[u] * s.v[u];
+                    to.v[(u & 1) * 2 + 1] = y[u] * c.v[u] + x[u] * s.v[u];
+                }
+            } else {
+                const float c = cosine[d / 2], s = sine[d / 2], x = a.v[0], y = b.v[0];
+                a.v[0] = x * c - y * s;
+                b.v[0] = y * c + x * s;
+            }
+        }
+        if (head < p.heads) {
+            const int64_t at = (static_cast<int64_t>(row) * p.heads + head) * dim;
+            store_values<V>(p.query, p.query_bf16, at + d, a);
+            store_values<V>(p.query, p.query_bf16, at + e, b);
+        } else if (page >= 0) {
+            const bool value = head >= p.heads + kv_heads;
+            const int64_t at = page_row(p.cache, page, head - p.heads - (value ? kv_heads : 0), entry);
+            store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + d, a);
+            store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + e, b);
+        }
+    }
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_rotary_tables(const b200_rotary_scaling* s, int32_t rot_dims, int64_t first, int64_t positions, float* cosine, float* sine, void* stream) {
+    if (!s || !cosine || !sine || rot_dims <= 0 || (rot_dims & 1) || first < 0 || positions < 0 || first > (int64_t{1} << 52) || positions > (int64_t{1} << 31)
+        || s->kind < B200_ROTARY_PLAIN || s->kind > B200_ROTARY_PARTS || !(s->base > 0.0) || !std::isfinite(s->base) || !std::isfinite(s->magnitude)) {
+        set_error("b200_rotary_tables: bad pointer, size, kind or base");
+        return B200_BAD_ARGUMENT;
+    }
+    if (s->kind != B200_ROTARY_PLAIN && (!(s->factor > 0.0) || !std::isfinite(s->factor))) {
+        set_error("b200_rotary_tables: the factor must be positive");
+        return B200_BAD_ARGUMENT;
+    }
+    if (s->kind == B200_ROTARY_PARTS && !(s->original > 0.0 && s->low < s->high && std::isfinite(s->original) && std::isfinite(s->low) && std::isfinite(s->high))) {
+        set_error("b200_rotary_tables: scaling by parts needs original > 0 and low < high");
+        return B200_BAD_ARGUMENT;
+    }
+    if (positions == 0) return B200_OK;
+    TableParams p{};
+    p.log_base = std::log(s->base);
+    // two entries have one frequency, f_0 = 1, whatever the base
+    if (s->kind == B200_ROTARY_BASE && rot_dims > 2) p.log_base += std::log(s->factor) * rot_dims / (rot_dims - 2);
+    p.factor = s->factor; p.original = s->original; p.low = s->low; p.high = s->high;
+    p.magnitude = s->magnitude == 0.0 ? 1.0 : s->magnitude;
+    p.kind = s->kind; p.half = rot_dims / 2; p.run = 8;
+    p.first = first; p.positions = positions; p.cosine = cosine; p.sine = sine;
+    const int64_t threads = (positions + p.run - 1) / p.run * p.half;
+    if ((threads + 255) / 256 > INT32_MAX) { set_error("b200_rotary_tables: the tables are too large"); return B200_UNSUPPORTED; }
+    return cuda_status(launch_dependent(rotary_tables_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, as_stream(stream), p),
+                       "rotary_tables_kernel launch");
+}
+
+extern "C" int b200_rotary_append(const b200_rotary_append_args* a, const b200_rows* pass, void* stream) {
+    AppendParams p{};
+    if (!rows_view(pass, p.rows)) return B200_BAD_ARGUMENT;
+    if (!a) { set_error("b200_rotary_append: no arguments"); return B200_BAD_ARGUMENT; }
+    if (!pages_view(a->cache, "b200_rotary_append", p.cache)) return B200_BAD_ARGUMENT;
+    const int dim = a->cache.head_dim;
+    const int64_t width = (static_cast<int64_t>(a->heads) + 2 * a->cache.kv_heads) * dim;
+    const int64_t stride = a->stride ? a->stride : width;
+    if (a->heads <= 0 || (dim & 1) || a->rot_dims < 0 || (a->rot_dims & 1) || a->rot_dims > dim || !a->projected || !a->query || stride < width
+        || width > INT32_MAX || (a->query_dtype != B200_F32 && a->query_dtype != B200_BF16)
+        || (a->rot_dims > 0 && (!a->cosine || !a->sine || a->positions <= 0))) {
+        set_error("b200_rotary_append: bad pointer, size or dtype");
+        return B200_BAD_ARGUMENT;
+    }
+    p.heads = a->heads; p.rot = a->rot_dims; p.pairs = a->rotate_pairs != 0; p.positions = a->positions;
+    p.cosine = a->cosine; p.sine = a->sine; p.projected = a->projected; p.offset = a->offset; p.stride = stride;
+    p.query_bf16 = a->query_dtype == B200_BF16; p.query = a->query;
+    // four values per access where every address allows it
+    uintptr_t bits = reinterpret_cast<uintptr_t>(a->projected) | reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->cache.key)
+                     | reinterpret_cast<uintptr_t>(a->cache.value);
+    if (a->rot_dims) bits |= reinterpret_cast<uintptr_t>(a->cosine) | reinterpret_cast<uintptr_t>(a->sine);
+    const bool wide = dim % 8 == 0 && a->rot_dims % 8 == 0 && stride % 4 == 0 && bits % 16 == 0;
+    const int64_t items = width / (wide ? 8 : 2);
+    const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>((items + 255) / 256 < 65535 ? (items + 255) / 256 : 65535));
+    return cuda_status(wide ? launch_dependent(rotary_append_kernel<4>, grid, dim3(256), 0, as_stream(stream), p)
+                            : launch_dependent(rotary_append_kernel<1>, grid, dim3(256), 0, as_stream(stream), p),
+                       "rotary_append_kernel launch");
+}

@@ -1,0 +1,501 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Two launches.  verify_rows_kernel: for every row of target and draft logits the maximum and the sum of its weights exp((x - max) / T); a row is
+// split over a cluster of CTAs that hold their part in registers, so the row is read once although the weights need the maximum first.
+// verify_finish_kernel: one cluster per sequence walks the acceptance tests, then draws from the residual of the row that refused: running sums
+// over segments of 128 values, in index order.  All sums are f64 and added in a fixed order, so the choice does not depend on the launch.
+#include "linear_common.cuh"
+#include "rows.cuh"
+
+#include <cmath>
+
+namespace b200 {
+namespace {
+
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kHeld = 16;                                    // 16-byte vectors of a row that a thread keeps in registers
+constexpr int kVerifyMostParts = 8;
+
+struct VerifyParams {
+    RowsView rows;
+    const float *logits, *draft;
+    int64_t stride;
+    int vocab, parts, chunk;      // CTAs per row, values per CTA (a multiple of 4)
+    float inverse;
+    const int64_t* ids;
+    const double *accept, *draw;
+    int32_t* accepted;
+    int64_t* next;
+    int advance;
+    float* row_max;               // [2 * rows]: target and draft of each row
+    double* row_sum;              // [2 * rows][parts]
+    Candidate* best;              // greedy: [rows][parts]
+};
+
+__device__ __forceinline__ float weight_of(float x, float most, float inverse) { return expf(__fmul_rn(__fsub_rn(x, most), inverse)); }
+
+// One CTA's part of a row, in vectors of four values on 16-byte boundaries: vector v holds the values 4 v - shift .. + 3 of the part.
+struct RowPart {
+    const float* base;
+    int length, shift, vectors;
+    __device__ __forceinline__ RowPart(const VerifyParams& p, const float* row, int part) {
+        const int begin = min(p.vocab, part * p.chunk);
+        base = row + begin;
+        length = min(p.vocab, begin + p.chunk) - begin;
+        shift = static_cast<int>((reinterpret_cast<uintptr_t>(base) >> 2) & 3);
+        vectors = length > 0 ? (length + shift + 3) / 4 : 0;
+    }
+    // Values of vector v as seen with `by` in the place of the own shift; outside the part -inf, the value without weight.
+    __device__ __forceinline__ float4 load(int v, int by) const {
+        const int at = 4 * v - by;
+        if (by == shift && at >= 0 && at + 4 <= length) return __ldcs(reinterpret_cast<const float4*>(base + at));
+        float r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r[u] = at + u >= 0 && at + u < length ? __ldcs(base + at + u) : -INFINITY;
+        return make_float4(r[0], r[1], r[2], r[3]);
+    }
+    __device__ __forceinline__ float4 load(int v) const { return load(v, shift); }
+};
+
+__device__ __forceinline__ int cluster_part() {
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    return static_cast<int>(rank);
+}
+__device__ __forceinline__ double load_cluster_double(uint32_t address) {
+    double value;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(value) : "r"(address) : "memory");
+    return value;
+}
+
+// grid: clusters of `parts` CTAs, two (target, draft) or one per row.
+template <bool GREEDY> __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const VerifyParams p) {
+    __shared__ float warp_max_of[kVerifyWarps];
+    __shared__ double warp_sum_of[kVerifyWarps];
+    __shared__ Candidate warp_best[kVerifyWarps];
+    __shared__ float part_max;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int part = cluster_part(), unit = blockIdx.x / p.parts;
+    const int sides = p.draft && !GREEDY ? 2 : 1;
+    const int row = unit / sides, side = unit % sides;
+    // (the whole cluster leaves together)
+    if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
+    if (side == 1 && row + 1 == __ldg(p.rows.first + __ldg(p.rows.sequence + row) + 1)) return;
+    const RowPart own(p, (side ? p.draft : p.logits) + row * p.stride, part);
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    const int tiles = max(1, (own.vectors + kVerifyThreads * kHeld - 1) / (kVerifyThreads * kHeld));
+    float4 held[kHeld];
+    if constexpr (GREEDY) {
+        Candidate best{-INFINITY, INT32_MAX};
+        for (int t = 0; t < tiles; ++t) {
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                const int v = (t * kHeld + j) * kVerifyThreads + thread;
+                held[j] = v < own.vectors ? own.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            }
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                const int at = 4 * ((t * kHeld + j) * kVerifyThreads + thread) - own.shift;
+                const float x[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const Candidate other{x[u], part * p.chunk + at + u};
+                    if (at + u >= 0 && at + u < own.length && preferred(other, best)) best = other;
+                }
+            }
+        }
+        for (int o = 16; o > 0; o >>= 1) {
+            const Candidate other{__shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.index, o)};
+            if (preferred(other, best)) best = other;
+        }
+        if (lane == 0) warp_best[warp] = best;
+        __syncthreads();
+        if (thread == 0) {
+            for (int w = 1; w < kVerifyWarps; ++w)
+                if (preferred(warp_best[w], best)) best = warp_best[w];
+            p.best[static_cast<int64_t>(row) * p.parts + part] = best;
+        }
+        return;
+    }
+    float most = -INFINITY;
+    for (int t = tiles - 1; t >= 0; --t) {   // the first tile stays in the registers
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int v = (t * kHeld + j) * kVerifyThreads + thread;
+            held[j] = v < own.vectors ? own.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) most = fmaxf(most, fmaxf(fmaxf(held[j].x, held[j].y), fmaxf(held[j].z, held[j].w)));
+    }
+    most = warp_max(most);
+    if (lane == 0) warp_max_of[warp] = most;
+    __syncthreads();
+    if (thread == 0) {
+        for (int w = 1; w < kVerifyWarps; ++w) most = fmaxf(most, warp_max_of[w]);
+        part_max = most;
+    }
+    cluster_sync_all();
+    most = -INFINITY;
+    for (int c = 0; c < p.parts; ++c) most = fmaxf(most, load_cluster_float(map_peer_shared(smem_u32(&part_max), static_cast<uint32_t>(c))));
+    double sum = 0.0;
+    for (int t = 0; t < tiles; ++t) {
+        if (t > 0) {
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                const int v = (t * kHeld + j) * kVerifyThreads + thread;
+                held[j] = v < own.vectors ? own.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            if ((t * kHeld + j) * kVerifyThreads >= own.vectors) break;
+            sum += static_cast<double>(weight_of(held[j].x, most, p.inverse));
+            sum += static_cast<double>(weight_of(held[j].y, most, p.inverse));
+            sum += static_cast<double>(weight_of(held[j].z, most, p.inverse));
+            sum += static_cast<double>(weight_of(held[j].w, most, p.inverse));
+        }
+    }
+    // values outside the part weigh nothing; where the row's maximum is itself -inf every weight is NaN, as for the values inside
+    sum = warp_sum(sum);
+    if (lane == 0) warp_sum_of[warp] = sum;
+    __syncthreads();
+    if (thread == 0) {
+        sum = 0.0;
+        for (int w = 0; w < kVerifyWarps; ++w) sum += warp_sum_of[w];
+        const int64_t at = 2 * static_cast<int64_t>(row) + side;
+        p.row_sum[at * p.parts + part] = sum;
+        if (part == 0) p.row_max[at] = most;
+    }
+    cluster_sync_all();   // the peers have read this CTA's maximum
+}
+
+struct RowStats {
+    float most;
+    double sum;
+    bool good;   // there are finite weights
+};
+__device__ __forceinline__ RowStats row_stats(const VerifyParams& p, int row, int side) {
+    const int64_t at = 2 * static_cast<int64_t>(row) + side;
+    RowStats r{p.row_max[at], 0.0, false};
+    for (int c = 0; c < p.parts; ++c) r.sum += p.row_sum[at * p.parts + c];
+    r.good = r.sum > 0.0 && r.sum < INFINITY;
+    return r;
+}
+
+// What is left of a value's probability: the target's share less the draft's.
+struct Residual {
+    float most, draft_most, inverse;
+    double scale, draft_scale;   // one over the sums
+    int without;                 // the draft that counts as certain, or -1
+    bool minus;                  // the draft's probabilities are taken off
+    __device__ __forceinline__ double value(float x, float y, int index) const {
+        double left = static_cast<double>(weight_of(x, most, inverse)) * scale;
+        if (minus) left -= static_cast<double>(weight_of(y, draft_most, inverse)) * draft_scale;
+        return index == without || !(left > 0.0) ? 0.0 : left;
+    }
+};
+
+// grid: a cluster of `parts` CTAs per sequence.  Dynamic shared memory: the sums of the part's segments of 128 values.
+__global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const VerifyParams p) {
+    extern __shared__ double segment_sum[];
+    __shared__ int stop_row;
+    __shared__ double part_total;
+    __shared__ Candidate warp_best[kVerifyWarps];
+    __shared__ Candidate part_best;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int part = cluster_part(), s = blockIdx.x / p.parts;
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    const int first = __ldg(p.rows.first + s), last = __ldg(p.rows.first + s + 1) - 1;
+    if (last < first) {
+        if (part == 0 && thread == 0) {
+            p.accepted[s] = 0;
+            p.next[s] = -1;
+        }
+        return;
+    }
+    // the first draft that is refused, else the last row
+    if (warp == 0) {
+        int stop = last;
+        for (int base = first; base < last; base += 32) {
+            const int row = base + lane;
+            bool refused = false;
+            if (row < last) {
+                const int64_t x = __ldg(p.ids + row + 1);
+                refused = true;
+                if (x >= 0 && x < p.vocab) {
+                    const RowStats t = row_stats(p, row, 0);
+                    double q = 1.0;
+                    if (p.draft) {
+                        const RowStats d = row_stats(p, row, 1);
+                        q = d.good ? static_cast<double>(weight_of(p.draft[row * p.stride + x], d.most, p.inverse)) / d.sum : NAN;
+                    }
+                    const double share = t.good ? static_cast<double>(weight_of(p.logits[row * p.stride + x], t.most, p.inverse)) / t.sum : NAN;
+                    refused = !(p.accept[row] * q < share);
+                }
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, refused);
+            if (found) {
+                stop = base + __ffs(found) - 1;
+                break;
+            }
+        }
+        if (lane == 0) stop_row = stop;
+    }
+    __syncthreads();
+    const int row = stop_row;
+    const RowStats stats = row_stats(p, row, 0);
+    Residual residual{stats.most, 0.0f, p.inverse, 1.0 / stats.sum, 0.0, -1, false};
+    if (row < last) {
+        const int64_t x = __ldg(p.ids + row + 1);
+        if (x >= 0 && x < p.vocab) {
+            if (p.draft) {
+                const RowStats d = row_stats(p, row, 1);
+                residual.minus = d.good;
+                residual.draft_most = d.most;
+                residual.draft_scale = 1.0 / d.sum;
+            } else {
+                residual.without = static_cast<int>(x);
+            }
+        }
+    }
+    const RowPart target(p, p.logits + row * p.stride, part);
+    const RowPart draft(p, (p.draft ? p.draft : p.logits) + row * p.stride, part);
+    const int begin = part * p.chunk;
+    if (!stats.good) {   // no distribution: the argmax, as b200_argmax has it
+        Candidate best{-INFINITY, INT32_MAX};
+        for (int i = thread; i < target.length; i += kVerifyThreads) {
+            const Candidate other{target.base[i], begin + i};
+            if (preferred(other, best)) best = other;
+        }
+        for (int o = 16; o > 0; o >>= 1) {
+            const Candidate other{__shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.index, o)};
+            if (preferred(other, best)) best = other;
+        }
+        if (lane == 0) warp_best[warp] = best;
+        __syncthreads();
+        if (thread == 0) {
+            for (int w = 1; w < kVerifyWarps; ++w)
+                if (preferred(warp_best[w], best)) best = warp_best[w];
+            part_best = best;
+        }
+        cluster_sync_all();
+        if (part == 0 && thread == 0) {
+            for (int c = 1; c < p.parts; ++c) {
+                const float2 raw = load_cluster_float2(map_peer_shared(smem_u32(&part_best), static_cast<uint32_t>(c)));
+                const Candidate other{raw.x, __float_as_int(raw.y)};
+                if (preferred(other, best)) best = other;
+            }
+            p.next[s] = best.index;
+        }
+        cluster_sync_all();
+    } else {
+        const int segments = (target.vectors + 31) / 32;
+        const int run = (segments + 31) / 32;   // segments that a lane of the first warp adds up
+        double total, before, lane_before, mine;
+        while (true) {
+            for (int g = warp; g < segments; g += kVerifyWarps) {
+                const int v = g * 32 + lane, at = begin + 4 * v - target.shift;
+                double sum = 0.0;
+                if (v < target.vectors) {
+                    const float4 x = target.load(v), y = residual.minus ? draft.load(v, target.shift) : x;
+                    sum = residual.value(x.x, y.x, at);
+                    sum += residual.value(x.y, y.y, at + 1);
+                    sum += residual.value(x.z, y.z, at + 2);
+                    sum += residual.value(x.w, y.w, at + 3);
+                }
+                sum = warp_sum(sum);
+                if (lane == 0) segment_sum[g] = sum;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                mine = 0.0;
+                for (int g = lane * run; g < min(segments, (lane + 1) * run); ++g) mine += segment_sum[g];
+                double up_to = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double other = __shfl_up_sync(0xffffffffu, up_to, o);
+                    if (lane >= o) up_to += other;
+                }
+                const double below = __shfl_up_sync(0xffffffffu, up_to, 1);
+                lane_before = lane ? below : 0.0;
+                if (lane == 31) part_total = up_to;
+            }
+            cluster_sync_all();
+            total = before = 0.0;
+            for (int c = 0; c < p.parts; ++c) {
+                if (c == part) before = total;
+                total += load_cluster_double(map_peer_shared(smem_u32(&part_total), static_cast<uint32_t>(c)));
+            }
+            if (total > 0.0 || (!residual.minus && residual.without < 0)) break;
+            // nothing is left by rounding: the target's own distribution (every CTA of the cluster comes to this together)
+            residual.minus = false;
+            residual.without = -1;
+            cluster_sync_all();
+        }
+        const double wanted = p.draw[s] * total;
+        // the first part whose running sum exceeds what is wanted; by rounding there may be none, then the last with any weight
+        int chosen = -1, heavy = 0;
+        double running = 0.0;
+        for (int c = 0; c < p.parts; ++c) {
+            const double here = load_cluster_double(map_peer_shared(smem_u32(&part_total), static_cast<uint32_t>(c)));
+            running += here;
+            if (here > 0.0) heavy = c;
+            if (chosen < 0 && here > 0.0 && running > wanted) chosen = c;
+        }
+        if (chosen < 0) chosen = heavy;
+        if (chosen == part && warp == 0) {
+            // the same among the segments, then among the segment's values
+            double sum = before + lane_before;
+            int segment = -1, some = -1;
+            for (int g = lane * run; g < min(segments, (lane + 1) * run); ++g) {
+                if (segment_sum[g] > 0.0) some = g;
+                if (segment_sum[g] > 0.0 && sum + segment_sum[g] > wanted) {
+                    segment = g;
+                    break;
+                }
+                sum += segment_sum[g];
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, segment >= 0);
+            if (found) {
+                const int from = __ffs(found) - 1;
+                segment = __shfl_sync(0xffffffffu, segment, from);
+                sum = __shfl_sync(0xffffffffu, sum, from);
+            } else {
+                segment = warp_max_int(some);
+                sum = -INFINITY;
+            }
+            const int v = segment * 32 + lane, at = begin + 4 * v - target.shift;
+            double left[4] = {0.0, 0.0, 0.0, 0.0};
+            if (v < target.vectors) {
+                const float4 x = target.load(v), y = residual.minus ? draft.load(v, target.shift) : x;
+                left[0] = residual.value(x.x, y.x, at);
+                left[1] = residual.value(x.y, y.y, at + 1);
+                left[2] = residual.value(x.z, y.z, at + 2);
+                left[3] = residual.value(x.w, y.w, at + 3);
+            }
+            double up_to = left[0] + left[1] + left[2] + left[3];
+            const double four = up_to;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double other = __shfl_up_sync(0xffffffffu, up_to, o);
+                if (lane >= o) up_to += other;
+            }
+            sum += up_to - four;
+            int index = -1, any = -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                sum += left[u];
+                if (left[u] > 0.0) {
+                    any = at + u;
+                    if (index < 0 && sum > wanted) index = at + u;
+                }
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, index >= 0);
+            index = hit ? __shfl_sync(0xffffffffu, index, __ffs(hit) - 1) : warp_max_int(any);
+            if (lane == 0) p.next[s] = index;
+        }
+        cluster_sync_all();   // the peers have read this CTA's total
+    }
+    if (part == 0 && thread == 0) {
+        p.accepted[s] = row - first;
+        if (p.advance) atomicAdd(p.rows.lengths + __ldg(p.rows.slot + s), row - first + 1);
+    }
+}
+
+// Temperature 0: a warp per sequence.
+__global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (s >= p.rows.sequences) return;
+    const int first = __ldg(p.rows.first + s), last = __ldg(p.rows.first + s + 1) - 1;
+    int stop = last, token = -1;
+    for (int base = first; base <= last; base += 32) {
+        const int row = base + lane;
+        Candidate best{-INFINITY, INT32_MAX};
+        if (row <= last)
+            for (int c = 0; c < p.parts; ++c) {
+                const Candidate other = p.best[static_cast<int64_t>(row) * p.parts + c];
+                if (preferred(other, best)) best = other;
+            }
+        const bool stops = row == last || (row < last && __ldg(p.ids + row + 1) != best.index);
+        const unsigned found = __ballot_sync(0xffffffffu, stops);
+        if (found) {
+            const int from = __ffs(found) - 1;
+            stop = base + from;
+            token = __shfl_sync(0xffffffffu, best.index, from);
+            break;
+        }
+    }
+    if (lane == 0) {
+        p.accepted[s] = last < first ? 0 : stop - first;
+        p.next[s] = token;
+        if (p.advance && last >= first) atomicAdd(p.rows.lengths + __ldg(p.rows.slot + s), stop - first + 1);
+    }
+}
+
+// CTAs per row: a CTA keeps its part of a row in registers.
+int verify_parts(int64_t vocab) {
+    int parts = 1;
+    while (parts < kVerifyMostParts && vocab > static_cast<int64_t>(parts) * 4096) parts *= 2;
+    return parts;
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" size_t b200_verify_scratch_bytes(const b200_verify_args* a, const b200_rows* pass) {
+    if (!a || !pass || pass->rows <= 0 || a->vocab <= 0) return 0;
+    const size_t units = 2 * static_cast<size_t>(pass->rows);
+    return units * kVerifyMostParts * sizeof(double) + units * sizeof(float) + 256;
+}
+
+extern "C" int b200_verify_drafts(const b200_verify_args* a, const b200_rows* pass, void* scratch, size_t scratch_bytes, void* stream) {
+    VerifyParams p{};
+    if (!rows_view(pass, p.rows)) return B200_BAD_ARGUMENT;
+    if (!a || !a->logits || !a->ids || !a->accepted || !a->next || a->vocab <= 0 || !std::isfinite(a->temperature) || a->temperature < 0.0
+        || (a->stride && a->stride < a->vocab) || (a->temperature > 0.0 && (!a->accept || !a->draw))) {
+        set_error("b200_verify_drafts: bad pointer, size or temperature");
+        return B200_BAD_ARGUMENT;
+    }
+    const float inverse = a->temperature > 0.0 ? static_cast<float>(1.0 / a->temperature) : 1.0f;
+    if (!std::isfinite(inverse) || inverse == 0.0f) { set_error("b200_verify_drafts: temperature %g is out of range", a->temperature); return B200_BAD_ARGUMENT; }
+    if (a->vocab > (1 << 23)) { set_error("b200_verify_drafts: more than 2^23 values per row are not supported"); return B200_UNSUPPORTED; }
+    const size_t need = b200_verify_scratch_bytes(a, pass);
+    if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 8) {
+        set_error("b200_verify_drafts: scratch of %zu bytes on an 8-byte boundary needed, %zu given", need, scratch_bytes);
+        return B200_BAD_ARGUMENT;
+    }
+    const bool greedy = a->temperature == 0.0;
+    p.logits = a->logits; p.draft = greedy ? nullptr : a->draft_logits; p.stride = a->stride ? a->stride : a->vocab;
+    p.vocab = static_cast<int>(a->vocab); p.parts = verify_parts(a->vocab);
+    p.chunk = ((p.vocab + p.parts - 1) / p.parts + 3) / 4 * 4;
+    p.inverse = inverse; p.ids = a->ids; p.accept = a->accept; p.draw = a->draw; p.accepted = a->accepted; p.next = a->next; p.advance = a->advance != 0;
+    const size_t units = 2 * static_cast<size_t>(p.rows.rows);
+    p.row_sum = static_cast<double*>(scratch);
+    p.best = static_cast<Candidate*>(scratch);
+    p.row_max = reinterpret_cast<float*>(p.row_sum + units * kVerifyMostParts);
+    cudaStream_t st = as_stream(stream);
+    const int64_t ctas = static_cast<int64_t>(p.rows.rows) * (p.draft ? 2 : 1) * p.parts;
+    if (ctas > INT32_MAX) { set_error("b200_verify_drafts: too many rows"); return B200_UNSUPPORTED; }
+    const dim3 cluster(static_cast<unsigned>(p.parts), 1, 1);
+    if (greedy) {
+        int status = cuda_status(launch_dependent_cluster(verify_rows_kernel<true>, dim3(static_cast<unsigned>(ctas)), dim3(kVerifyThreads), 0, st, cluster, p),
+                                 "verify_rows_kernel launch");
+        if (status != B200_OK) return status;
+        return cuda_status(launch_dependent(verify_greedy_kernel, dim3(static_cast<unsigned>((p.rows.sequences + 3) / 4)), dim3(128), 0, st, p),
+                           "verify_greedy_kernel launch");
+    }
+    const int status = cuda_status(launch_dependent_cluster(verify_rows_kernel<false>, dim3(static_cast<unsigned>(ctas)), dim3(kVerifyThreads), 0, st, cluster, p),
+                                   "verify_rows_kernel launch");
+    if (status != B200_OK) return status;
+    const size_t smem = static_cast<size_t>((p.chunk + 3) / 4 + 1 + 31) / 32 * sizeof(double);
+    if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(verify_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    return cuda_status(launch_dependent_cluster(verify_finish_kernel, dim3(static_cast<unsigned>(p.rows.sequences * p.parts)), dim3(kVerifyThreads), smem, st, cluster, p),
+                       "verify_finish_kernel launch");
+}

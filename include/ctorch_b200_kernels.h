@@ -615,6 +615,113 @@ B200_API int b200_experts_grouped(const b200_experts* args, const int32_t* rank,
 /* Whether b200_experts_grouped takes these sizes, and whether it is the faster form. */
 B200_API int32_t b200_experts_takes_grouped(const b200_experts* args);
 
+/* ---- drafted tokens behind a shared prompt -------------------------------------------------------------------------------
+ * (no counterpart in the reference)
+ *
+ * What a server needs that answers many packed sequences (b200_rows) over one or a few long prompts, with tokens drafted ahead: a view of
+ * paged keys and values that several sequences may share pages of, the rotation that is applied while rows are appended, attention that
+ * reads a shared prompt once for all its sequences, and the verification of the drafts.  Rows behind the last sequence (from
+ * first[sequences] on, as in a pass of fixed size that is not full) are left as they were. */
+
+/* Paged keys and values in the caller's memory, or those of a cache (b200_kv_cache_pages): pools [pages][kv_heads][page_size][head_dim] and a
+ * table of page numbers in device memory.  A page may stand in several places of one table and in several tables.  A table entry outside
+ * [0, pages) is a page of zeros that nothing is written to. */
+typedef struct b200_kv_pages {
+    int32_t dtype, kv_heads, head_dim, page_size;
+    int32_t sequences, pages_per_sequence;
+    int64_t pages;                 /* in each pool */
+    void* key;
+    void* value;
+    const int32_t* table;          /* [sequences][pages_per_sequence] */
+} b200_kv_pages;
+B200_API int b200_kv_cache_pages(const b200_kv_cache* cache, b200_kv_pages* out);
+
+/* Cosines and sines of the positions first .. first + positions - 1, f32 [positions][rot_dims / 2], from angles in f64: magnitude *
+ * cos(position * f_i), i < rot_dims / 2.  PLAIN: f_i = base^(-2 i / rot_dims).  LINEAR: f_i / factor.  BASE: base * factor^(rot_dims /
+ * (rot_dims - 2)) in place of base, which leaves f_0 and divides the last f_i by the factor.  PARTS: with turns = original * f_i / (2 pi), the
+ * turns that entry i makes in the `original` positions of the training, f_i stays where turns >= high, becomes f_i / factor where turns <=
+ * low, and is mixed linearly in between. */
+enum b200_rotary_kind { B200_ROTARY_PLAIN = 0, B200_ROTARY_LINEAR = 1, B200_ROTARY_BASE = 2, B200_ROTARY_PARTS = 3 };
+typedef struct b200_rotary_scaling {
+    int32_t kind;
+    double base;
+    double factor;                 /* LINEAR, BASE, PARTS */
+    double original, low, high;    /* PARTS */
+    double magnitude;              /* of both tables; 0: 1 */
+} b200_rotary_scaling;
+B200_API int b200_rotary_tables(const b200_rotary_scaling* scaling, int32_t rot_dims, int64_t first, int64_t positions, float* cosine, float* sine,
+                                void* stream);
+
+/* The rows of a pass between their projection and their attention: the first rot_dims entries of every query and key head turn by the
+ * row's angle, keys and values are appended to the sequence's slot of the cache at positions lengths[slot] + r - first[s] (lengths do not move
+ * on: b200_rows_advance), queries are written out.  The angle is that of the position plus offset[s]: the length of the prefix that the slot's
+ * tokens stand behind.  Rows whose angle lies past the tables do not turn (as with b200_chunk_prepare); rows past the slot's pages are not
+ * appended. */
+typedef struct b200_rotary_append_args {
+    int32_t heads;
+    int32_t rot_dims;              /* even, 0 .. head_dim */
+    int32_t rotate_pairs;          /* 0: entry i turns with entry i + rot_dims / 2; 1: entry 2i with entry 2i + 1 */
+    const float* cosine;           /* [positions, rot_dims / 2] */
+    const float* sine;
+    int32_t positions;
+    const int32_t* offset;         /* [sequences] or NULL: 0 */
+    const float* projected;        /* rows [q: heads*dim | k: kv_heads*dim | v: kv_heads*dim | ...], stride floats apart */
+    int64_t stride;                /* 0: (heads + 2 kv_heads) * dim */
+    int32_t query_dtype;           /* B200_F32 or B200_BF16 */
+    void* query;                   /* [rows, heads, dim] */
+    b200_kv_pages cache;           /* sequences: the slots */
+} b200_rotary_append_args;
+B200_API int b200_rotary_append(const b200_rotary_append_args* args, const b200_rows* pass, void* stream);
+
+/* Grouped-query attention of a pass over a prefix that the sequences of a group share and over each sequence's own tokens: row r of
+ * sequence s in group g sees the first prefix_length[group_prefix[g]] positions of that prefix and, in slot[s] of the cache, the positions 0 ..
+ * lengths[slot[s]] + r - first[s], which the cache must already hold.  One softmax(scale q.k) over both.  A prefix's keys and values are read
+ * once for all rows of a group.  Group g owns the sequences group_first[g] .. group_first[g + 1] - 1 of the pass; a sequence in no group has no
+ * prefix, a prefix or slot number outside its table no positions; a row that sees nothing gives zeros.  Prefix and cache may be tables over the
+ * same pools. */
+typedef struct b200_prefix_args {
+    int32_t heads;
+    float scale;
+    const void* query;             /* [rows, heads, dim] in the caches' type */
+    b200_kv_pages cache;           /* sequences: the slots */
+    b200_kv_pages prefix;          /* sequences: the prefixes; not read without groups */
+    int32_t groups;
+    const int32_t* group_first;    /* [groups + 1] */
+    const int32_t* group_prefix;   /* [groups] */
+    const int32_t* prefix_length;  /* [prefixes] */
+} b200_prefix_args;
+/* max_length and max_prefix: upper bounds of lengths[slot] + rows of a sequence and of a prefix's length, by which the work is split (the pages
+ * of a table bound what is read).  The result [rows, heads*dim] in f32 (out) and / or as planes, out_stride elements between rows (0: heads*dim).
+ * bf16 caches: products of bf16 queries, keys, weights and values with f32 sums, so a result is good to bf16. */
+B200_API size_t b200_prefix_scratch_bytes(const b200_prefix_args* args, const b200_rows* pass, int32_t max_length, int32_t max_prefix);
+B200_API int b200_prefix_attention(const b200_prefix_args* args, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch,
+                                   size_t scratch_bytes, float* out, void* out_hi, void* out_lo, int64_t out_stride, void* stream);
+
+/* Drafted tokens against the target's probabilities.  The rows of a sequence are the logits behind its last sure token and behind each draft:
+ * ids[first[s]] is that token, ids[first[s] + 1] .. the drafts, and row r judges ids[r + 1].  With p = softmax(logits[r] / temperature), q the same
+ * of draft_logits[r], and x = ids[r + 1]: x is accepted if accept[r] q(x) < p(x), until the first that is not.  The next token is then drawn from
+ * the residual max(p - q, 0) of the row that refused, or from p of the sequence's last row when all drafts were accepted: the first index whose
+ * running sum exceeds draw[s] times the total.  Tokens so chosen are distributed as if drawn from p one by one.  Without draft_logits the
+ * drafts count as certain (q(x) = 1): what a lookup in the text gives.  temperature 0: a draft is accepted if it is the argmax (b200_argmax's
+ * rule), the next token is the argmax; no random numbers are read.  A draft outside [0, vocab) is refused, with p as the residual; so is one
+ * whose row of draft_logits has no finite weights.  A row of logits without finite weights (NaN or +inf in it, or nothing but -inf) accepts
+ * nothing and gives its argmax.  Weights are exp((x - max) * (1 / temperature)) in f32, their sums f64. */
+typedef struct b200_verify_args {
+    int64_t vocab;                 /* up to 2^23 */
+    int64_t stride;                /* floats between rows of logits and draft_logits; 0: vocab */
+    const float* logits;           /* [rows, vocab] */
+    const float* draft_logits;     /* [rows, vocab] or NULL; the sequences' last rows are not read */
+    const int64_t* ids;            /* [rows] */
+    double temperature;
+    const double* accept;          /* [rows] in [0, 1); the sequences' last rows are not read */
+    const double* draw;            /* [sequences] in [0, 1) */
+    int32_t* accepted;             /* [sequences] drafts accepted */
+    int64_t* next;                 /* [sequences] the token behind them; -1 for a sequence without rows */
+    int32_t advance;               /* 1: lengths[slot[s]] += accepted[s] + 1, the rows of the pass whose tokens stand */
+} b200_verify_args;
+B200_API size_t b200_verify_scratch_bytes(const b200_verify_args* args, const b200_rows* pass);
+B200_API int b200_verify_drafts(const b200_verify_args* args, const b200_rows* pass, void* scratch, size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
