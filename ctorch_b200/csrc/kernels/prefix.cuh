@@ -1,0 +1,153 @@
+// Work items of the attention over a shared prefix and own tokens: what its kernels share.
+#pragma once
+
+#include "paged.cuh"
+#include "rows.cuh"
+
+namespace b200 {
+
+constexpr int kUnit = 64;   // keys of a step; splits are whole steps
+
+struct PrefixParams {
+    RowsView rows;
+    PagesView own, prefix;
+    int heads, group, dim, groups;
+    const int32_t *group_first, *group_prefix, *prefix_length;
+    const void* query;
+    float scale;               // times log2(e)
+    int prefix_splits, own_splits;
+    int prefix_tiles;          // row tiles of all groups, at most
+    int own_tiles;             // row tiles per sequence, at most
+    int prefix_rows, own_rows; // pairs of a row tile
+    int beside;                // 1: the prefix's items are another kernel's, launched just before, beside which this one runs
+    int32_t* status;
+    float* part_o;             // [rows * heads][splits][dim]
+    float* part_ml;            // [rows * heads][splits][2]
+    float* out;
+    __nv_bfloat16 *out_hi, *out_lo;
+    int64_t out_stride;
+};
+
+struct KeySpan { int begin, end; };
+// Split `index` of `total` keys.
+__device__ __forceinline__ KeySpan split_span(int total, int splits, int index) {
+    const int steps = (total + kUnit - 1) / kUnit, per = (steps + splits - 1) / splits;
+    const int begin = min(total, index * per * kUnit);
+    return {begin, min(total, begin + per * kUnit)};
+}
+__device__ __forceinline__ int used_splits(int total, int splits) {
+    const int steps = (total + kUnit - 1) / kUnit;
+    if (steps == 0) return 0;
+    const int per = (steps + splits - 1) / splits;
+    return (steps + per - 1) / per;
+}
+
+__device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
+    const int slot = __ldg(p.group_prefix + g);
+    if (slot < 0 || slot >= p.prefix.sequences) return 0;
+    return max(0, min(__ldg(p.prefix_length + slot), p.prefix.capacity()));
+}
+__device__ __forceinline__ int own_keys(const PrefixParams& p, int slot, int count) {
+    if (slot < 0 || slot >= p.own.sequences) return 0;
+    return max(0, min(p.rows.lengths[slot] + count, p.own.capacity()));
+}
+
+// The group that owns sequence s, -1 if none does.
+__device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
+    int low = 0, high = p.groups;   // the last group that begins at or before s
+    while (low < high) {
+        const int middle = (low + high) / 2;
+        if (__ldg(p.group_first + middle) <= s) low = middle + 1;
+        else high = middle;
+    }
+    return low > 0 && s < __ldg(p.group_first + low) ? low - 1 : -1;
+}
+
+// One item: the rows m_begin .. m_count - 1 of (row, head of the group) pairs from `row` on, and a span of keys.
+struct Item {
+    bool live, causal;
+    int row, m_begin, m_count;   // first row of the group or sequence; pair m is row + m / group, head kv_head * group + m % group
+    int kv_head, slot, split;    // split: which partial result
+    int visible;                 // keys that pair 0 sees (causal: pair m sees m / group more)
+    KeySpan keys;
+};
+
+// Items are numbered split-major inside a kind; the prefix's, which are longer, come first.  Every warp works this out for itself.
+__device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
+    Item it{};
+    const int kv_heads = p.own.kv_heads, prefix_items = p.prefix_tiles * kv_heads * p.prefix_splits;
+    const int lane = threadIdx.x & 31;
+    if (index < prefix_items) {
+        it.kv_head = index % kv_heads;
+        const int rest = index / kv_heads;
+        int tile = rest % p.prefix_tiles;
+        it.split = rest / p.prefix_tiles;
+        // tile -> group: the groups' tile counts are added up 32 at a time
+        for (int base = 0; base < p.groups; base += 32) {
+            const int g = base + lane;
+            int begin = 0, rows = 0, tiles = 0;
+            if (g < p.groups) {
+                begin = __ldg(p.rows.first + __ldg(p.group_first + g));
+                rows = max(0, __ldg(p.rows.first + __ldg(p.group_first + g + 1)) - begin);
+                tiles = (rows * p.group + p.prefix_rows - 1) / p.prefix_rows;
+            }
+            int up_to = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, up_to, o);
+                if (lane >= o) up_to += other;
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, up_to > tile);
+            if (found) {
+                const int from = __ffs(found) - 1;
+                it.row = __shfl_sync(0xffffffffu, begin, from);
+                it.m_count = __shfl_sync(0xffffffffu, rows, from) * p.group;
+                it.m_begin = (tile - __shfl_sync(0xffffffffu, up_to - tiles, from)) * p.prefix_rows;
+                const int group = base + from, keys = prefix_keys(p, group);
+                it.slot = __ldg(p.group_prefix + group);
+                it.keys = split_span(keys, p.prefix_splits, it.split);
+                it.visible = keys;
+                it.live = it.keys.begin < it.keys.end;
+                return it;
+            }
+            tile -= __shfl_sync(0xffffffffu, up_to, 31);
+        }
+        return it;
+    }
+    index -= prefix_items;
+    it.kv_head = index % kv_heads;
+    int rest = index / kv_heads;
+    const int tile = rest % p.own_tiles;
+    rest /= p.own_tiles;
+    const int s = rest % p.rows.sequences, split = rest / p.rows.sequences;
+    it.split = p.prefix_splits + split;
+    it.row = __ldg(p.rows.first + s);
+    const int count = max(0, __ldg(p.rows.first + s + 1) - it.row);
+    it.m_count = count * p.group;
+    it.m_begin = tile * p.own_rows;
+    it.slot = __ldg(p.rows.slot + s);
+    const int keys = own_keys(p, it.slot, count);
+    it.keys = split_span(keys, p.own_splits, split);
+    it.causal = true;
+    it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
+    if (it.live) it.visible = p.rows.lengths[it.slot] + 1;
+    return it;
+}
+
+// A kernel that runs beside the prefix's: that one let it start when everything before both was complete, so it need not wait to begin; it waits
+// before it ends, so that it is complete no earlier than the other and the merge can wait for this one alone.
+__device__ __forceinline__ void begin_items(const PrefixParams& p) {
+    if (!p.beside) grid_dependency_wait();
+    grid_launch_dependents();
+}
+__device__ __forceinline__ void end_items(const PrefixParams& p) {
+    if (p.beside) grid_dependency_wait();
+}
+__device__ __forceinline__ int first_item(const PrefixParams& p) { return p.beside ? p.prefix_tiles * p.own.kv_heads * p.prefix_splits : 0; }
+
+// Where pair m of an item leaves its partial result: row of [rows * heads][splits].
+__device__ __forceinline__ int64_t partial_row(const PrefixParams& p, const Item& it, int m) {
+    return ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * (p.prefix_splits + p.own_splits) + it.split;
+}
+
+}  // namespace b200

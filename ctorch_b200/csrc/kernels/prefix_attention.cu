@@ -6,143 +6,13 @@
 // sum, accumulator) per row and head, and the merge kernel joins them under one softmax:
 //   m = max m_i,  out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i      (scores in units of log2 e).
 #include "mma.cuh"
-#include "paged.cuh"
-#include "rows.cuh"
+#include "prefix.cuh"
+#include "prefix_tensor.cuh"
 
 #include <cmath>
 
 namespace b200 {
 namespace {
-
-constexpr int kUnit = 64;   // keys of a step; splits are whole steps
-
-struct PrefixParams {
-    RowsView rows;
-    PagesView own, prefix;
-    int heads, group, dim, groups;
-    const int32_t *group_first, *group_prefix, *prefix_length;
-    const void* query;
-    float scale;               // times log2(e)
-    int prefix_splits, own_splits;
-    int prefix_tiles;          // row tiles of all groups, at most
-    int own_tiles;             // row tiles per sequence, at most
-    float* part_o;             // [rows * heads][splits][dim]
-    float* part_ml;            // [rows * heads][splits][2]
-    float* out;
-    __nv_bfloat16 *out_hi, *out_lo;
-    int64_t out_stride;
-};
-
-struct KeySpan { int begin, end; };
-// Split `index` of `total` keys.
-__device__ __forceinline__ KeySpan split_span(int total, int splits, int index) {
-    const int steps = (total + kUnit - 1) / kUnit, per = (steps + splits - 1) / splits;
-    const int begin = min(total, index * per * kUnit);
-    return {begin, min(total, begin + per * kUnit)};
-}
-__device__ __forceinline__ int used_splits(int total, int splits) {
-    const int steps = (total + kUnit - 1) / kUnit;
-    if (steps == 0) return 0;
-    const int per = (steps + splits - 1) / splits;
-    return (steps + per - 1) / per;
-}
-
-__device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
-    const int slot = __ldg(p.group_prefix + g);
-    if (slot < 0 || slot >= p.prefix.sequences) return 0;
-    return max(0, min(__ldg(p.prefix_length + slot), p.prefix.capacity()));
-}
-__device__ __forceinline__ int own_keys(const PrefixParams& p, int slot, int count) {
-    if (slot < 0 || slot >= p.own.sequences) return 0;
-    return max(0, min(p.rows.lengths[slot] + count, p.own.capacity()));
-}
-
-// The group that owns sequence s, -1 if none does.
-__device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
-    int low = 0, high = p.groups;   // the last group that begins at or before s
-    while (low < high) {
-        const int middle = (low + high) / 2;
-        if (__ldg(p.group_first + middle) <= s) low = middle + 1;
-        else high = middle;
-    }
-    return low > 0 && s < __ldg(p.group_first + low) ? low - 1 : -1;
-}
-
-// One item: the rows m_begin .. m_count - 1 of (row, head of the group) pairs from `row` on, and a span of keys.
-struct Item {
-    bool live, causal;
-    int row, m_begin, m_count;   // first row of the group or sequence; pair m is row + m / group, head kv_head * group + m % group
-    int kv_head, slot, split;    // split: which partial result
-    int visible;                 // keys that pair 0 sees (causal: pair m sees m / group more)
-    KeySpan keys;
-};
-
-// Items are numbered split-major inside a kind; the prefix's, which are longer, come first.  Every warp works this out for itself.
-__device__ __forceinline__ Item find_item(const PrefixParams& p, int index, int tile_rows) {
-    Item it{};
-    const int kv_heads = p.own.kv_heads, prefix_items = p.prefix_tiles * kv_heads * p.prefix_splits;
-    const int lane = threadIdx.x & 31;
-    if (index < prefix_items) {
-        it.kv_head = index % kv_heads;
-        const int rest = index / kv_heads;
-        int tile = rest % p.prefix_tiles;
-        it.split = rest / p.prefix_tiles;
-        // tile -> group: the groups' tile counts are added up 32 at a time
-        for (int base = 0; base < p.groups; base += 32) {
-            const int g = base + lane;
-            int begin = 0, rows = 0, tiles = 0;
-            if (g < p.groups) {
-                begin = __ldg(p.rows.first + __ldg(p.group_first + g));
-                rows = max(0, __ldg(p.rows.first + __ldg(p.group_first + g + 1)) - begin);
-                tiles = (rows * p.group + tile_rows - 1) / tile_rows;
-            }
-            int up_to = tiles;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, up_to, o);
-                if (lane >= o) up_to += other;
-            }
-            const unsigned found = __ballot_sync(0xffffffffu, up_to > tile);
-            if (found) {
-                const int from = __ffs(found) - 1;
-                it.row = __shfl_sync(0xffffffffu, begin, from);
-                it.m_count = __shfl_sync(0xffffffffu, rows, from) * p.group;
-                it.m_begin = (tile - __shfl_sync(0xffffffffu, up_to - tiles, from)) * tile_rows;
-                const int group = base + from, keys = prefix_keys(p, group);
-                it.slot = __ldg(p.group_prefix + group);
-                it.keys = split_span(keys, p.prefix_splits, it.split);
-                it.visible = keys;
-                it.live = it.keys.begin < it.keys.end;
-                return it;
-            }
-            tile -= __shfl_sync(0xffffffffu, up_to, 31);
-        }
-        return it;
-    }
-    index -= prefix_items;
-    it.kv_head = index % kv_heads;
-    int rest = index / kv_heads;
-    const int tile = rest % p.own_tiles;
-    rest /= p.own_tiles;
-    const int s = rest % p.rows.sequences, split = rest / p.rows.sequences;
-    it.split = p.prefix_splits + split;
-    it.row = __ldg(p.rows.first + s);
-    const int count = max(0, __ldg(p.rows.first + s + 1) - it.row);
-    it.m_count = count * p.group;
-    it.m_begin = tile * tile_rows;
-    it.slot = __ldg(p.rows.slot + s);
-    const int keys = own_keys(p, it.slot, count);
-    it.keys = split_span(keys, p.own_splits, split);
-    it.causal = true;
-    it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
-    if (it.live) it.visible = p.rows.lengths[it.slot] + 1;
-    return it;
-}
-
-// Where pair m of an item leaves its partial result: row of [rows * heads][splits].
-__device__ __forceinline__ int64_t partial_row(const PrefixParams& p, const Item& it, int m) {
-    return ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * (p.prefix_splits + p.own_splits) + it.split;
-}
 
 // ---- any type and head size: f32 products on the CUDA cores --------------------------------------------------------------------------------
 constexpr int kPlainRows = 32, kPlainKeys = 32, kPlainThreads = 128;
@@ -156,10 +26,9 @@ __host__ __device__ constexpr int plain_smem(int dim) {
 // accumulators.
 template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) prefix_plain_kernel(const PrefixParams p) {
     extern __shared__ __align__(16) float plain_shared[];
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const Item it = find_item(p, blockIdx.x, kPlainRows);
-    if (!it.live) return;
+    begin_items(p);
+    const Item it = find_item(p, first_item(p) + blockIdx.x);
+    if (!it.live) return end_items(p);
     const int width = plain_width(p.dim), pitch = width + 4;
     float* query = plain_shared;
     float* key = query + kPlainRows * width;
@@ -260,6 +129,7 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
             for (int u = 0; u < 4; ++u)
                 if (32 * c + 4 * tx + u < p.dim) p.part_o[at * p.dim + 32 * c + 4 * tx + u] = acc[r][c][u];
     }
+    end_items(p);
 }
 
 // ---- bf16, heads of 8 n <= 128 values: mma.sync ---------------------------------------------------------------------------------------------
@@ -322,10 +192,9 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
     extern __shared__ __align__(128) unsigned char mma_shared[];
     constexpr int kKeys = SPLIT ? 16 : 64;       // keys per warp and step
     constexpr int kTiles = kKeys / 8, kSteps = HD / 16, kColumns = HD / 8;
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const Item it = find_item(p, blockIdx.x, SPLIT ? 16 : 64);
-    if (!it.live) return;
+    begin_items(p);
+    const Item it = find_item(p, first_item(p) + blockIdx.x);
+    if (!it.live) return end_items(p);
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
     const PagesView& view = it.causal ? p.own : p.prefix;
     const uint32_t shared = smem_u32(mma_shared);
@@ -516,6 +385,7 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
                 if (8 * n < p.dim) *reinterpret_cast<float2*>(p.part_o + to * p.dim + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
         }
     }
+    end_items(p);
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------------------------
@@ -556,10 +426,11 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p)
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------
 constexpr int kMostDim = 256;
 
-enum class Form { plain, mma_split, mma_rows };
+enum class Form { plain, mma };
 struct Plan {
     Form form;
-    int tile_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
+    bool tensor;               // the prefix's items are the tcgen05 kernel's
+    int prefix_rows, own_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
 };
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
@@ -572,21 +443,27 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     const bool mma = a.cache.dtype == B200_BF16 && a.cache.head_dim % 8 == 0 && a.cache.head_dim <= 128 && bits % 16 == 0;
     const int64_t pairs = pass.rows * group;
     const int groups = a.groups < pass.sequences ? a.groups : pass.sequences;
-    plan.form = !mma ? Form::plain : pairs <= 16 * static_cast<int64_t>(pass.sequences) ? Form::mma_split : Form::mma_rows;
-    if (mma && a.groups && pairs > 16 * static_cast<int64_t>(a.groups)) plan.form = Form::mma_rows;
-    plan.tile_rows = plan.form == Form::plain ? kPlainRows : plan.form == Form::mma_split ? 16 : 64;
     const bool prefix = a.groups > 0 && max_prefix > 0;
-    plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.tile_rows) + groups : 0;
-    plan.own_tiles = ceil_div(static_cast<int64_t>(pass.max_count) * group, plan.tile_rows);
-    auto splits = [&](int64_t items, int keys) {
+    plan.form = mma ? Form::mma : Form::plain;
+    plan.tensor = mma && prefix && pairs > 32 * static_cast<int64_t>(groups) && prefix_tensor_takes(a.prefix, a.scale);
+    // a tile of 16 pairs, or of 64 where most would not fit
+    const int64_t own_pairs = static_cast<int64_t>(pass.max_count) * group;
+    plan.own_rows = !mma ? kPlainRows : own_pairs <= 16 || (!plan.tensor && prefix && pairs <= 16 * static_cast<int64_t>(groups)) ? 16 : 64;
+    if (mma && prefix && !plan.tensor && pairs > 16 * static_cast<int64_t>(groups)) plan.own_rows = 64;
+    plan.prefix_rows = plan.tensor ? kTensorRows : plan.own_rows;
+    plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.prefix_rows) + groups : 0;
+    plan.own_tiles = ceil_div(own_pairs, plan.own_rows);
+    auto splits = [&](int64_t items, int keys, int ctas) {
         const int most = ceil_div(keys, 4 * kUnit);
-        int n = static_cast<int>(2 * 148 / (items > 0 ? items : 1));
+        int n = static_cast<int>(ctas / (items > 0 ? items : 1));
         if (n > most) n = most;
         if (n > 64) n = 64;
         return n < 1 ? 1 : n;
     };
-    plan.prefix_splits = prefix ? splits(static_cast<int64_t>(plan.prefix_tiles) * kv_heads, max_prefix) : 0;
-    plan.own_splits = splits(static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads, max_length);
+    // tiles that the rows fill: the last tile of every group is counted half
+    const int64_t filled = ceil_div(pairs, plan.prefix_rows) > groups ? ceil_div(pairs, plan.prefix_rows) : groups;
+    plan.prefix_splits = prefix ? splits(filled * kv_heads, max_prefix, plan.tensor ? 148 : 2 * 148) : 0;
+    plan.own_splits = splits(static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads, max_length, 2 * 148);
     return plan;
 }
 
@@ -619,8 +496,8 @@ template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned item
     return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p);
 }
 
-template <int HD> cudaError_t launch_mma(const PrefixParams& p, bool split, unsigned items, cudaStream_t stream) {
-    auto kernel = split ? prefix_mma_kernel<HD, true> : prefix_mma_kernel<HD, false>;
+template <int HD> cudaError_t launch_mma(const PrefixParams& p, unsigned items, cudaStream_t stream) {
+    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, true> : prefix_mma_kernel<HD, false>;
     constexpr int smem = MmaShape<HD>::smem_bytes;
     const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (status != cudaSuccess) return status;
@@ -661,24 +538,34 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     p.query = a->query;
     p.scale = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
     p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits; p.prefix_tiles = plan.prefix_tiles; p.own_tiles = plan.own_tiles;
+    p.prefix_rows = plan.prefix_rows; p.own_rows = plan.own_rows;
     p.part_o = static_cast<float*>(scratch);
     p.part_ml = p.part_o + static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * p.dim;
     p.out = out; p.out_hi = static_cast<__nv_bfloat16*>(out_hi); p.out_lo = static_cast<__nv_bfloat16*>(out_lo);
     p.out_stride = out_stride ? out_stride : width;
-    const int64_t items = (static_cast<int64_t>(plan.prefix_tiles) * plan.prefix_splits + static_cast<int64_t>(pass->sequences) * plan.own_tiles * plan.own_splits)
-                          * a->cache.kv_heads;
+    const int64_t prefix_items = static_cast<int64_t>(plan.prefix_tiles) * plan.prefix_splits * a->cache.kv_heads;
+    const int64_t own_items = static_cast<int64_t>(pass->sequences) * plan.own_tiles * plan.own_splits * a->cache.kv_heads;
     const int64_t merges = (pass->rows * a->heads + 3) / 4;
-    if (items > INT32_MAX || merges > INT32_MAX || static_cast<int64_t>(pass->rows) * p.group > INT32_MAX / 2) {
+    if (prefix_items + own_items > INT32_MAX || merges > INT32_MAX || static_cast<int64_t>(pass->rows) * p.group > INT32_MAX / 2) {
         set_error("b200_prefix_attention: too many rows");
         return B200_UNSUPPORTED;
     }
     cudaStream_t s = as_stream(stream);
+    if (plan.tensor) {
+        int device = 0;
+        B200_CUDA(cudaGetDevice(&device));
+        p.status = device_status_word(device);
+        if (!p.status) { set_error("b200_prefix_attention: the device status word could not be allocated"); return B200_NO_DEVICE; }
+        const int status = launch_prefix_tensor(p, static_cast<int>(prefix_items), s);
+        if (status != B200_OK) return status;
+        p.beside = 1;
+    }
+    const unsigned items = static_cast<unsigned>(plan.tensor ? own_items : prefix_items + own_items);
     cudaError_t launched;
-    if (plan.form == Form::plain)
-        launched = a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, static_cast<unsigned>(items), s) : launch_plain<float>(p, static_cast<unsigned>(items), s);
-    else if (p.dim <= 64) launched = launch_mma<64>(p, plan.form == Form::mma_split, static_cast<unsigned>(items), s);
-    else if (p.dim <= 96) launched = launch_mma<96>(p, plan.form == Form::mma_split, static_cast<unsigned>(items), s);
-    else launched = launch_mma<128>(p, plan.form == Form::mma_split, static_cast<unsigned>(items), s);
+    if (plan.form == Form::plain) launched = a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, s) : launch_plain<float>(p, items, s);
+    else if (p.dim <= 64) launched = launch_mma<64>(p, items, s);
+    else if (p.dim <= 96) launched = launch_mma<96>(p, items, s);
+    else launched = launch_mma<128>(p, items, s);
     const int status = cuda_status(launched, "b200_prefix_attention launch");
     if (status != B200_OK) return status;
     return cuda_status(launch_dependent(prefix_merge_kernel, dim3(static_cast<unsigned>(merges)), dim3(128), 0, s, p), "prefix_merge_kernel launch");

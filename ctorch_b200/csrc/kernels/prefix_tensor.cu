@@ -1,0 +1,321 @@
+// The shared prefix of b200_prefix_attention on tcgen05: groups with many rows.
+//
+// A CTA has two tiles of 128 (row, head) pairs and a span of keys, 128 at a time.  Per tile and step: S = Q K^T into tensor memory (128 x 128 f32),
+// a softmax warpgroup - a thread per pair - turns S into bf16 weights P in the same columns, O += P V with P read from tensor memory.  The tensor
+// cores work on one tile while the other's softmax runs.
+//   warps 0-3, 4-7   softmax of tile 0 and 1 (lane quarter = warp % 4), at the end the tile's partial result
+//   warp 8           copies K and V steps through a ring of shared-memory slots with TMA, page by page
+//   warp 9           tensor memory and all products
+// O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the maximum its weights are relative to: they
+// are relative to the same one in the sum and in O, so the quotient is the softmax all the same, and weights up to 2^8 lose nothing in f32 and bf16.
+#include "mma.cuh"
+#include "prefix.cuh"
+#include "prefix_tensor.cuh"
+#include "tcgen05.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kTensorThreads = 320;
+constexpr float kLazy = 8.0f;
+
+template <int HD> struct TensorShape {
+    static constexpr int blocks = HD / 64;                          // 64 values: one swizzled row of 128 bytes
+    static constexpr int block_bytes = kTensorKeys * 128;
+    static constexpr int tile_bytes = blocks * block_bytes;         // 128 rows of Q, K or V
+    static constexpr int slots = HD == 128 ? 5 : 8;
+    static constexpr int smem_bytes = (2 + slots) * tile_bytes + 1024 + 1024;   // slack of the 1024-byte alignment, control words
+    static constexpr uint32_t scores = mma_instruction_bf16(128, kTensorKeys);
+    static constexpr uint32_t sums = mma_instruction_bf16(128, HD) | kTransposedB;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
+                                                                          const PrefixParams p, const int box_rows) {
+    using S = TensorShape<HD>;
+    extern __shared__ uint8_t tensor_shared[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tensor_shared) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* ring = smem + 2 * S::tile_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + S::slots * S::tile_bytes);
+    uint64_t* empty = full + S::slots;
+    uint64_t* q_ready = empty + S::slots;
+    uint64_t* s_full = q_ready + 1;     // [2] S of a step is in tensor memory
+    uint64_t* p_ready = s_full + 2;     // [2] the weights of a step are
+    uint64_t* o_done = p_ready + 2;     // [2] a step's values are added to O
+    uint64_t* tail = o_done + 2;        // what the last step's pages hold behind its keys is zeroed
+    uint64_t* drained = tail + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    volatile int* alive = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    begin_items(p);
+    const Item it = find_item(p, blockIdx.x);
+    if (!it.live) return;
+    const int tiles = it.m_count - it.m_begin > 128 ? 2 : 1;
+    const int steps = (it.keys.end - it.keys.begin + kTensorKeys - 1) / kTensorKeys;
+    const int last_keys = it.keys.end - it.keys.begin - (steps - 1) * kTensorKeys;
+    const bool has_tail = last_keys % box_rows != 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::slots; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(q_ready, 128 * tiles);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_ready[t], 128);
+            mbar_init(&o_done[t], 1);
+        }
+        mbar_init(tail, 1);
+        mbar_init(drained, 1);
+        *alive = 1;
+        mbar_fence_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    // for whole warps; every wait ends: after a limit, or when another role has given up
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!mbar_wait(bar, parity)) {
+            atomicExch(p.status, B200_DEVICE_TIMEOUT);
+            *alive = 0;
+        }
+        return __all_sync(0xffffffffu, *alive != 0) != 0;
+    };
+
+    if (warp == 8) {
+        const int per_head = p.prefix.page_size, heads = p.prefix.kv_heads;
+        const int outside = static_cast<int>(p.prefix.pages) * heads * per_head;   // a row past the pools: zeros
+        int issued = 0;
+        for (int j = 0; j < 2 * steps; ++j, ++issued) {
+            const int slot = j % S::slots, step = j / 2;
+            if (!wait(&empty[slot], ((j / S::slots) & 1) ^ 1)) break;
+            if (lane == 0) mbar_expect_tx(&full[slot], S::tile_bytes);
+            __syncwarp();
+            const int boxes = kTensorKeys / box_rows * S::blocks;   // at most 32
+            if (lane < boxes) {
+                const int block = lane % S::blocks, row = lane / S::blocks * box_rows;
+                const int position = it.keys.begin + step * kTensorKeys + row;
+                int y = outside;
+                if (position < it.keys.end) {
+                    const int page = page_of(p.prefix, it.slot, position / per_head);
+                    if (page >= 0) y = (page * heads + it.kv_head) * per_head + position % per_head;
+                }
+                tma_load_2d(ring + slot * S::tile_bytes + block * S::block_bytes + row * 128, j & 1 ? &value_map : &key_map, block * 64, y, &full[slot]);
+            }
+            __syncwarp();
+        }
+        if (issued == 2 * steps && has_tail) {
+            // rows of the last box behind the keys may hold anything, and a weight of 0 does not cancel what is no number
+            const int j = 2 * steps - 1, slot = j % S::slots;
+            if (wait(&full[slot], (j / S::slots) & 1)) {
+                const int behind = (last_keys + box_rows - 1) / box_rows * box_rows - last_keys;
+                for (int i = lane; i < behind * 8 * S::blocks; i += 32)
+                    *reinterpret_cast<uint4*>(ring + slot * S::tile_bytes + i / (behind * 8) * S::block_bytes + last_keys * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tail);
+            }
+        }
+        if (*alive == 0)   // no copy is in flight when the CTA leaves
+            for (int j = max(0, issued - S::slots); j < issued; ++j) mbar_wait(&full[j % S::slots], (j / S::slots) & 1);
+    } else if (warp == 9) {
+        const uint32_t queries = smem_u32(smem), slots = smem_u32(ring);
+        auto scores = [&](int t, int step) {
+            const uint32_t key = slots + (2 * step) % S::slots * S::tile_bytes;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+                tc_mma_bf16(tmem + t * 128, operand_descriptor(queries + t * S::tile_bytes + k / 4 * S::block_bytes) + 2 * (k % 4),
+                            operand_descriptor(key + k / 4 * S::block_bytes) + 2 * (k % 4), S::scores, k != 0);
+            tc_commit(&s_full[t]);
+        };
+        bool going = wait(q_ready, 0) && wait(&full[0], 0);
+        tc_fence_after_sync();
+        if (going && elect_one()) {
+            for (int t = 0; t < tiles; ++t) scores(t, 0);
+            tc_commit(&empty[0]);
+        }
+        for (int step = 0; step < steps && going; ++step) {
+            const int v = 2 * step + 1, k = v + 1;
+            const bool more = step + 1 < steps;
+            going = wait(&full[v % S::slots], (v / S::slots) & 1) && (!more || wait(&full[k % S::slots], (k / S::slots) & 1))
+                    && (more || !has_tail || wait(tail, 0));
+            for (int t = 0; t < tiles && going; ++t) {
+                going = wait(&p_ready[t], step & 1);
+                tc_fence_after_sync();
+                if (going && elect_one()) {
+                    const uint32_t value = slots + v % S::slots * S::tile_bytes;
+#pragma unroll
+                    for (int i = 0; i < kTensorKeys / 16; ++i)
+                        tc_mma_bf16_tmem(tmem + 256 + t * HD, tmem + t * 128 + 8 * i, operand_descriptor_transposed(value + i * 2048, S::block_bytes), S::sums, (step | i) != 0);
+                    tc_commit(&o_done[t]);
+                    if (more) scores(t, step + 1);
+                }
+            }
+            if (going && elect_one()) {
+                tc_commit(&empty[v % S::slots]);
+                if (more) tc_commit(&empty[k % S::slots]);
+            }
+        }
+        if (*alive == 0) {   // nor a product
+            if (elect_one()) tc_commit(drained);
+            mbar_wait(drained, 0);
+        }
+    } else if (warp / 4 < tiles) {
+        const int t = warp / 4, row = threadIdx.x % 128;
+        const int m_tile = it.m_begin + t * 128;
+        // the tile's queries, as TMA would lay them out; a negative scale becomes one of the queries
+        {
+            const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+            constexpr int kPieces = 8 * S::blocks;
+            for (int i = row; i < 128 * kPieces; i += 128) {
+                const int r = i / kPieces, c = i % kPieces, m = m_tile + r;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (m < it.m_count) {
+                    x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query)
+                                                             + ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * HD + 8 * c));
+                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                }
+                *reinterpret_cast<uint4*>(smem + t * S::tile_bytes + c / 8 * S::block_bytes + r * 128 + (((c ^ r) & 7) << 4)) = x;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(q_ready);
+        }
+        const float scale = fabsf(p.scale);
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * HD;
+        float most = -INFINITY, sum = 0.0f;   // the maximum that the weights are relative to
+        bool going = true;
+        for (int step = 0; step < steps; ++step) {
+            going = wait(&s_full[t], step & 1);
+            if (!going) break;
+            tc_fence_after_sync();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_load_32_async(s_at + 32 * c, s[c]);
+            tmem_wait_loads();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
+            const int live = min(kTensorKeys, it.keys.end - it.keys.begin - step * kTensorKeys);
+            if (live < kTensorKeys) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * c + i >= live) s[c][i] = 0xff800000u;   // -inf
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+            const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+            const bool grows = here > most + kLazy;
+            if (__any_sync(0xffffffffu, grows)) {
+                const float factor = grows ? exp2_fast(most - here) : 1.0f;
+                if (grows) most = here;
+                sum *= factor;
+                if (step > 0) {
+                    going = wait(&o_done[t], (step - 1) & 1);
+                    if (!going) break;
+                    tc_fence_after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_load_32(o_at + 32 * c, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                        tmem_store_32(o_at + 32 * c, o);
+                    }
+                }
+            }
+            const float base = most == -INFINITY ? 0.0f : -most;
+            float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t weights[32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float a = exp2_fast(fmaf(__uint_as_float(s[2 * half + c][i]), scale, base));
+                        const float b = exp2_fast(fmaf(__uint_as_float(s[2 * half + c][i + 1]), scale, base));
+                        add[(i / 2) & 1] += a;
+                        add[2 + ((i / 2) & 1)] += b;
+                        weights[16 * c + i / 2] = pack_bf16(a, b);
+                    }
+                tmem_store_32(s_at + 32 * half, weights);
+            }
+            sum += (add[0] + add[1]) + (add[2] + add[3]);
+            tmem_wait_stores();
+            tc_fence_before_sync();
+            mbar_arrive(&p_ready[t]);
+        }
+        if (going && wait(&o_done[t], (steps - 1) & 1)) {
+            tc_fence_after_sync();
+            const int m = m_tile + row;
+            const int64_t to = m < it.m_count ? partial_row(p, it, m) : 0;
+            if (m < it.m_count) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most, sum);
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_load_32(o_at + 32 * c, o);
+                if (m < it.m_count) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(p.part_o + to * HD + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Rows of a TMA box: a part of a page of at most 64 rows whose multiples are the tiles' and the pages' borders.
+int box_rows_of(int page_size) {
+    for (int rows = 64; rows >= 8; rows /= 2)
+        if (page_size % rows == 0) return rows;
+    return 0;
+}
+
+template <int HD> int launch_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
+    encode_tiled_fn encode = tensor_map_encoder();
+    if (!encode) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return B200_NO_DEVICE; }
+    const int box_rows = box_rows_of(p.prefix.page_size);
+    const cuuint64_t dims[2] = {HD, static_cast<cuuint64_t>(p.prefix.pages) * p.prefix.kv_heads * p.prefix.page_size};
+    const cuuint64_t strides[1] = {HD * 2};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, ones[2] = {1, 1};
+    CUtensorMap maps[2];
+    for (int which = 0; which < 2; ++which) {
+        const CUresult result = encode(&maps[which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.prefix.pool[which], dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (result != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with %d", static_cast<int>(result)); return B200_BAD_ARGUMENT; }
+    }
+    auto kernel = prefix_tensor_kernel<HD>;
+    B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TensorShape<HD>::smem_bytes));
+    return cuda_status(launch_dependent(kernel, dim3(static_cast<unsigned>(items)), dim3(kTensorThreads), TensorShape<HD>::smem_bytes, stream, maps[0], maps[1], p, box_rows),
+                       "prefix_tensor_kernel launch");
+}
+
+}  // namespace
+
+bool prefix_tensor_takes(const b200_kv_pages& prefix, float scale) {
+    return prefix.dtype == B200_BF16 && (prefix.head_dim == 64 || prefix.head_dim == 128) && box_rows_of(prefix.page_size) > 0 && scale != 0.0f
+           && prefix.pages * prefix.kv_heads * prefix.page_size < INT32_MAX;
+}
+
+int launch_prefix_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
+    return p.dim == 128 ? launch_tensor<128>(p, items, stream) : launch_tensor<64>(p, items, stream);
+}
+
+}  // namespace b200

@@ -36,6 +36,42 @@ __device__ __forceinline__ void tmem_load_32(uint32_t address, uint32_t (&r)[32]
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The same without the wait: several loads in flight, then tmem_wait_loads() and tmem_loaded() on each.
+__device__ __forceinline__ void tmem_load_32_async(uint32_t address, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(address) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Keeps every use of a load's registers behind the wait.
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+__device__ __forceinline__ void tmem_store_32(uint32_t address, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+          "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+          "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(address) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The A operand from tensor memory: row i in lane i, two bf16 of the K side per column.
+__device__ __forceinline__ void tc_mma_bf16_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
 // Shared-memory matrix descriptor of a K-major operand tile [rows][64 bf16] written by TMA with 128-byte swizzle:
 // 8-row groups of 1024 bytes follow each other (stride byte offset 1024), descriptor version 1, layout type 2.
 __device__ __forceinline__ uint64_t operand_descriptor(uint32_t smem_address) {
@@ -47,6 +83,19 @@ __device__ __forceinline__ uint64_t operand_descriptor(uint32_t smem_address) {
     d |= static_cast<uint64_t>(2) << 61;                          // 128-byte swizzle
     return d;
 }
+
+// The same of a tile whose contiguous side is M or N: [K rows][64 bf16] blocks, `block_bytes` between the blocks of 64; groups of eight K rows
+// follow each other every 1024 bytes.
+__device__ __forceinline__ uint64_t operand_descriptor_transposed(uint32_t smem_address, uint32_t block_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_address & 0x3ffff) >> 4);
+    d |= static_cast<uint64_t>(block_bytes >> 4) << 16;           // leading byte offset: between blocks of 64 of the contiguous side
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+constexpr uint32_t kTransposedB = 1u << 16;   // instruction descriptor: B's contiguous side is N
 
 // Instruction descriptor of tcgen05.mma.kind::f16: f32 accumulator, bf16 x bf16, both operands K-major, A with `m` rows
 // (64 or 128), B with `n` rows (a multiple of 16 up to 256).

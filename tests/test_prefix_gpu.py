@@ -191,6 +191,8 @@ ATTENTIONS = {  # dtype, heads, kv_heads, dim, page, prefixes' lengths, first se
     "sequences in no group": ("bf16", 8, 2, 64, 16, [80, 60], [1, 3, 4], [1, 0], [1, 2, 1, 3, 1, 2], [20, 3, 40, 0, 7, 100]),
     "sequences without rows": ("bf16", 8, 2, 64, 16, [80, 60], [0, 2, 5], [0, 1], [0, 2, 0, 0, 3], [20, 3, 40, 0, 7]),
     "a prefix named twice, one that is none": ("bf16", 8, 2, 64, 16, [80, 60], [0, 2, 3, 4], [1, 1, 7], [1, 2, 1, 3], [20, 3, 40, 0]),
+    "two tiles and a bit": ("bf16", 16, 2, 128, 32, [1500, 700, 64], [0, 5, 7, 8], [1, 0, 2], [9, 9, 9, 9, 9, 30, 34, 1], [3, 0, 100, 33, 64, 5, 8, 90]),
+    "pages of 8": ("bf16", 8, 1, 64, 8, [333, 120], [0, 6, 12], [0, 1], [1 + i % 4 for i in range(12)], [7 * i for i in range(12)]),
     "long prefix": ("bf16", 8, 1, 64, 64, [5000], [0, 20], [0], [2] * 20, [60 + i for i in range(20)]),
     "forty groups": ("bf16", 2, 1, 64, 16, [30 + i for i in range(40)], list(range(41)), list(range(40)), [1 + i % 3 for i in range(40)], [i for i in range(40)]),
 }
@@ -266,6 +268,20 @@ def test_attention(name, spread):
     assert (np.abs(planes - got) <= BF16_STEP * np.abs(got) + 1e-38).all()
     # the planes hold 16 bits: what is left of the first one's rounding is rounded once more
     assert (np.abs(planes + host(lo)[:state.live, :width].reshape(want.shape) - got) <= BF16_STEP ** 2 * np.abs(got) + 1e-38).all()
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-6, 0.7])
+@pytest.mark.parametrize("name", ["drafts", "many rows", "heads of 80", "f32"])
+def test_scales(name, scale):
+    state, cache, prefix, query, of = attention_state(name)
+    out = torch.empty((state.rows, of["heads"] * of["dim"]), device="cuda")
+    call = Attention(state, cache, prefix, query, of)
+    call.a.scale = scale
+    call(out)
+    f, heads = of, of["heads"]
+    want, mass, size, keys = O.attention(host(query)[:state.live], heads, float(np.float32(scale)), cache.oracle(), [int(s) for s in state.slots], [int(x) for x in state.first],
+                                         [int(n) for n in state.lengths], prefix.oracle(), f["group_first"], f["group_prefix"], f["prefixes"])
+    assert (np.abs(host(out).reshape(want.shape) - want) <= attention_bound(of, mass, size, keys)).all()
 
 
 @pytest.mark.parametrize("name", ["drafts", "many rows", "f32", "long prefix"])
