@@ -52,17 +52,6 @@ __device__ __forceinline__ int own_keys(const PrefixParams& p, int slot, int cou
     return max(0, min(p.rows.lengths[slot] + count, p.own.capacity()));
 }
 
-// The group that owns sequence s, -1 if none does.
-__device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
-    int low = 0, high = p.groups;   // the last group that begins at or before s
-    while (low < high) {
-        const int middle = (low + high) / 2;
-        if (__ldg(p.group_first + middle) <= s) low = middle + 1;
-        else high = middle;
-    }
-    return low > 0 && s < __ldg(p.group_first + low) ? low - 1 : -1;
-}
-
 // One item: the rows m_begin .. m_count - 1 of (row, head of the group) pairs from `row` on, and a span of keys.
 struct Item {
     bool live, causal;

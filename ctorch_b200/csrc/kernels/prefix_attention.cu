@@ -9,6 +9,7 @@
 #include "prefix.cuh"
 #include "prefix_tensor.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace b200 {
@@ -133,114 +134,114 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
 }
 
 // ---- bf16, heads of 8 n <= 128 values: mma.sync ---------------------------------------------------------------------------------------------
-constexpr int kMmaThreads = 128, kMmaStages = 3;
+constexpr int kMmaWarps = 4, kMmaThreads = (kMmaWarps + 1) * 32;   // four warps of products, one that copies
 
 template <int HD> struct MmaShape {                              // HD: the head size rounded up to 64, 96 or 128
-    static constexpr int row_bytes = HD <= 64 ? 128 : 256;
-    static constexpr int tile_bytes = kUnit * row_bytes;         // K or V of one step
-    static constexpr int stage_bytes = 2 * tile_bytes;
-    static constexpr int smem_bytes = kMmaStages * stage_bytes;
-    static constexpr int slots = row_bytes / 16;                 // 16-byte pieces of a row
-    static constexpr int rows_per_pass = kMmaThreads / slots;
-    static constexpr int passes = kUnit / rows_per_pass;
+    static constexpr int blocks = HD <= 64 ? 1 : 2;              // of 64 values: rows of 128 bytes as TMA's swizzle lays them out
+    static constexpr int block_bytes = kUnit * 128;
+    static constexpr int tile_bytes = blocks * block_bytes;      // K or V of one step
+    static constexpr int stages = blocks == 1 ? 4 : 3;           // 64 or 96 KB in flight per CTA, three or two CTAs per SM
+    static constexpr int smem_bytes = stages * 2 * tile_bytes + 1024 + 256;   // slack of the 1024-byte alignment, control words
 };
-// Byte offset of 16-byte piece c of row r: pieces are permuted inside groups of eight, so that ldmatrix and the copies are free of conflicts.
-template <int HD> __device__ __forceinline__ uint32_t piece_offset(int r, int c) {
-    return static_cast<uint32_t>(r * MmaShape<HD>::row_bytes + (((c & ~7) | ((c ^ r) & 7)) << 4));
+// Byte offset of 16-byte piece c of row r.
+__device__ __forceinline__ uint32_t piece_offset(int r, int c) { return static_cast<uint32_t>((c >> 3) * kUnit * 128 + r * 128 + (((c ^ r) & 7) << 4)); }
+__device__ __forceinline__ void mma_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kMmaWarps * 32) : "memory"); }
+__device__ __forceinline__ bool mma_any(bool mine) {
+    uint32_t any;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "n"(kMmaWarps * 32) : "memory");
+    return any != 0;
 }
 
 // Steps with keys that some pairs of the tile do not see: a weight of 0 does not cancel a value that is no number, so such values leave the tile
-// before the products, and are added here to the accumulators of the pairs that do see them.
-template <int HD> __device__ __noinline__ void move_values_out(unsigned char* value, int pieces, int begin, int warp_key, int keys, const int (&seen)[2], float (&acc)[HD / 8][4]) {
-    const int lane = threadIdx.x & 31, quad = lane & 3;
-    for (int k = warp_key; k < warp_key + keys; ++k)
-        for (int n = 0; n < pieces; ++n) {
-            const uint32_t two = *reinterpret_cast<const uint32_t*>(value + piece_offset<HD>(k, n) + 4 * quad);
-            const float v[2] = {bf16_lo(two), bf16_hi(two)};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!isfinite(v[e & 1]) && begin + k < seen[e >> 1]) {
-#pragma unroll
-                    for (int i = 0; i < HD / 8; ++i)
-                        if (i == n) acc[i][e] += v[e & 1];
-                }
-        }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kUnit * pieces * 8; i += kMmaThreads) {
-        uint16_t* x = reinterpret_cast<uint16_t*>(value + piece_offset<HD>(i / (pieces * 8), i / 8 % pieces)) + i % 8;
-        if ((*x & 0x7f80) == 0x7f80) *x = 0;
-    }
-    __syncthreads();
-}
-template <int HD> __device__ __forceinline__ void guard_values(const PrefixParams& p, const Item& it, unsigned char* value, int begin, int warp_key, int keys,
-                                                               const int (&seen)[2], float (&acc)[HD / 8][4]) {
-    const int pieces = p.dim / 8;
+// before the products, and are added to the accumulators of the pairs that do see them.
+template <int HD> __device__ __forceinline__ void guard_values(unsigned char* value, int pieces, int begin, int warp_key, int keys, const int (&seen)[2],
+                                                               float (&acc)[HD / 8][4]) {
+    constexpr int kThreads = kMmaWarps * 32;
     bool odd = false;
-    for (int i = threadIdx.x; i < kUnit * pieces; i += kMmaThreads) {
-        const uint4 x = *reinterpret_cast<const uint4*>(value + piece_offset<HD>(i / pieces, i % pieces));
+    for (int i = threadIdx.x; i < kUnit * pieces; i += kThreads) {
+        const uint4 x = *reinterpret_cast<const uint4*>(value + piece_offset(i / pieces, i % pieces));
         const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) odd |= (words[u] & 0x7f80u) == 0x7f80u || (words[u] & 0x7f800000u) == 0x7f800000u;
     }
-    if (__syncthreads_or(odd)) move_values_out<HD>(value, pieces, begin, warp_key, keys, seen, acc);
+    if (!mma_any(odd)) return;
+    const int quad = threadIdx.x & 3;
+    for (int k = warp_key; k < warp_key + keys; ++k)
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+            if (n >= pieces) continue;
+            const uint32_t two = *reinterpret_cast<const uint32_t*>(value + piece_offset(k, n) + 4 * quad);
+            const float v[2] = {bf16_lo(two), bf16_hi(two)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!isfinite(v[e & 1]) && begin + k < seen[e >> 1]) acc[n][e] += v[e & 1];
+        }
+    mma_barrier();
+    for (int i = threadIdx.x; i < kUnit * pieces * 8; i += kThreads) {
+        uint16_t* x = reinterpret_cast<uint16_t*>(value + piece_offset(i / (pieces * 8), i / 8 % pieces)) + i % 8;
+        if ((*x & 0x7f80) == 0x7f80) *x = 0;
+    }
+    mma_barrier();
 }
+
+struct MmaMaps { CUtensorMap own[2], prefix[2]; };   // K and V
 
 // SPLIT: a tile of 16 pairs, each warp takes 16 of the 64 keys of a step and the warps' results are joined at the end; otherwise a tile of 64 pairs,
 // 16 per warp, all of which use the same keys.
-template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) prefix_mma_kernel(const PrefixParams p) {
+template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
     using S = MmaShape<HD>;
-    extern __shared__ __align__(128) unsigned char mma_shared[];
+    extern __shared__ unsigned char mma_shared[];
     constexpr int kKeys = SPLIT ? 16 : 64;       // keys per warp and step
     constexpr int kTiles = kKeys / 8, kSteps = HD / 16, kColumns = HD / 8;
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mma_shared) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + S::stages * 2 * S::tile_bytes);
+    uint64_t* empty = full + S::stages;
+    volatile int* alive = reinterpret_cast<volatile int*>(empty + S::stages);
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    if (thread == 0) {
+        for (int i = 0; i < S::stages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kMmaWarps);
+        }
+        *alive = 1;
+        mbar_fence_init();
+    }
     begin_items(p);
     const Item it = find_item(p, first_item(p) + blockIdx.x);
+    __syncthreads();
     if (!it.live) return end_items(p);
-    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
-    const PagesView& view = it.causal ? p.own : p.prefix;
-    const uint32_t shared = smem_u32(mma_shared);
-    const int pieces = p.dim / 8;
-    if (pieces < S::slots && pieces < HD / 8) {   // the columns past the head's size stay zero
-        for (int i = thread; i < kMmaStages * 2 * kUnit * S::slots; i += kMmaThreads) {
-            const int r = i / S::slots, c = i % S::slots;
-            if (c >= pieces) *reinterpret_cast<uint4*>(mma_shared + r / kUnit * S::tile_bytes + piece_offset<HD>(r % kUnit, c)) = make_uint4(0, 0, 0, 0);
-        }
-    }
-    // Every thread copies piece `c` of the rows r0, r0 + rows_per_pass, ...; the page numbers of a step are fetched one step ahead of its copies.
-    const int c = thread % S::slots, r0 = thread / S::slots;
     const int steps = (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
-    const int64_t piece = static_cast<int64_t>(it.kv_head) * view.page_size * view.head_dim + c * 8;
-    int64_t at[S::passes];   // of the row in the pools, -1: zeros
-    auto fetch = [&](int step) {
-#pragma unroll
-        for (int i = 0; i < S::passes; ++i) {
-            const int position = it.keys.begin + step * kUnit + r0 + i * S::rows_per_pass;
-            at[i] = -1;
-            if (c < pieces && position < it.keys.end) {
+    // after a wait that ran out every role goes through the rest without waiting
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (*alive && !mbar_wait(bar, parity)) {
+            atomicExch(p.status, B200_DEVICE_TIMEOUT);
+            *alive = 0;
+        }
+    };
+    if (warp == kMmaWarps) {
+        const PagesView& view = it.causal ? p.own : p.prefix;
+        const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
+        const int boxes = kUnit / box_rows * S::blocks;                                      // at most 16 per tensor
+        const int which = lane / boxes, block = lane % S::blocks, row = lane % boxes / S::blocks * box_rows;
+        const CUtensorMap* map = it.causal ? &maps.own[which & 1] : &maps.prefix[which & 1];
+        int issued = 0;
+        for (; issued < steps; ++issued) {
+            const int stage = issued % S::stages, position = it.keys.begin + issued * kUnit + row;
+            int y = outside;
+            if (which < 2 && position < it.keys.end) {
                 const int page = page_of(view, it.slot, position / view.page_size);
-                if (page >= 0) at[i] = (static_cast<int64_t>(page) * view.kv_heads * view.page_size + position % view.page_size) * view.head_dim + piece;
+                if (page >= 0) y = (page * view.kv_heads + it.kv_head) * view.page_size + position % view.page_size;
             }
+            wait(&empty[stage], ((issued / S::stages) & 1) ^ 1);
+            if (!__all_sync(0xffffffffu, *alive != 0)) break;
+            if (lane == 0) mbar_expect_tx(&full[stage], 2 * S::tile_bytes);
+            __syncwarp();
+            if (which < 2) tma_load_2d(ring + (stage * 2 + which) * S::tile_bytes + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
         }
-    };
-    auto copy = [&](int step) {
-        const uint32_t stage = shared + step % kMmaStages * S::stage_bytes;
-        if (c < pieces) {
-#pragma unroll
-            for (int i = 0; i < S::passes; ++i) {
-                const uint32_t to = stage + piece_offset<HD>(r0 + i * S::rows_per_pass, c);
-                const bool live = at[i] >= 0;
-                const int64_t from = live ? at[i] : 0;
-                copy_async_16(to, static_cast<const __nv_bfloat16*>(view.pool[0]) + from, live);
-                copy_async_16(to + S::tile_bytes, static_cast<const __nv_bfloat16*>(view.pool[1]) + from, live);
-            }
-        }
-    };
-    fetch(0);
-    for (int step = 0; step < kMmaStages - 1; ++step) {
-        if (step < steps) {
-            copy(step);
-            fetch(step + 1);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (issued < steps)   // no copy is in flight when the CTA leaves
+            for (int j = max(0, issued - S::stages); j < issued; ++j) mbar_wait(&full[j % S::stages], (j / S::stages) & 1);
+        return end_items(p);
     }
     // query fragments
     const int quad = lane & 3, m0 = it.m_begin + (SPLIT ? 0 : warp * 16) + (lane >> 2);
@@ -265,25 +266,28 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
     const int warp_key = SPLIT ? warp * 16 : 0;
     const int first_limit = it.causal ? it.visible + it.m_begin / p.group : it.keys.end;   // keys that the tile's first pair sees
     for (int step = 0; step < steps; ++step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kMmaStages - 2) : "memory");
-        __syncthreads();
-        if (step + kMmaStages - 1 < steps) {
-            copy(step + kMmaStages - 1);
-            fetch(step + kMmaStages);
+        const int stage = step % S::stages, begin = it.keys.begin + step * kUnit;
+        wait(&full[stage], (step / S::stages) & 1);
+        unsigned char* values = ring + (stage * 2 + 1) * S::tile_bytes;
+        const uint32_t key = smem_u32(ring) + stage * 2 * S::tile_bytes, value = key + S::tile_bytes;
+        if (begin + kUnit > it.keys.end && it.keys.end % box_rows) {
+            // rows of the last box behind the keys may hold anything
+            const int from = it.keys.end - begin, behind = (from + box_rows - 1) / box_rows * box_rows - from;
+            for (int i = thread; i < behind * 8 * S::blocks; i += kMmaWarps * 32)
+                *reinterpret_cast<uint4*>(values + i / (behind * 8) * S::block_bytes + from * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
+            mma_barrier();
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        const uint32_t key = shared + step % kMmaStages * S::stage_bytes, value = key + S::tile_bytes;
         float score[kTiles][4] = {};
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
             for (int n = 0; n < kTiles; n += 2) {
                 uint32_t b[4];   // keys n*8 .. +7 and +8 .. +15, both halves of the 16 values
-                ldsm_x4(b, key + piece_offset<HD>(warp_key + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                ldsm_x4(b, key + piece_offset(warp_key + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
                 mma_16816(score[n], q[k], b[0], b[1]);
                 mma_16816(score[n + 1], q[k], b[2], b[3]);
             }
-        const int first_key = it.keys.begin + step * kUnit + warp_key + 2 * quad;
+        const int first_key = begin + warp_key + 2 * quad;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             float top = most[r];
@@ -315,8 +319,7 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
                 acc[n][2 * r + 1] *= shrink;
             }
         }
-        if (min(it.keys.end, it.keys.begin + (step + 1) * kUnit) > first_limit)
-            guard_values<HD>(p, it, mma_shared + (value - shared), it.keys.begin + step * kUnit, warp_key, kKeys, seen, acc);
+        if (min(it.keys.end, begin + kUnit) > first_limit) guard_values<HD>(values, p.dim / 8, begin, warp_key, kKeys, seen, acc);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k) {
             const uint32_t a[4] = {pack_bf16(score[2 * k][0], score[2 * k][1]), pack_bf16(score[2 * k][2], score[2 * k][3]),
@@ -324,22 +327,23 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
 #pragma unroll
             for (int n = 0; n < kColumns; n += 2) {
                 uint32_t b[4];
-                ldsm_x4_trans(b, value + piece_offset<HD>(warp_key + 16 * k + (lane & 15), n + (lane >> 4)));
+                ldsm_x4_trans(b, value + piece_offset(warp_key + 16 * k + (lane & 15), n + (lane >> 4)));
                 mma_16816(acc[n], a, b[0], b[1]);
                 mma_16816(acc[n + 1], a, b[2], b[3]);
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
     }
     if constexpr (SPLIT) {
-        // join the warps: [warp][16 rows][HD] accumulators behind [warp][16][2] maxima and sums
-        __syncthreads();
-        float* joined = reinterpret_cast<float*>(mma_shared);
+        // join the warps, in the ring that nothing is copied to any more: [warp][16 rows][HD] accumulators behind [warp][16][2] maxima and sums
+        mma_barrier();
+        float* joined = reinterpret_cast<float*>(ring);
         float* rows_of = joined + 4 * 16 * 2;
         constexpr int kPitch = HD + 4;
 #pragma unroll
@@ -353,9 +357,9 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
             for (int n = 0; n < kColumns; ++n)
                 *reinterpret_cast<float2*>(rows_of + (warp * 16 + m) * kPitch + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
         }
-        __syncthreads();
+        mma_barrier();
         const int live = min(16, it.m_count - it.m_begin);
-        for (int i = thread; i < live * (HD / 4); i += kMmaThreads) {
+        for (int i = thread; i < live * (HD / 4); i += kMmaWarps * 32) {
             const int m = i / (HD / 4), d = i % (HD / 4) * 4;
             float top = -INFINITY, total = 0.0f;
 #pragma unroll
@@ -389,37 +393,77 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------------------------
-// A warp per row and head.
-__global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p) {
+constexpr int kMergeWarps = 4, kMostSplits = 64;
+
+// A warp per row and head.  V = 4 (head sizes of 4 n): a group of `lanes` lanes reads one partial result at 16 bytes per lane, the warp's groups take
+// turns over the splits and are added at the end.
+template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const PrefixParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
-    const int64_t index = blockIdx.x * 4 + static_cast<int64_t>(threadIdx.x >> 5);
+    const int64_t index = blockIdx.x * static_cast<int64_t>(kMergeWarps) + static_cast<int64_t>(threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const int row = static_cast<int>(index / p.heads);
-    if (row >= min(p.rows.rows, __ldg(p.rows.first + p.rows.sequences))) return;
-    const int s = __ldg(p.rows.sequence + row), g = group_of(p, s);
+    if (row >= p.rows.rows || row >= __ldg(p.rows.first + p.rows.sequences)) return;
+    const int s = __ldg(p.rows.sequence + row);
+    const int slot = __ldg(p.rows.slot + s), count = __ldg(p.rows.first + s + 1) - __ldg(p.rows.first + s);
+    int g = -1;
+    for (int base = 0; base < p.groups; base += 32) {
+        const int c = base + lane;
+        const unsigned found = __ballot_sync(0xffffffffu, c < p.groups && __ldg(p.group_first + c) <= s && s < __ldg(p.group_first + c + 1));
+        if (found) {
+            g = base + __ffs(found) - 1;
+            break;
+        }
+    }
     const int from_prefix = g < 0 ? 0 : used_splits(prefix_keys(p, g), p.prefix_splits);
-    const int from_own = used_splits(own_keys(p, __ldg(p.rows.slot + s), __ldg(p.rows.first + s + 1) - __ldg(p.rows.first + s)), p.own_splits);
-    const int parts = from_prefix + from_own;
+    const int parts = from_prefix + used_splits(own_keys(p, slot, count), p.own_splits);
     const int64_t base = index * (p.prefix_splits + p.own_splits);
-    auto place = [&](int i) { return base + (i < from_prefix ? i : p.prefix_splits + i - from_prefix); };
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[2 * place(i)]);
+    const int skip = p.prefix_splits - from_prefix;
+    constexpr int kHeld = 2 * kMostSplits / 32;
+    float most[kHeld], weight[kHeld], top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int i = 32 * j + lane;
+        const float2 ml = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (base + i + (i < from_prefix ? 0 : skip))) : make_float2(-INFINITY, 0.0f);
+        most[j] = ml.x;
+        weight[j] = ml.y;
+        top = fmaxf(top, ml.x);
+    }
     top = warp_max(top);
-    float total = 0.0f;
-    if (top > -INFINITY)
-        for (int i = lane; i < parts; i += 32) total += exp2f(p.part_ml[2 * place(i)] - top) * p.part_ml[2 * place(i) + 1];
+    const float zero = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const float f = exp2f(most[j] - zero);
+        total += f * weight[j];
+        weight[j] = f;
+    }
     total = warp_sum(total);
-    const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+    // a row that sees nothing gives zeros; one whose weights are no numbers gives no numbers
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const int pieces = p.dim / V;
+    const int lanes = pieces >= 32 ? 32 : pieces > 16 ? 32 : pieces > 8 ? 16 : 8, groups = 32 / lanes, turn = lane / lanes;
     const int64_t to = row * p.out_stride + index % p.heads * p.dim;
-    for (int d = lane; d < p.dim; d += 32) {
-        float o = 0.0f;
-        if (top > -INFINITY)
-            for (int i = 0; i < parts; ++i) {
-                const float f = exp2f(p.part_ml[2 * place(i)] - top);
-                if (f > 0.0f) o += f * p.part_o[place(i) * p.dim + d];
+    for (int d = lane % lanes; d - lane % lanes < pieces; d += lanes) {
+        Lanes<V> o{};
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+#pragma unroll 8
+            for (int i = 0; i < 32; i += groups) {
+                if (32 * j + i >= parts) break;
+                const int part = 32 * j + i + turn;
+                const float f = __shfl_sync(0xffffffffu, weight[j], i + turn);
+                if (part < parts && d < pieces && f != 0.0f) {
+                    const Lanes<V> v = load_lanes<V>(p.part_o + (base + part + (part < from_prefix ? 0 : skip)) * p.dim + d * V);
+#pragma unroll
+                    for (int u = 0; u < V; ++u) o.v[u] += f * v.v[u];
+                }
             }
-        store_forms(o * inverse, to + d, p.out, p.out_hi, p.out_lo);
+        }
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            for (int x = lanes; x < 32; x *= 2) o.v[u] += __shfl_xor_sync(0xffffffffu, o.v[u], x);
+            if (turn == 0 && d < pieces) store_forms(o.v[u] * inverse, to + d * V + u, p.out, p.out_hi, p.out_lo);
+        }
     }
 }
 
@@ -433,6 +477,10 @@ struct Plan {
     int prefix_rows, own_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
 };
 
+bool mma_takes(const b200_kv_pages& pages) {
+    return pages.head_dim % 8 == 0 && pages.head_dim <= 128 && pages.page_size % 8 == 0 && pages.pages * pages.kv_heads * pages.page_size < INT32_MAX;
+}
+
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length, int max_prefix) {
@@ -440,7 +488,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     const int kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
     uintptr_t bits = reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.cache.key) | reinterpret_cast<uintptr_t>(a.cache.value);
     if (a.groups) bits |= reinterpret_cast<uintptr_t>(a.prefix.key) | reinterpret_cast<uintptr_t>(a.prefix.value);
-    const bool mma = a.cache.dtype == B200_BF16 && a.cache.head_dim % 8 == 0 && a.cache.head_dim <= 128 && bits % 16 == 0;
+    const bool mma = a.cache.dtype == B200_BF16 && mma_takes(a.cache) && (!a.groups || mma_takes(a.prefix)) && bits % 16 == 0;
     const int64_t pairs = pass.rows * group;
     const int groups = a.groups < pass.sequences ? a.groups : pass.sequences;
     const bool prefix = a.groups > 0 && max_prefix > 0;
@@ -457,7 +505,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
         const int most = ceil_div(keys, 4 * kUnit);
         int n = static_cast<int>(ctas / (items > 0 ? items : 1));
         if (n > most) n = most;
-        if (n > 64) n = 64;
+        if (n > kMostSplits) n = kMostSplits;
         return n < 1 ? 1 : n;
     };
     // tiles that the rows fill: the last tile of every group is counted half
@@ -496,12 +544,17 @@ template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned item
     return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p);
 }
 
-template <int HD> cudaError_t launch_mma(const PrefixParams& p, unsigned items, cudaStream_t stream) {
+template <int HD> int launch_mma(const PrefixParams& p, unsigned items, cudaStream_t stream) {
     auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, true> : prefix_mma_kernel<HD, false>;
     constexpr int smem = MmaShape<HD>::smem_bytes;
-    const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (status != cudaSuccess) return status;
-    return launch_dependent(kernel, dim3(items), dim3(kMmaThreads), static_cast<size_t>(smem), stream, p);
+    MmaMaps maps;
+    int box_rows = page_box_rows(p.own.page_size);
+    if (p.groups && !p.beside) box_rows = std::min(box_rows, page_box_rows(p.prefix.page_size));   // powers of two
+    int status = page_maps(p.own, box_rows, maps.own);
+    if (status == B200_OK && p.groups && !p.beside) status = page_maps(p.prefix, box_rows, maps.prefix);
+    if (status != B200_OK) return status;
+    B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return cuda_status(launch_dependent(kernel, dim3(items), dim3(kMmaThreads), static_cast<size_t>(smem), stream, maps, p, box_rows), "prefix_mma_kernel launch");
 }
 
 }  // namespace
@@ -545,28 +598,30 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     p.out_stride = out_stride ? out_stride : width;
     const int64_t prefix_items = static_cast<int64_t>(plan.prefix_tiles) * plan.prefix_splits * a->cache.kv_heads;
     const int64_t own_items = static_cast<int64_t>(pass->sequences) * plan.own_tiles * plan.own_splits * a->cache.kv_heads;
-    const int64_t merges = (pass->rows * a->heads + 3) / 4;
+    const int64_t merges = (pass->rows * a->heads + kMergeWarps - 1) / kMergeWarps;
     if (prefix_items + own_items > INT32_MAX || merges > INT32_MAX || static_cast<int64_t>(pass->rows) * p.group > INT32_MAX / 2) {
         set_error("b200_prefix_attention: too many rows");
         return B200_UNSUPPORTED;
     }
     cudaStream_t s = as_stream(stream);
-    if (plan.tensor) {
+    int status;
+    if (plan.form == Form::mma) {
         int device = 0;
         B200_CUDA(cudaGetDevice(&device));
         p.status = device_status_word(device);
         if (!p.status) { set_error("b200_prefix_attention: the device status word could not be allocated"); return B200_NO_DEVICE; }
-        const int status = launch_prefix_tensor(p, static_cast<int>(prefix_items), s);
+    }
+    if (plan.tensor) {
+        status = launch_prefix_tensor(p, static_cast<int>(prefix_items), s);
         if (status != B200_OK) return status;
         p.beside = 1;
     }
     const unsigned items = static_cast<unsigned>(plan.tensor ? own_items : prefix_items + own_items);
-    cudaError_t launched;
-    if (plan.form == Form::plain) launched = a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, s) : launch_plain<float>(p, items, s);
-    else if (p.dim <= 64) launched = launch_mma<64>(p, items, s);
-    else if (p.dim <= 96) launched = launch_mma<96>(p, items, s);
-    else launched = launch_mma<128>(p, items, s);
-    const int status = cuda_status(launched, "b200_prefix_attention launch");
+    if (plan.form == Form::plain)
+        status = cuda_status(a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, s) : launch_plain<float>(p, items, s), "prefix_plain_kernel launch");
+    else
+        status = p.dim <= 64 ? launch_mma<64>(p, items, s) : p.dim <= 96 ? launch_mma<96>(p, items, s) : launch_mma<128>(p, items, s);
     if (status != B200_OK) return status;
-    return cuda_status(launch_dependent(prefix_merge_kernel, dim3(static_cast<unsigned>(merges)), dim3(128), 0, s, p), "prefix_merge_kernel launch");
+    auto merge = p.dim % 4 == 0 ? prefix_merge_kernel<4> : prefix_merge_kernel<1>;
+    return cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(merges)), dim3(kMergeWarps * 32), 0, s, p), "prefix_merge_kernel launch");
 }

@@ -29,6 +29,16 @@ template <int HD> struct TensorShape {
     static constexpr uint32_t sums = mma_instruction_bf16(128, HD) | kTransposedB;
 };
 
+// Scores behind the last key weigh nothing.
+__device__ __forceinline__ void hide_scores(uint32_t (&s)[2][32], int live) {
+    if (live >= 64) return;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= live) s[c][i] = 0xff800000u;   // -inf
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                                                                           const PrefixParams p, const int box_rows) {
@@ -173,15 +183,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
         {
             const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
             constexpr int kPieces = 8 * S::blocks;
-            for (int i = row; i < 128 * kPieces; i += 128) {
-                const int r = i / kPieces, c = i % kPieces, m = m_tile + r;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (m < it.m_count) {
-                    x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query)
-                                                             + ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * HD + 8 * c));
-                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+#pragma unroll
+            for (int first = 0; first < kPieces; first += 8) {
+                uint4 x[8];   // requested together
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int i = (first + u) * 128 + row, c = i % kPieces, m = m_tile + i / kPieces;
+                    x[u] = make_uint4(0, 0, 0, 0);
+                    if (m < it.m_count)
+                        x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query)
+                                                                    + ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * HD + 8 * c));
                 }
-                *reinterpret_cast<uint4*>(smem + t * S::tile_bytes + c / 8 * S::block_bytes + r * 128 + (((c ^ r) & 7) << 4)) = x;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int i = (first + u) * 128 + row, c = i % kPieces, r = i / kPieces;
+                    x[u].x ^= flip; x[u].y ^= flip; x[u].z ^= flip; x[u].w ^= flip;
+                    *reinterpret_cast<uint4*>(smem + t * S::tile_bytes + c / 8 * S::block_bytes + r * 128 + (((c ^ r) & 7) << 4)) = x[u];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(q_ready);
@@ -195,25 +213,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             going = wait(&s_full[t], step & 1);
             if (!going) break;
             tc_fence_after_sync();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_load_32_async(s_at + 32 * c, s[c]);
-            tmem_wait_loads();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
+            // two looks at the scores: holding all 128 of a row between the maximum and the weights would take too many registers
             const int live = min(kTensorKeys, it.keys.end - it.keys.begin - step * kTensorKeys);
-            if (live < kTensorKeys) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * c + i >= live) s[c][i] = 0xff800000u;   // -inf
-            }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int half = 0; half < 2; ++half) {
+                uint32_t s[2][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                for (int c = 0; c < 2; ++c) tmem_load_32_async(s_at + 64 * half + 32 * c, s[c]);
+                tmem_wait_loads();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) tmem_loaded(s[c]);
+                hide_scores(s, live - 64 * half);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[c / 2][i + c % 2]));
+            }
             const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
             const bool grows = here > most + kLazy;
             if (__any_sync(0xffffffffu, grows)) {
@@ -238,17 +254,24 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                uint32_t weights[32];
+                uint32_t s[2][32], weights[32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) tmem_load_32_async(s_at + 64 * half + 32 * c, s[c]);
+                tmem_wait_loads();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) tmem_loaded(s[c]);
+                hide_scores(s, live - 64 * half);
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float a = exp2_fast(fmaf(__uint_as_float(s[2 * half + c][i]), scale, base));
-                        const float b = exp2_fast(fmaf(__uint_as_float(s[2 * half + c][i + 1]), scale, base));
+                        const float a = exp2_fast(fmaf(__uint_as_float(s[c][i]), scale, base));
+                        const float b = exp2_fast(fmaf(__uint_as_float(s[c][i + 1]), scale, base));
                         add[(i / 2) & 1] += a;
                         add[2 + ((i / 2) & 1)] += b;
                         weights[16 * c + i / 2] = pack_bf16(a, b);
                     }
+                // the columns of scores that both looks are done with
                 tmem_store_32(s_at + 32 * half, weights);
             }
             sum += (add[0] + add[1]) + (add[2] + add[3]);
@@ -281,26 +304,11 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     }
 }
 
-// Rows of a TMA box: a part of a page of at most 64 rows whose multiples are the tiles' and the pages' borders.
-int box_rows_of(int page_size) {
-    for (int rows = 64; rows >= 8; rows /= 2)
-        if (page_size % rows == 0) return rows;
-    return 0;
-}
-
 template <int HD> int launch_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
-    encode_tiled_fn encode = tensor_map_encoder();
-    if (!encode) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return B200_NO_DEVICE; }
-    const int box_rows = box_rows_of(p.prefix.page_size);
-    const cuuint64_t dims[2] = {HD, static_cast<cuuint64_t>(p.prefix.pages) * p.prefix.kv_heads * p.prefix.page_size};
-    const cuuint64_t strides[1] = {HD * 2};
-    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, ones[2] = {1, 1};
+    const int box_rows = page_box_rows(p.prefix.page_size);
     CUtensorMap maps[2];
-    for (int which = 0; which < 2; ++which) {
-        const CUresult result = encode(&maps[which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.prefix.pool[which], dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (result != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with %d", static_cast<int>(result)); return B200_BAD_ARGUMENT; }
-    }
+    const int status = page_maps(p.prefix, box_rows, maps);
+    if (status != B200_OK) return status;
     auto kernel = prefix_tensor_kernel<HD>;
     B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TensorShape<HD>::smem_bytes));
     return cuda_status(launch_dependent(kernel, dim3(static_cast<unsigned>(items)), dim3(kTensorThreads), TensorShape<HD>::smem_bytes, stream, maps[0], maps[1], p, box_rows),
@@ -309,9 +317,28 @@ template <int HD> int launch_tensor(const PrefixParams& p, int items, cudaStream
 
 }  // namespace
 
+int page_box_rows(int page_size) {
+    for (int rows = 64; rows >= 8; rows /= 2)
+        if (page_size % rows == 0) return rows;
+    return 0;
+}
+
+int page_maps(const PagesView& pages, int box_rows, CUtensorMap* maps) {
+    encode_tiled_fn encode = tensor_map_encoder();
+    if (!encode) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return B200_NO_DEVICE; }
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(pages.head_dim), static_cast<cuuint64_t>(pages.pages) * pages.kv_heads * pages.page_size};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pages.head_dim) * 2};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, ones[2] = {1, 1};
+    for (int which = 0; which < 2; ++which) {
+        const CUresult result = encode(&maps[which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages.pool[which], dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (result != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with %d", static_cast<int>(result)); return B200_BAD_ARGUMENT; }
+    }
+    return B200_OK;
+}
+
 bool prefix_tensor_takes(const b200_kv_pages& prefix, float scale) {
-    return prefix.dtype == B200_BF16 && (prefix.head_dim == 64 || prefix.head_dim == 128) && box_rows_of(prefix.page_size) > 0 && scale != 0.0f
-           && prefix.pages * prefix.kv_heads * prefix.page_size < INT32_MAX;
+    return (prefix.head_dim == 64 || prefix.head_dim == 128) && scale != 0.0f;
 }
 
 int launch_prefix_tensor(const PrefixParams& p, int items, cudaStream_t stream) {

@@ -7,7 +7,12 @@ namespace b200 {
 
 constexpr int kTensorRows = 256, kTensorKeys = 128;   // (row, head) pairs of a CTA, keys of a step
 
-// Whether the kernel can take a prefix (16-byte aligned pools).
+// Rows of a TMA box of a page: a part of it of at most 64 rows, at least 8; 0 where there is none.
+int page_box_rows(int page_size);
+// Tensor maps of the keys and the values: rows of a page's head, 64 values x box_rows at a time.
+int page_maps(const PagesView& pages, int box_rows, CUtensorMap* maps);
+
+// Whether the kernel takes a prefix that prefix_mma_kernel takes.
 bool prefix_tensor_takes(const b200_kv_pages& prefix, float scale);
 // Items of the prefix alone; p.prefix_rows is kTensorRows.
 int launch_prefix_tensor(const PrefixParams& p, int items, cudaStream_t stream);

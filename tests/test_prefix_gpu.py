@@ -270,6 +270,25 @@ def test_attention(name, spread):
     assert (np.abs(planes + host(lo)[:state.live, :width].reshape(want.shape) - got) <= BF16_STEP ** 2 * np.abs(got) + 1e-38).all()
 
 
+@pytest.mark.parametrize("counts", [[1, 1], [3, 9], [40, 20]])
+@pytest.mark.parametrize("own_page,prefix_page", [(16, 64), (128, 24), (7, 32), (32, 9)])
+def test_prefix_and_cache_with_pages_of_their_own(own_page, prefix_page, counts):
+    rng = np.random.default_rng(own_page)
+    lengths, length = [30, 61], 150
+    span, prefix_span = -(-110 // own_page), -(-length // prefix_page)
+    cache = Paged("bf16", 2, own_page, 64, 2 * span, rng.permutation(2 * span).reshape(2, span), rng)
+    prefix = Paged("bf16", 2, prefix_page, 64, prefix_span, rng.permutation(prefix_span).reshape(1, prefix_span), rng)
+    state = Pass(counts, [1, 0], lengths)
+    cache.spoil([lengths[0] + counts[1], lengths[1] + counts[0]])
+    prefix.spoil([length])
+    query = dev(rng.standard_normal((state.rows, 8, 64), dtype=np.float32), torch.bfloat16)
+    of = dict(heads=8, dim=64, prefixes=[length], group_first=[0, 2], group_prefix=[0], dtype="bf16", max_length=110, max_prefix=length)
+    out = torch.empty((state.rows, 512), device="cuda")
+    Attention(state, cache, prefix, query, of)(out)
+    want, mass, size, keys = wanted(state, cache, prefix, query, of)
+    assert (np.abs(host(out).reshape(want.shape) - want) <= attention_bound(of, mass, size, keys)).all()
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-6, 0.7])
 @pytest.mark.parametrize("name", ["drafts", "many rows", "heads of 80", "f32"])
 def test_scales(name, scale):
