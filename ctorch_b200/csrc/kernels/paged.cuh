@@ -18,6 +18,39 @@ __device__ __forceinline__ int page_of(const PagesView& v, int sequence, int log
     const int page = __ldg(v.table + static_cast<int64_t>(sequence) * v.pages_per_seq + logical);
     return page >= 0 && page < v.pages ? page : -1;
 }
+// Pool rows of the positions from, from + stride, ... of a sequence, as a copying warp walks them.  Page numbers are asked for two steps before they are
+// wanted, since the way to L2 and back is longer than a step; places in the table and the page move on without divisions.
+struct PageStream {
+    const PagesView& view;
+    const int32_t* table;
+    int index, place, whole, rest, position, stride, end;   // index and place of the position that is asked for next
+    int number[2], at[2];
+    __device__ __forceinline__ PageStream(const PagesView& view, int sequence, int from, int stride, int end)
+        : view(view), table(view.table + static_cast<int64_t>(sequence) * view.pages_per_seq), index(from / view.page_size), place(from % view.page_size),
+          whole(stride / view.page_size), rest(stride % view.page_size), position(from), stride(stride), end(end) {
+        ask(0);
+        ask(1);
+    }
+    __device__ __forceinline__ void ask(int i) {
+        number[i] = position < end ? __ldg(table + index) : -1;
+        at[i] = place;
+        position += stride;
+        index += whole;
+        place += rest;
+        if (place >= view.page_size) {
+            place -= view.page_size;
+            ++index;
+        }
+    }
+    // Row of the pools' [pages * kv_heads * page_size] rows that holds the next position; `outside` where there is none.
+    __device__ __forceinline__ int next(int head, int outside) {
+        const int page = number[0], row = at[0];
+        number[0] = number[1];
+        at[0] = at[1];
+        ask(1);
+        return page >= 0 && page < view.pages ? (page * view.kv_heads + head) * view.page_size + row : outside;
+    }
+};
 // First element of one head's row in a page.
 __device__ __forceinline__ int64_t page_row(const PagesView& v, int page, int head, int slot) {
     return ((static_cast<int64_t>(page) * v.kv_heads + head) * v.page_size + slot) * v.head_dim;

@@ -222,22 +222,22 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) pre
     if (warp == kMmaWarps) {
         const PagesView& view = it.causal ? p.own : p.prefix;
         const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
-        const int boxes = kUnit / box_rows * S::blocks;                                      // at most 16 per tensor
-        const int which = lane / boxes, block = lane % S::blocks, row = lane % boxes / S::blocks * box_rows;
+        const int across = boxes_per_row(box_rows, p.dim), boxes = kUnit / box_rows * across;   // at most 16 per tensor
+        const int which = lane / boxes, block = lane % across, row = lane % boxes / across * box_rows;
         const CUtensorMap* map = it.causal ? &maps.own[which & 1] : &maps.prefix[which & 1];
+        PageStream pages(view, it.slot, it.keys.begin + row, kUnit, which < 2 ? it.keys.end : 0);
         int issued = 0;
         for (; issued < steps; ++issued) {
-            const int stage = issued % S::stages, position = it.keys.begin + issued * kUnit + row;
-            int y = outside;
-            if (which < 2 && position < it.keys.end) {
-                const int page = page_of(view, it.slot, position / view.page_size);
-                if (page >= 0) y = (page * view.kv_heads + it.kv_head) * view.page_size + position % view.page_size;
-            }
+            const int stage = issued % S::stages, y = pages.next(it.kv_head, outside);
             wait(&empty[stage], ((issued / S::stages) & 1) ^ 1);
             if (!__all_sync(0xffffffffu, *alive != 0)) break;
             if (lane == 0) mbar_expect_tx(&full[stage], 2 * S::tile_bytes);
             __syncwarp();
-            if (which < 2) tma_load_2d(ring + (stage * 2 + which) * S::tile_bytes + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
+            unsigned char* to = ring + (stage * 2 + which) * S::tile_bytes;
+            if (which < 2) {
+                if (across < S::blocks) tma_load_3d(to, map, 0, y, 0, &full[stage]);
+                else tma_load_2d(to + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
+            }
         }
         if (issued < steps)   // no copy is in flight when the CTA leaves
             for (int j = max(0, issued - S::stages); j < issued; ++j) mbar_wait(&full[j % S::stages], (j / S::stages) & 1);

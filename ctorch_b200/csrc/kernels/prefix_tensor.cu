@@ -1,11 +1,11 @@
 // The shared prefix of b200_prefix_attention on tcgen05: groups with many rows.
 //
-// A CTA has two tiles of 128 (row, head) pairs and a span of keys, 128 at a time.  Per tile and step: S = Q K^T into tensor memory (128 x 128 f32),
-// a softmax warpgroup - a thread per pair - turns S into bf16 weights P in the same columns, O += P V with P read from tensor memory.  The tensor
-// cores work on one tile while the other's softmax runs.
+// A CTA has two tiles of 128 (row, head) pairs and a span of keys, 64 at a time.  Per tile and step: S = Q K^T into tensor memory (128 x 64 f32),
+// a softmax warpgroup - a thread per pair - turns S into bf16 weights P in the same columns, O += P V with P read from tensor memory.  Each tile has two
+// such buffers of scores, so that its softmax works on one while the products of the other are under way, and the two tiles share the tensor cores.
 //   warps 0-3, 4-7   softmax of tile 0 and 1 (lane quarter = warp % 4), at the end the tile's partial result
 //   warp 8           copies K and V steps through a ring of shared-memory slots with TMA, page by page
-//   warp 9           tensor memory and all products
+//   warps 9, 10      all products of tile 0 and 1 (a product keeps its issuing warp as long as the tensor cores); warp 9 also has the tensor memory
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the maximum its weights are relative to: they
 // are relative to the same one in the sum and in O, so the quotient is the softmax all the same, and weights up to 2^8 lose nothing in f32 and bf16.
 #include "mma.cuh"
@@ -16,22 +16,26 @@
 namespace b200 {
 namespace {
 
-constexpr int kTensorThreads = 320;
+constexpr int kTensorThreads = 352;
 constexpr float kLazy = 8.0f;
 
 template <int HD> struct TensorShape {
     static constexpr int blocks = HD / 64;                          // 64 values: one swizzled row of 128 bytes
-    static constexpr int block_bytes = kTensorKeys * 128;
-    static constexpr int tile_bytes = blocks * block_bytes;         // 128 rows of Q, K or V
-    static constexpr int slots = HD == 128 ? 5 : 8;
-    static constexpr int smem_bytes = (2 + slots) * tile_bytes + 1024 + 1024;   // slack of the 1024-byte alignment, control words
+    static constexpr int query_block = 128 * 128, key_block = kTensorKeys * 128;
+    static constexpr int query_bytes = blocks * query_block;        // a tile's queries
+    static constexpr int step_bytes = blocks * key_block;           // K or V of a step
+    static constexpr int slots = 10;
+    static constexpr int smem_bytes = 2 * query_bytes + slots * step_bytes + 1024 + 1024;   // slack of the 1024-byte alignment, control words
     static constexpr uint32_t scores = mma_instruction_bf16(128, kTensorKeys);
     static constexpr uint32_t sums = mma_instruction_bf16(128, HD) | kTransposedB;
 };
+// The ring carries K0, K1, V0, K2, V1, ...: scores run ahead of the values by a step.
+__device__ __forceinline__ int key_item(int step) { return step ? 2 * step - 1 : 0; }
+__device__ __forceinline__ int value_item(int step, int steps) { return step + 1 < steps ? 2 * step + 2 : 2 * steps - 1; }
 
 // Scores behind the last key weigh nothing.
 __device__ __forceinline__ void hide_scores(uint32_t (&s)[2][32], int live) {
-    if (live >= 64) return;
+    if (live >= kTensorKeys) return;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -45,16 +49,16 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     using S = TensorShape<HD>;
     extern __shared__ uint8_t tensor_shared[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tensor_shared) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* ring = smem + 2 * S::tile_bytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(ring + S::slots * S::tile_bytes);
+    uint8_t* ring = smem + 2 * S::query_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + S::slots * S::step_bytes);
     uint64_t* empty = full + S::slots;
     uint64_t* q_ready = empty + S::slots;
-    uint64_t* s_full = q_ready + 1;     // [2] S of a step is in tensor memory
-    uint64_t* p_ready = s_full + 2;     // [2] the weights of a step are
-    uint64_t* o_done = p_ready + 2;     // [2] a step's values are added to O
-    uint64_t* tail = o_done + 2;        // what the last step's pages hold behind its keys is zeroed
+    uint64_t* s_full = q_ready + 2;     // [tile][step & 1] S of a step is in tensor memory
+    uint64_t* p_ready = s_full + 4;     // [tile][step & 1] the weights of a step are
+    uint64_t* o_done = p_ready + 4;     // [tile][step & 1] a step's values are added to O
+    uint64_t* tail = o_done + 4;        // what the last step's pages hold behind its keys is zeroed
     uint64_t* drained = tail + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
     volatile int* alive = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -68,16 +72,16 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::slots; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], tiles);
         }
-        mbar_init(q_ready, 128 * tiles);
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(&s_full[t], 1);
-            mbar_init(&p_ready[t], 128);
-            mbar_init(&o_done[t], 1);
+        for (int t = 0; t < 2; ++t) mbar_init(&q_ready[t], 4);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_ready[i], 4);
+            mbar_init(&o_done[i], 1);
         }
         mbar_init(tail, 1);
-        mbar_init(drained, 1);
+        for (int t = 0; t < 2; ++t) mbar_init(&drained[t], 1);
         *alive = 1;
         mbar_fence_init();
     }
@@ -91,6 +95,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     const uint32_t tmem = *tmem_slot;
     // for whole warps; every wait ends: after a limit, or when another role has given up
     auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
         if (!mbar_wait(bar, parity)) {
             atomicExch(p.status, B200_DEVICE_TIMEOUT);
             *alive = 0;
@@ -99,24 +104,28 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     };
 
     if (warp == 8) {
-        const int per_head = p.prefix.page_size, heads = p.prefix.kv_heads;
-        const int outside = static_cast<int>(p.prefix.pages) * heads * per_head;   // a row past the pools: zeros
-        int issued = 0;
+        const int outside = static_cast<int>(p.prefix.pages) * p.prefix.kv_heads * p.prefix.page_size;   // a row past the pools: zeros
+        const int across = boxes_per_row(box_rows, HD), boxes = kTensorKeys / box_rows * across;   // at most 16
+        const int block = lane % across, row = lane / across * box_rows;
+        PageStream pages(p.prefix, it.slot, it.keys.begin + row, kTensorKeys, lane < boxes ? it.keys.end : 0);
+        int issued = 0, key_row = outside, value_row = outside;
         for (int j = 0; j < 2 * steps; ++j, ++issued) {
-            const int slot = j % S::slots, step = j / 2;
+            const int slot = j % S::slots;
+            const bool values = j == 2 * steps - 1 || (j > 0 && j % 2 == 0);
+            if (!values) {
+                value_row = key_row;   // the values of a step come behind the keys of the next
+                key_row = pages.next(it.kv_head, outside);
+            }
+            const int y = !values || j == 2 * steps - 1 ? key_row : value_row;
             if (!wait(&empty[slot], ((j / S::slots) & 1) ^ 1)) break;
-            if (lane == 0) mbar_expect_tx(&full[slot], S::tile_bytes);
+            if (lane == 0) mbar_expect_tx(&full[slot], S::step_bytes);
             __syncwarp();
-            const int boxes = kTensorKeys / box_rows * S::blocks;   // at most 32
-            if (lane < boxes) {
-                const int block = lane % S::blocks, row = lane / S::blocks * box_rows;
-                const int position = it.keys.begin + step * kTensorKeys + row;
-                int y = outside;
-                if (position < it.keys.end) {
-                    const int page = page_of(p.prefix, it.slot, position / per_head);
-                    if (page >= 0) y = (page * heads + it.kv_head) * per_head + position % per_head;
-                }
-                tma_load_2d(ring + slot * S::tile_bytes + block * S::block_bytes + row * 128, j & 1 ? &value_map : &key_map, block * 64, y, &full[slot]);
+            uint8_t* to = ring + slot * S::step_bytes;
+            const CUtensorMap* map = values ? &value_map : &key_map;
+            if (across < S::blocks) {
+                if (lane == 0) tma_load_3d(to, map, 0, y, 0, &full[slot]);
+            } else if (lane < boxes) {
+                tma_load_2d(to + block * S::key_block + row * 128, map, block * 64, y, &full[slot]);
             }
             __syncwarp();
         }
@@ -126,7 +135,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             if (wait(&full[slot], (j / S::slots) & 1)) {
                 const int behind = (last_keys + box_rows - 1) / box_rows * box_rows - last_keys;
                 for (int i = lane; i < behind * 8 * S::blocks; i += 32)
-                    *reinterpret_cast<uint4*>(ring + slot * S::tile_bytes + i / (behind * 8) * S::block_bytes + last_keys * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(ring + slot * S::step_bytes + i / (behind * 8) * S::key_block + last_keys * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tail);
@@ -134,47 +143,50 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
         }
         if (*alive == 0)   // no copy is in flight when the CTA leaves
             for (int j = max(0, issued - S::slots); j < issued; ++j) mbar_wait(&full[j % S::slots], (j / S::slots) & 1);
-    } else if (warp == 9) {
-        const uint32_t queries = smem_u32(smem), slots = smem_u32(ring);
-        auto scores = [&](int t, int step) {
-            const uint32_t key = slots + (2 * step) % S::slots * S::tile_bytes;
+    } else if (warp >= 9) {
+        // The operands of the products come from uniform registers, which the compiler can only fill cheaply where it sees that a value is the same in
+        // the whole warp: hence the broadcasts, and descriptors made outside the elected regions.
+        const int t = __shfl_sync(0xffffffffu, warp - 9, 0), last = __shfl_sync(0xffffffffu, steps, 0) - 1;
+        const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), slots = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+        const uint64_t query = operand_descriptor(__shfl_sync(0xffffffffu, smem_u32(smem), 0) + t * S::query_bytes);
+        const uint32_t s_at = base + t * 128, o_at = base + 256 + t * HD;
+        auto ready = [&](int item) { return wait(&full[item % S::slots], (item / S::slots) & 1); };
+        auto key_of = [&](int item) { return operand_descriptor(slots + item % S::slots * S::step_bytes); };
+        auto scores = [&](int buffer, int item, uint64_t key) {   // one lane
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k)
-                tc_mma_bf16(tmem + t * 128, operand_descriptor(queries + t * S::tile_bytes + k / 4 * S::block_bytes) + 2 * (k % 4),
-                            operand_descriptor(key + k / 4 * S::block_bytes) + 2 * (k % 4), S::scores, k != 0);
-            tc_commit(&s_full[t]);
+                tc_mma_bf16(s_at + buffer * 64, query + (k / 4 * S::query_block >> 4) + 2 * (k % 4), key + (k / 4 * S::key_block >> 4) + 2 * (k % 4), S::scores, k != 0);
+            tc_commit(&s_full[2 * t + buffer]);
+            tc_commit(&empty[item % S::slots]);
         };
-        bool going = wait(q_ready, 0) && wait(&full[0], 0);
-        tc_fence_after_sync();
-        if (going && elect_one()) {
-            for (int t = 0; t < tiles; ++t) scores(t, 0);
-            tc_commit(&empty[0]);
+        bool going = t < tiles && wait(&q_ready[t], 0);
+        for (int step = 0; step < 2; ++step) {
+            if (step > last || !going) break;
+            const int k = key_item(step);
+            going = ready(k);
+            tc_fence_after_sync();
+            const uint64_t key = key_of(k);
+            if (going && elect_one()) scores(step, k, key);
         }
-        for (int step = 0; step < steps && going; ++step) {
-            const int v = 2 * step + 1, k = v + 1;
-            const bool more = step + 1 < steps;
-            going = wait(&full[v % S::slots], (v / S::slots) & 1) && (!more || wait(&full[k % S::slots], (k / S::slots) & 1))
-                    && (more || !has_tail || wait(tail, 0));
-            for (int t = 0; t < tiles && going; ++t) {
-                going = wait(&p_ready[t], step & 1);
-                tc_fence_after_sync();
-                if (going && elect_one()) {
-                    const uint32_t value = slots + v % S::slots * S::tile_bytes;
-#pragma unroll
-                    for (int i = 0; i < kTensorKeys / 16; ++i)
-                        tc_mma_bf16_tmem(tmem + 256 + t * HD, tmem + t * 128 + 8 * i, operand_descriptor_transposed(value + i * 2048, S::block_bytes), S::sums, (step | i) != 0);
-                    tc_commit(&o_done[t]);
-                    if (more) scores(t, step + 1);
-                }
-            }
+        for (int step = 0; step <= last; ++step) {
+            if (!going) break;
+            const int v = value_item(step, last + 1), k = key_item(step + 2), buffer = step & 1;
+            const bool more = step + 2 <= last;
+            going = ready(v) && (step < last || !has_tail || wait(tail, 0)) && (!more || ready(k)) && wait(&p_ready[2 * t + buffer], (step >> 1) & 1);
+            tc_fence_after_sync();
+            const uint64_t value = operand_descriptor_transposed(slots + v % S::slots * S::step_bytes, S::key_block), key = key_of(k);
             if (going && elect_one()) {
+#pragma unroll
+                for (int i = 0; i < kTensorKeys / 16; ++i)
+                    tc_mma_bf16_tmem(o_at, s_at + buffer * 64 + 8 * i, value + i * 128, S::sums, (step | i) != 0);
+                tc_commit(&o_done[2 * t + buffer]);
                 tc_commit(&empty[v % S::slots]);
-                if (more) tc_commit(&empty[k % S::slots]);
+                if (more) scores(buffer, k, key);
             }
         }
         if (*alive == 0) {   // nor a product
-            if (elect_one()) tc_commit(drained);
-            mbar_wait(drained, 0);
+            if (elect_one()) tc_commit(&drained[t]);
+            mbar_wait(&drained[t], 0);
         }
     } else if (warp / 4 < tiles) {
         const int t = warp / 4, row = threadIdx.x % 128;
@@ -198,11 +210,12 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
                 for (int u = 0; u < 8; ++u) {
                     const int i = (first + u) * 128 + row, c = i % kPieces, r = i / kPieces;
                     x[u].x ^= flip; x[u].y ^= flip; x[u].z ^= flip; x[u].w ^= flip;
-                    *reinterpret_cast<uint4*>(smem + t * S::tile_bytes + c / 8 * S::block_bytes + r * 128 + (((c ^ r) & 7) << 4)) = x[u];
+                    *reinterpret_cast<uint4*>(smem + t * S::query_bytes + c / 8 * S::query_block + r * 128 + (((c ^ r) & 7) << 4)) = x[u];
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(q_ready);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready[t]);
         }
         const float scale = fabsf(p.scale);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -210,26 +223,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
         float most = -INFINITY, sum = 0.0f;   // the maximum that the weights are relative to
         bool going = true;
         for (int step = 0; step < steps; ++step) {
-            going = wait(&s_full[t], step & 1);
+            const int buffer = 2 * t + (step & 1);
+            const uint32_t s_here = s_at + (step & 1) * 64;
+            going = wait(&s_full[buffer], (step >> 1) & 1);
             if (!going) break;
             tc_fence_after_sync();
-            // two looks at the scores: holding all 128 of a row between the maximum and the weights would take too many registers
-            const int live = min(kTensorKeys, it.keys.end - it.keys.begin - step * kTensorKeys);
+            uint32_t s[2][32];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_load_32_async(s_here + 32 * c, s[c]);
+            tmem_wait_loads();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_loaded(s[c]);
+            hide_scores(s, it.keys.end - it.keys.begin - step * kTensorKeys);
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t s[2][32];
+            for (int i = 0; i < 32; i += 2)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_load_32_async(s_at + 64 * half + 32 * c, s[c]);
-                tmem_wait_loads();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_loaded(s[c]);
-                hide_scores(s, live - 64 * half);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[c / 2][i + c % 2]));
-            }
+                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[c / 2][i + c % 2]));
             const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
             const bool grows = here > most + kLazy;
             if (__any_sync(0xffffffffu, grows)) {
@@ -237,7 +247,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
                 if (grows) most = here;
                 sum *= factor;
                 if (step > 0) {
-                    going = wait(&o_done[t], (step - 1) & 1);
+                    going = wait(&o_done[2 * t + ((step - 1) & 1)], ((step - 1) >> 1) & 1);
                     if (!going) break;
                     tc_fence_after_sync();
 #pragma unroll 1
@@ -252,34 +262,25 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             }
             const float base = most == -INFINITY ? 0.0f : -most;
             float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t weights[32];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t s[2][32], weights[32];
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_load_32_async(s_at + 64 * half + 32 * c, s[c]);
-                tmem_wait_loads();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_loaded(s[c]);
-                hide_scores(s, live - 64 * half);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float a = exp2_fast(fmaf(__uint_as_float(s[c][i]), scale, base));
-                        const float b = exp2_fast(fmaf(__uint_as_float(s[c][i + 1]), scale, base));
-                        add[(i / 2) & 1] += a;
-                        add[2 + ((i / 2) & 1)] += b;
-                        weights[16 * c + i / 2] = pack_bf16(a, b);
-                    }
-                // the columns of scores that both looks are done with
-                tmem_store_32(s_at + 32 * half, weights);
-            }
+                for (int i = 0; i < 32; i += 2) {
+                    const float a = exp2_fast(fmaf(__uint_as_float(s[c][i]), scale, base));
+                    const float b = exp2_fast(fmaf(__uint_as_float(s[c][i + 1]), scale, base));
+                    add[(i / 2) & 1] += a;
+                    add[2 + ((i / 2) & 1)] += b;
+                    weights[16 * c + i / 2] = pack_bf16(a, b);
+                }
+            tmem_store_32(s_here, weights);
             sum += (add[0] + add[1]) + (add[2] + add[3]);
             tmem_wait_stores();
             tc_fence_before_sync();
-            mbar_arrive(&p_ready[t]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[buffer]);
         }
-        if (going && wait(&o_done[t], (steps - 1) & 1)) {
+        if (going && wait(&o_done[2 * t + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1)) {
             tc_fence_after_sync();
             const int m = m_tile + row;
             const int64_t to = m < it.m_count ? partial_row(p, it, m) : 0;
@@ -326,12 +327,14 @@ int page_box_rows(int page_size) {
 int page_maps(const PagesView& pages, int box_rows, CUtensorMap* maps) {
     encode_tiled_fn encode = tensor_map_encoder();
     if (!encode) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return B200_NO_DEVICE; }
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(pages.head_dim), static_cast<cuuint64_t>(pages.pages) * pages.kv_heads * pages.page_size};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pages.head_dim) * 2};
-    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, ones[2] = {1, 1};
+    const cuuint64_t rows = static_cast<cuuint64_t>(pages.pages) * pages.kv_heads * pages.page_size, bytes = static_cast<cuuint64_t>(pages.head_dim) * 2;
+    const bool whole = boxes_per_row(box_rows, pages.head_dim) == 1 && pages.head_dim > 64;
+    // [64 values][rows][blocks of 64 values], or [values][rows]
+    const cuuint64_t dims[3] = {whole ? 64 : static_cast<cuuint64_t>(pages.head_dim), rows, static_cast<cuuint64_t>(pages.head_dim / 64)}, strides[2] = {bytes, 128};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(pages.head_dim / 64)}, ones[3] = {1, 1, 1};
     for (int which = 0; which < 2; ++which) {
-        const CUresult result = encode(&maps[which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages.pool[which], dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        const CUresult result = encode(&maps[which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, whole ? 3 : 2, pages.pool[which], dims, strides, box, ones,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (result != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with %d", static_cast<int>(result)); return B200_BAD_ARGUMENT; }
     }
     return B200_OK;
