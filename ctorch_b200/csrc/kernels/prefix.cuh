@@ -35,11 +35,12 @@ __device__ __forceinline__ KeySpan split_span(int total, int splits, int index) 
     const int begin = min(total, index * per * kUnit);
     return {begin, min(total, begin + per * kUnit)};
 }
-__device__ __forceinline__ int used_splits(int total, int splits) {
+// The splits of `total` keys that begin before key `seen`.
+__device__ __forceinline__ int used_splits(int total, int splits, int seen) {
     const int steps = (total + kUnit - 1) / kUnit;
-    if (steps == 0) return 0;
-    const int per = (steps + splits - 1) / splits;
-    return (steps + per - 1) / per;
+    if (steps == 0 || seen <= 0) return 0;
+    const int per = (steps + splits - 1) / splits * kUnit;
+    return (min(seen, total) + per - 1) / per;
 }
 
 __device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
@@ -119,7 +120,12 @@ __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
     it.keys = split_span(keys, p.own_splits, split);
     it.causal = true;
     it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
-    if (it.live) it.visible = p.rows.lengths[it.slot] + 1;
+    if (it.live) {
+        it.visible = p.rows.lengths[it.slot] + 1;
+        // no further than the tile's last pair sees
+        it.keys.end = min(it.keys.end, it.visible + (min(it.m_begin + p.own_rows, it.m_count) - 1) / p.group);
+        it.live = it.keys.begin < it.keys.end;
+    }
     return it;
 }
 

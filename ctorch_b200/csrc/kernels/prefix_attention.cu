@@ -189,7 +189,7 @@ struct MmaMaps { CUtensorMap own[2], prefix[2]; };   // K and V
 
 // SPLIT: a tile of 16 pairs, each warp takes 16 of the 64 keys of a step and the warps' results are joined at the end; otherwise a tile of 64 pairs,
 // 16 per warp, all of which use the same keys.
-template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
+template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
     using S = MmaShape<HD>;
     extern __shared__ unsigned char mma_shared[];
     constexpr int kKeys = SPLIT ? 16 : 64;       // keys per warp and step
@@ -405,7 +405,7 @@ template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merg
     const int row = static_cast<int>(index / p.heads);
     if (row >= p.rows.rows || row >= __ldg(p.rows.first + p.rows.sequences)) return;
     const int s = __ldg(p.rows.sequence + row);
-    const int slot = __ldg(p.rows.slot + s), count = __ldg(p.rows.first + s + 1) - __ldg(p.rows.first + s);
+    const int slot = __ldg(p.rows.slot + s), first = __ldg(p.rows.first + s), count = __ldg(p.rows.first + s + 1) - first;
     int g = -1;
     for (int base = 0; base < p.groups; base += 32) {
         const int c = base + lane;
@@ -415,8 +415,9 @@ template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merg
             break;
         }
     }
-    const int from_prefix = g < 0 ? 0 : used_splits(prefix_keys(p, g), p.prefix_splits);
-    const int parts = from_prefix + used_splits(own_keys(p, slot, count), p.own_splits);
+    const int shared = g < 0 ? 0 : prefix_keys(p, g), own = own_keys(p, slot, count);
+    const int from_prefix = used_splits(shared, p.prefix_splits, shared);
+    const int parts = from_prefix + (own > 0 ? used_splits(own, p.own_splits, p.rows.lengths[slot] + row - first + 1) : 0);
     const int64_t base = index * (p.prefix_splits + p.own_splits);
     const int skip = p.prefix_splits - from_prefix;
     constexpr int kHeld = 2 * kMostSplits / 32;
@@ -580,8 +581,8 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
         return B200_BAD_ARGUMENT;
     }
     const size_t need = b200_prefix_scratch_bytes(a, pass, max_length, max_prefix);
-    if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16) {
-        set_error("b200_prefix_attention: scratch of %zu bytes on a 16-byte boundary needed, %zu given", need, scratch_bytes);
+    if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 32) {
+        set_error("b200_prefix_attention: scratch of %zu bytes on a 32-byte boundary needed, %zu given", need, scratch_bytes);
         return B200_BAD_ARGUMENT;
     }
     const Plan plan = make_plan(*a, *pass, max_length, max_prefix);

@@ -340,6 +340,25 @@ def test_what_a_row_does_not_see_may_be_no_number(name, odd):
     assert not torch.isfinite(after[last]).any()
 
 
+@pytest.mark.parametrize("name", ["drafts", "wide heads", "many rows", "f32", "heads of 80"])
+@pytest.mark.parametrize("where", range(0, 24, 3))
+def test_one_key_that_is_no_number_spoils_all_that_see_it(name, where):
+    """A NaN in a prefix's key, at any place of a step: the rows of that prefix's groups are NaN, the others as before."""
+    state, cache, prefix, query, of = attention_state(name)
+    before, after = (torch.empty((state.rows, of["heads"], of["dim"]), device="cuda") for _ in range(2))
+    call = Attention(state, cache, prefix, query, of)
+    call(before)
+    page = prefix.key.shape[2]
+    shared = of["group_prefix"][0]
+    cache.key[prefix.table[shared, where // page], :, where % page, 1] = float("nan")
+    call(after)
+    spoilt = np.zeros(state.rows, dtype=bool)
+    for g, number in enumerate(of["group_prefix"]):
+        if number == shared:
+            spoilt[state.first[of["group_first"][g]]:state.first[of["group_first"][g + 1]]] = True
+    assert torch.isnan(after[spoilt]).all() and torch.equal(after[~spoilt], before[~spoilt])
+
+
 def test_infinite_values_that_a_row_sees_reach_its_result():
     state, cache, prefix, query, of = attention_state("drafts")
     s, page = 0, cache.key.shape[2]
