@@ -8,10 +8,25 @@ namespace b200 {
 
 constexpr int kUnit = 64;   // keys of a step; splits are whole steps
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^k the power of two from d on and f = ceil(2^(31 + k) / d) < 2^32, f d - 2^(31 + k) < d <= 2^k, so
+// n f / 2^(31 + k) exceeds n / d by less than n 2^k / (d 2^(31 + k)) < 1 / d.
+struct Divider {
+    uint32_t factor;
+    int shift;   // -1: d = 1
+};
+inline Divider divider(int d) {
+    int k = 0;
+    while ((1 << k) < d) ++k;
+    if (k == 0) return {0, -1};
+    return {static_cast<uint32_t>(((uint64_t{1} << (31 + k)) + d - 1) / d), k - 1};
+}
+__device__ __forceinline__ int divide(int n, Divider d) { return d.shift < 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.factor) >> d.shift); }
+
 struct PrefixParams {
     RowsView rows;
     PagesView own, prefix;
     int heads, group, dim, groups;
+    Divider by_group;
     const int32_t *group_first, *group_prefix, *prefix_length;
     const void* query;
     float scale;               // times log2(e)
@@ -43,8 +58,8 @@ __device__ __forceinline__ int used_splits(int total, int splits, int seen) {
     return (min(seen, total) + per - 1) / per;
 }
 
-__device__ __forceinline__ int prefix_keys(const PrefixParams& p, int g) {
-    const int slot = __ldg(p.group_prefix + g);
+// Keys of the prefix in a slot of its table.
+__device__ __forceinline__ int prefix_keys(const PrefixParams& p, int slot) {
     if (slot < 0 || slot >= p.prefix.sequences) return 0;
     return max(0, min(__ldg(p.prefix_length + slot), p.prefix.capacity()));
 }
@@ -75,10 +90,13 @@ __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
         // tile -> group: the groups' tile counts are added up 32 at a time
         for (int base = 0; base < p.groups; base += 32) {
             const int g = base + lane;
-            int begin = 0, rows = 0, tiles = 0;
-            if (g < p.groups) {
-                begin = __ldg(p.rows.first + __ldg(p.group_first + g));
-                rows = max(0, __ldg(p.rows.first + __ldg(p.group_first + g + 1)) - begin);
+            int begin = 0, rows = 0, tiles = 0, slot = -1, keys = 0;
+            if (g < p.groups) {   // two rounds of loads that do not wait for one another
+                const int from = __ldg(p.group_first + g), to = __ldg(p.group_first + g + 1);
+                slot = __ldg(p.group_prefix + g);
+                begin = __ldg(p.rows.first + from);
+                rows = max(0, __ldg(p.rows.first + to) - begin);
+                keys = prefix_keys(p, slot);
                 tiles = (rows * p.group + p.prefix_rows - 1) / p.prefix_rows;
             }
             int up_to = tiles;
@@ -93,8 +111,8 @@ __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
                 it.row = __shfl_sync(0xffffffffu, begin, from);
                 it.m_count = __shfl_sync(0xffffffffu, rows, from) * p.group;
                 it.m_begin = (tile - __shfl_sync(0xffffffffu, up_to - tiles, from)) * p.prefix_rows;
-                const int group = base + from, keys = prefix_keys(p, group);
-                it.slot = __ldg(p.group_prefix + group);
+                it.slot = __shfl_sync(0xffffffffu, slot, from);
+                keys = __shfl_sync(0xffffffffu, keys, from);
                 it.keys = split_span(keys, p.prefix_splits, it.split);
                 it.visible = keys;
                 it.live = it.keys.begin < it.keys.end;
@@ -116,16 +134,14 @@ __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
     it.m_count = count * p.group;
     it.m_begin = tile * p.own_rows;
     it.slot = __ldg(p.rows.slot + s);
-    const int keys = own_keys(p, it.slot, count);
+    const int length = it.slot >= 0 && it.slot < p.own.sequences ? p.rows.lengths[it.slot] : INT32_MIN / 2;
+    const int keys = max(0, min(length + count, p.own.capacity()));
     it.keys = split_span(keys, p.own_splits, split);
     it.causal = true;
+    it.visible = length + 1;
+    // no further than the tile's last pair sees
+    it.keys.end = min(it.keys.end, it.visible + divide(max(0, min(it.m_begin + p.own_rows, it.m_count) - 1), p.by_group));
     it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
-    if (it.live) {
-        it.visible = p.rows.lengths[it.slot] + 1;
-        // no further than the tile's last pair sees
-        it.keys.end = min(it.keys.end, it.visible + (min(it.m_begin + p.own_rows, it.m_count) - 1) / p.group);
-        it.live = it.keys.begin < it.keys.end;
-    }
     return it;
 }
 
@@ -140,9 +156,12 @@ __device__ __forceinline__ void end_items(const PrefixParams& p) {
 }
 __device__ __forceinline__ int first_item(const PrefixParams& p) { return p.beside ? p.prefix_tiles * p.own.kv_heads * p.prefix_splits : 0; }
 
-// Where pair m of an item leaves its partial result: row of [rows * heads][splits].
+// Pair m of an item among the pass's rows * heads, and where it leaves its partial result, a row of [rows * heads][splits].
+__device__ __forceinline__ int64_t pair_row(const PrefixParams& p, const Item& it, int m) {
+    return static_cast<int64_t>(it.row) * p.heads + it.kv_head * p.group + static_cast<int64_t>(divide(m, p.by_group)) * (p.heads - p.group) + m;
+}
 __device__ __forceinline__ int64_t partial_row(const PrefixParams& p, const Item& it, int m) {
-    return ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * (p.prefix_splits + p.own_splits) + it.split;
+    return pair_row(p, it, m) * (p.prefix_splits + p.own_splits) + it.split;
 }
 
 }  // namespace b200

@@ -40,13 +40,13 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
     for (int i = thread; i < kPlainRows * width; i += kPlainThreads) {
         const int m = it.m_begin + i / width, d = i % width;
         query[i] = m < it.m_count && d < p.dim
-                       ? load_as_f32(static_cast<const T*>(p.query), ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * p.dim + d)
+                       ? load_as_f32(static_cast<const T*>(p.query), pair_row(p, it, m) * p.dim + d)
                        : 0.0f;
     }
     float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, acc[2][BLOCKS][4] = {};
     int limit[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) limit[r] = it.causal ? min(it.keys.end, it.visible + (it.m_begin + 2 * ty + r) / p.group) : it.keys.end;
+    for (int r = 0; r < 2; ++r) limit[r] = it.causal ? min(it.keys.end, it.visible + divide(it.m_begin + 2 * ty + r, p.by_group)) : it.keys.end;
     for (int begin = it.keys.begin; begin < it.keys.end; begin += kPlainKeys) {
         __syncthreads();
         for (int i = thread; i < kPlainKeys * width; i += kPlainThreads) {
@@ -187,12 +187,12 @@ template <int HD> __device__ __forceinline__ void guard_values(unsigned char* va
 
 struct MmaMaps { CUtensorMap own[2], prefix[2]; };   // K and V
 
-// SPLIT: a tile of 16 pairs, each warp takes 16 of the 64 keys of a step and the warps' results are joined at the end; otherwise a tile of 64 pairs,
-// 16 per warp, all of which use the same keys.
-template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
+// A tile has 64 / PARTS pairs, 16 per warp: PARTS warps share the 64 keys of a step, and their results are joined at the end.  Tiles of 16 pairs (PARTS 4) for
+// single tokens, of 64 where there are as many pairs, so that no warp multiplies rows that are not there.
+template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
     using S = MmaShape<HD>;
     extern __shared__ unsigned char mma_shared[];
-    constexpr int kKeys = SPLIT ? 16 : 64;       // keys per warp and step
+    constexpr int kKeys = 64 / PARTS, kRowGroups = 4 / PARTS;   // keys per warp and step
     constexpr int kTiles = kKeys / 8, kSteps = HD / 16, kColumns = HD / 8;
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mma_shared) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + S::stages * 2 * S::tile_bytes);
@@ -244,13 +244,13 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads, 2) 
         return end_items(p);
     }
     // query fragments
-    const int quad = lane & 3, m0 = it.m_begin + (SPLIT ? 0 : warp * 16) + (lane >> 2);
+    const int quad = lane & 3, row_group = warp % kRowGroups, m0 = it.m_begin + row_group * 16 + (lane >> 2);
     uint32_t q[kSteps][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int m = m0 + 8 * r;
         const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.query)
-                                   + ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * p.dim;
+                                   + pair_row(p, it, m) * p.dim;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
@@ -261,10 +261,10 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads, 2) 
     }
     int seen[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) seen[r] = it.causal ? min(it.keys.end, it.visible + (m0 + 8 * r) / p.group) : it.keys.end;
+    for (int r = 0; r < 2; ++r) seen[r] = it.causal ? min(it.keys.end, it.visible + divide(m0 + 8 * r, p.by_group)) : it.keys.end;
     float acc[kColumns][4] = {}, most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    const int warp_key = SPLIT ? warp * 16 : 0;
-    const int first_limit = it.causal ? it.visible + it.m_begin / p.group : it.keys.end;   // keys that the tile's first pair sees
+    const int warp_key = warp / kRowGroups * kKeys;
+    const int first_limit = it.causal ? it.visible + divide(it.m_begin, p.by_group) : it.keys.end;   // keys that the tile's first pair sees
     for (int step = 0; step < steps; ++step) {
         const int stage = step % S::stages, begin = it.keys.begin + step * kUnit;
         wait(&full[stage], (step / S::stages) & 1);
@@ -340,37 +340,36 @@ template <int HD, bool SPLIT> __global__ void __launch_bounds__(kMmaThreads, 2) 
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
     }
-    if constexpr (SPLIT) {
-        // join the warps, in the ring that nothing is copied to any more: [warp][16 rows][HD] accumulators behind [warp][16][2] maxima and sums
+    if constexpr (PARTS > 1) {
+        // join the warps, in the ring that nothing is copied to any more: [part][rows][HD] accumulators behind [part][rows][2] maxima and sums
         mma_barrier();
+        constexpr int kRows = 64 / PARTS, kPitch = HD + 4;
         float* joined = reinterpret_cast<float*>(ring);
         float* rows_of = joined + 4 * 16 * 2;
-        constexpr int kPitch = HD + 4;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int m = (lane >> 2) + 8 * r;
+            const int at = warp / kRowGroups * kRows + row_group * 16 + (lane >> 2) + 8 * r;
             if (quad == 0) {
-                joined[(warp * 16 + m) * 2] = most[r];
-                joined[(warp * 16 + m) * 2 + 1] = sum[r];
+                joined[at * 2] = most[r];
+                joined[at * 2 + 1] = sum[r];
             }
 #pragma unroll
-            for (int n = 0; n < kColumns; ++n)
-                *reinterpret_cast<float2*>(rows_of + (warp * 16 + m) * kPitch + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+            for (int n = 0; n < kColumns; ++n) *reinterpret_cast<float2*>(rows_of + at * kPitch + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
         }
         mma_barrier();
-        const int live = min(16, it.m_count - it.m_begin);
+        const int live = min(kRows, it.m_count - it.m_begin);
         for (int i = thread; i < live * (HD / 4); i += kMmaWarps * 32) {
             const int m = i / (HD / 4), d = i % (HD / 4) * 4;
             float top = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, joined[(w * 16 + m) * 2]);
+            for (int w = 0; w < PARTS; ++w) top = fmaxf(top, joined[(w * kRows + m) * 2]);
             const float base = top == -INFINITY ? 0.0f : top;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = exp2_fast(joined[(w * 16 + m) * 2] - base);
-                const float4 v = *reinterpret_cast<const float4*>(rows_of + (w * 16 + m) * kPitch + d);
-                total += f * joined[(w * 16 + m) * 2 + 1];
+            for (int w = 0; w < PARTS; ++w) {
+                const float f = exp2_fast(joined[(w * kRows + m) * 2] - base);
+                const float4 v = *reinterpret_cast<const float4*>(rows_of + (w * kRows + m) * kPitch + d);
+                total += f * joined[(w * kRows + m) * 2 + 1];
                 o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
             }
             const int64_t to = partial_row(p, it, it.m_begin + m);
@@ -397,13 +396,15 @@ constexpr int kMergeWarps = 4, kMostSplits = 64;
 
 // A warp per row and head.  V = 4 (head sizes of 4 n): a group of `lanes` lanes reads one partial result at 16 bytes per lane, the warp's groups take
 // turns over the splits and are added at the end.
+// The pass's arrays were complete before the kernels that left the partial results began, so what is to be read is worked out while those still run.
 template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const PrefixParams p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int64_t index = blockIdx.x * static_cast<int64_t>(kMergeWarps) + static_cast<int64_t>(threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const int row = static_cast<int>(index / p.heads);
-    if (row >= p.rows.rows || row >= __ldg(p.rows.first + p.rows.sequences)) return;
+    if (row >= p.rows.rows || row >= __ldg(p.rows.first + p.rows.sequences)) {
+        grid_dependency_wait();
+        return;
+    }
     const int s = __ldg(p.rows.sequence + row);
     const int slot = __ldg(p.rows.slot + s), first = __ldg(p.rows.first + s), count = __ldg(p.rows.first + s + 1) - first;
     int g = -1;
@@ -415,11 +416,13 @@ template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merg
             break;
         }
     }
-    const int shared = g < 0 ? 0 : prefix_keys(p, g), own = own_keys(p, slot, count);
+    const int shared = g < 0 ? 0 : prefix_keys(p, __ldg(p.group_prefix + g)), own = own_keys(p, slot, count);
     const int from_prefix = used_splits(shared, p.prefix_splits, shared);
     const int parts = from_prefix + (own > 0 ? used_splits(own, p.own_splits, p.rows.lengths[slot] + row - first + 1) : 0);
     const int64_t base = index * (p.prefix_splits + p.own_splits);
     const int skip = p.prefix_splits - from_prefix;
+    grid_dependency_wait();
+    grid_launch_dependents();
     constexpr int kHeld = 2 * kMostSplits / 32;
     float most[kHeld], weight[kHeld], top = -INFINITY, total = 0.0f;
 #pragma unroll
@@ -484,6 +487,31 @@ bool mma_takes(const b200_kv_pages& pages) {
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
+int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Splits of the prefix's keys for the tcgen05 kernel.  Its CTAs have an SM each, and the own tokens' CTAs, which are bound by memory, run on the SMs that
+// it leaves: few splits leave more of them and fewer partial results, many shorten the prefix's own time.  In us: a CTA takes 9 and 0.8 per step; an SM
+// streams up to 60 KB of own keys and values, all of them together 5.5 MB; partial results go out and back at 5 MB.
+int tensor_splits(int64_t items, int max_prefix, double own_bytes, double part_bytes) {
+    const int steps = ceil_div(max_prefix, kTensorKeys);
+    int best = 1;
+    double least = 1e30;
+    for (int n = 1; n <= kMostSplits && n <= steps; ++n) {
+        const int64_t ctas = items * n, waves = ceil_div64(ctas, 148);
+        const double prefix = static_cast<double>(waves) * (9.0 + 0.8 * ceil_div(steps, n));
+        const double rest = static_cast<double>(waves * 148 - ctas);   // SMs that the last wave leaves
+        const double rate = std::min(5.5e6, std::max(rest, 1.0) * 6e4), own = own_bytes / 5.5e6;
+        const double last = 9.0 + 0.8 * ceil_div(steps, n);            // the last wave, beside which own tokens run
+        const double beside = std::min(last, own_bytes / rate);
+        const double time = prefix + std::max(0.0, own - beside * rate / 5.5e6) + n * part_bytes / 5e6;
+        if (time < least) {
+            least = time;
+            best = n;
+        }
+    }
+    return best;
+}
+
 Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length, int max_prefix) {
     Plan plan{};
     const int kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
@@ -495,10 +523,10 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     const bool prefix = a.groups > 0 && max_prefix > 0;
     plan.form = mma ? Form::mma : Form::plain;
     plan.tensor = mma && prefix && pairs > 32 * static_cast<int64_t>(groups) && prefix_tensor_takes(a.prefix, a.scale);
-    // a tile of 16 pairs, or of 64 where most would not fit
+    // tiles of 16, 32 or 64 pairs: the smallest that holds the most that a sequence (or, with the prefix's items among them, a group) has
     const int64_t own_pairs = static_cast<int64_t>(pass.max_count) * group;
-    plan.own_rows = !mma ? kPlainRows : own_pairs <= 16 || (!plan.tensor && prefix && pairs <= 16 * static_cast<int64_t>(groups)) ? 16 : 64;
-    if (mma && prefix && !plan.tensor && pairs > 16 * static_cast<int64_t>(groups)) plan.own_rows = 64;
+    const int64_t most_pairs = prefix && !plan.tensor ? std::max(own_pairs, ceil_div64(pairs, groups)) : own_pairs;
+    plan.own_rows = !mma ? kPlainRows : most_pairs <= 16 ? 16 : most_pairs <= 32 ? 32 : 64;
     plan.prefix_rows = plan.tensor ? kTensorRows : plan.own_rows;
     plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.prefix_rows) + groups : 0;
     plan.own_tiles = ceil_div(own_pairs, plan.own_rows);
@@ -509,10 +537,16 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
         if (n > kMostSplits) n = kMostSplits;
         return n < 1 ? 1 : n;
     };
-    // tiles that the rows fill: the last tile of every group is counted half
-    const int64_t filled = ceil_div(pairs, plan.prefix_rows) > groups ? ceil_div(pairs, plan.prefix_rows) : groups;
-    plan.prefix_splits = prefix ? splits(filled * kv_heads, max_prefix, plan.tensor ? 148 : 2 * 148) : 0;
-    plan.own_splits = splits(static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads, max_length, 2 * 148);
+    const int64_t own_items = static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads;
+    plan.own_splits = splits(own_items, max_length, 2 * 148);
+    if (!prefix) return plan;
+    // tiles that the rows fill: the last tile of every group is half empty
+    const int64_t filled = std::max<int64_t>(ceil_div(pairs, plan.prefix_rows), groups) * kv_heads;
+    if (!plan.tensor) {
+        plan.prefix_splits = splits(filled, max_prefix, 2 * 148);
+        return plan;
+    }
+    plan.prefix_splits = tensor_splits(filled, max_prefix, static_cast<double>(pass.sequences) * kv_heads * max_length * a.cache.head_dim * 4, static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8);
     return plan;
 }
 
@@ -546,7 +580,7 @@ template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned item
 }
 
 template <int HD> int launch_mma(const PrefixParams& p, unsigned items, cudaStream_t stream) {
-    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, true> : prefix_mma_kernel<HD, false>;
+    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, 4> : p.own_rows == 32 ? prefix_mma_kernel<HD, 2> : prefix_mma_kernel<HD, 1>;
     constexpr int smem = MmaShape<HD>::smem_bytes;
     MmaMaps maps;
     int box_rows = page_box_rows(p.own.page_size);
@@ -586,7 +620,7 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
         return B200_BAD_ARGUMENT;
     }
     const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
-    p.heads = a->heads; p.group = a->heads / a->cache.kv_heads; p.dim = a->cache.head_dim;
+    p.heads = a->heads; p.group = a->heads / a->cache.kv_heads; p.by_group = divider(p.group); p.dim = a->cache.head_dim;
     p.groups = plan.prefix_splits ? a->groups : 0;
     p.group_first = a->group_first; p.group_prefix = a->group_prefix; p.prefix_length = a->prefix_length;
     p.query = a->query;

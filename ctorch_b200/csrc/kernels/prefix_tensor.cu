@@ -236,23 +236,19 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
         {
             const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
             constexpr int kPieces = 8 * S::blocks;
+            uint4 x[kPieces];   // requested together; a row's pieces by neighbouring threads
+            const int c = row % kPieces;
 #pragma unroll
-            for (int first = 0; first < kPieces; first += 8) {
-                uint4 x[8];   // requested together
+            for (int u = 0; u < kPieces; ++u) {
+                const int m = m_tile + row / kPieces + u * (128 / kPieces);
+                x[u] = make_uint4(0, 0, 0, 0);
+                if (m < it.m_count) x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query) + pair_row(p, it, m) * HD + 8 * c));
+            }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int i = (first + u) * 128 + row, c = i % kPieces, m = m_tile + i / kPieces;
-                    x[u] = make_uint4(0, 0, 0, 0);
-                    if (m < it.m_count)
-                        x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query)
-                                                                    + ((static_cast<int64_t>(it.row) + m / p.group) * p.heads + it.kv_head * p.group + m % p.group) * HD + 8 * c));
-                }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int i = (first + u) * 128 + row, c = i % kPieces, r = i / kPieces;
-                    x[u].x ^= flip; x[u].y ^= flip; x[u].z ^= flip; x[u].w ^= flip;
-                    *reinterpret_cast<uint4*>(smem + t * S::query_bytes + c / 8 * S::query_block + r * 128 + (((c ^ r) & 7) << 4)) = x[u];
-                }
+            for (int u = 0; u < kPieces; ++u) {
+                const int r = row / kPieces + u * (128 / kPieces);
+                x[u].x ^= flip; x[u].y ^= flip; x[u].z ^= flip; x[u].w ^= flip;
+                *reinterpret_cast<uint4*>(smem + t * S::query_bytes + c / 8 * S::query_block + r * 128 + (((c ^ r) & 7) << 4)) = x[u];
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -336,19 +332,31 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
         }
         if (going && wait(&o_done[2 * t + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1)) {
             tc_fence_after_sync();
+            // a thread has a row of O: through the tile's part of shared memory, whose queries nobody needs any more, so that the lanes of a store write
+            // neighbouring pieces; 64 values of the warp's 32 rows at a time, pieces permuted against bank conflicts
             const int m = m_tile + row;
-            const int64_t to = m < it.m_count ? partial_row(p, it, m) : 0;
-            if (m < it.m_count) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most, sum);
+            const int64_t to = m < it.m_count ? partial_row(p, it, m) : -1;
+            if (to >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most, sum);
+            uint8_t* rows = smem + t * S::query_bytes + (warp & 3) * (S::query_bytes / 4);
+            constexpr int kPieces = S::query_bytes / 4 / 32 / 16;   // 16 (8) pieces of four values: 64 (32) values
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                tmem_load_32(o_at + 32 * c, o);
-                if (m < it.m_count) {
+            for (int first = 0; first < HD; first += 4 * kPieces) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8)   // whole sectors of 32 bytes
-                        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p.part_o + to * HD + 32 * c + i), "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]),
-                                     "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7]) : "memory");
+                for (int c = 0; c < kPieces / 8; ++c) {
+                    uint32_t o[32];
+                    tmem_load_32(o_at + first + 32 * c, o);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(rows + lane * kPieces * 16 + (((8 * c + i) ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int r = i * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
+                    const int64_t at = __shfl_sync(0xffffffffu, to, r);
+                    if (at >= 0) *reinterpret_cast<uint4*>(p.part_o + at * HD + first + 4 * c) = *reinterpret_cast<const uint4*>(rows + r * kPieces * 16 + ((c ^ (r & 7)) << 4));
+                }
+                __syncwarp();
             }
         }
     }
