@@ -34,6 +34,7 @@ struct PrefixParams {
     int prefix_tiles;          // row tiles of all groups, at most
     int own_tiles;             // row tiles per sequence, at most
     int prefix_rows, own_rows; // pairs of a row tile
+    int items;                 // of this launch
     int beside;                // 1: the prefix's items are another kernel's, launched just before, beside which this one runs
     int32_t* status;
     float* part_o;             // [rows * heads][splits][dim]
@@ -145,14 +146,14 @@ __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
     return it;
 }
 
-// A kernel that runs beside the prefix's: that one let it start when everything before both was complete, so it need not wait to begin; it waits
-// before it ends, so that it is complete no earlier than the other and the merge can wait for this one alone.
+// A kernel that runs beside the prefix's: that one let it start when everything before both was complete, so it need not wait to begin; its first CTA waits
+// before it ends, so that the kernel is complete no earlier than the other and the merge can wait for this one alone.
 __device__ __forceinline__ void begin_items(const PrefixParams& p) {
     if (!p.beside) grid_dependency_wait();
     grid_launch_dependents();
 }
 __device__ __forceinline__ void end_items(const PrefixParams& p) {
-    if (p.beside) grid_dependency_wait();
+    if (p.beside && blockIdx.x == 0) grid_dependency_wait();
 }
 __device__ __forceinline__ int first_item(const PrefixParams& p) { return p.beside ? p.prefix_tiles * p.own.kv_heads * p.prefix_splits : 0; }
 

@@ -140,8 +140,10 @@ template <int HD> struct MmaShape {                              // HD: the head
     static constexpr int blocks = HD <= 64 ? 1 : 2;              // of 64 values: rows of 128 bytes as TMA's swizzle lays them out
     static constexpr int block_bytes = kUnit * 128;
     static constexpr int tile_bytes = blocks * block_bytes;      // K or V of one step
-    static constexpr int stages = blocks == 1 ? 4 : 3;           // 64 or 96 KB in flight per CTA, three or two CTAs per SM
-    static constexpr int smem_bytes = stages * 2 * tile_bytes + 1024 + 256;   // slack of the 1024-byte alignment, control words
+    // What two CTAs per SM leave room for beside the area where warps' results are joined.
+    static constexpr int stages(int parts) { return blocks == 1 ? 4 : parts > 1 ? 2 : 3; }
+    static constexpr int join_bytes(int parts) { return parts > 1 ? 64 * (HD + 4) * 4 + 64 * 2 * 4 : 0; }
+    static constexpr int smem_bytes(int parts) { return stages(parts) * 2 * tile_bytes + join_bytes(parts) + 1024 + 512; }   // slack of the 1024-byte alignment, control words
 };
 // Byte offset of 16-byte piece c of row r.
 __device__ __forceinline__ uint32_t piece_offset(int r, int c) { return static_cast<uint32_t>((c >> 3) * kUnit * 128 + r * 128 + (((c ^ r) & 7) << 4)); }
@@ -152,6 +154,9 @@ __device__ __forceinline__ bool mma_any(bool mine) {
                  : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "n"(kMmaWarps * 32) : "memory");
     return any != 0;
 }
+
+// Between this thread's own stores to a stage and the copy that refills it.
+__device__ __forceinline__ void own_writes_done() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Steps with keys that some pairs of the tile do not see: a weight of 0 does not cancel a value that is no number, so such values leave the tile
 // before the products, and are added to the accumulators of the pairs that do see them.
@@ -182,37 +187,45 @@ template <int HD> __device__ __forceinline__ void guard_values(unsigned char* va
         uint16_t* x = reinterpret_cast<uint16_t*>(value + piece_offset(i / (pieces * 8), i / 8 % pieces)) + i % 8;
         if ((*x & 0x7f80) == 0x7f80) *x = 0;
     }
+    own_writes_done();
     mma_barrier();
 }
 
 struct MmaMaps { CUtensorMap own[2], prefix[2]; };   // K and V
 
 // A tile has 64 / PARTS pairs, 16 per warp: PARTS warps share the 64 keys of a step, and their results are joined at the end.  Tiles of 16 pairs (PARTS 4) for
-// single tokens, of 64 where there are as many pairs, so that no warp multiplies rows that are not there.
+// single tokens, of 64 where there are as many pairs, so that no warp multiplies rows that are not there.  A CTA takes item after item; the copying warp finds
+// them and runs ahead of the products, so that keys of the next item are on their way while the last one's results are written.
 template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
     using S = MmaShape<HD>;
     extern __shared__ unsigned char mma_shared[];
+    constexpr int kStages = S::stages(PARTS);
     constexpr int kKeys = 64 / PARTS, kRowGroups = 4 / PARTS;   // keys per warp and step
     constexpr int kTiles = kKeys / 8, kSteps = HD / 16, kColumns = HD / 8;
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mma_shared) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(ring + S::stages * 2 * S::tile_bytes);
-    uint64_t* empty = full + S::stages;
-    volatile int* alive = reinterpret_cast<volatile int*>(empty + S::stages);
+    float* joined = reinterpret_cast<float*>(ring + kStages * 2 * S::tile_bytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(joined) + S::join_bytes(PARTS));
+    uint64_t* empty = full + kStages;
+    uint64_t* item_full = empty + kStages;   // [2] items found ahead
+    uint64_t* item_empty = item_full + 2;
+    Item* item_of = reinterpret_cast<Item*>(item_empty + 2);
+    volatile int* alive = reinterpret_cast<volatile int*>(item_of + 2);
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
     if (thread == 0) {
-        for (int i = 0; i < S::stages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], kMmaWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&item_full[i], 1);
+            mbar_init(&item_empty[i], kMmaWarps);
         }
         *alive = 1;
         mbar_fence_init();
     }
-    begin_items(p);
-    const Item it = find_item(p, first_item(p) + blockIdx.x);
     __syncthreads();
-    if (!it.live) return end_items(p);
-    const int steps = (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
-    // after a wait that ran out every role goes through the rest without waiting
+    begin_items(p);
+    // after a wait that ran out every role goes through the rest of its item without waiting, and leaves
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (*alive && !mbar_wait(bar, parity)) {
             atomicExch(p.status, B200_DEVICE_TIMEOUT);
@@ -220,175 +233,202 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
         }
     };
     if (warp == kMmaWarps) {
-        const PagesView& view = it.causal ? p.own : p.prefix;
-        const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
         const int across = boxes_per_row(box_rows, p.dim), boxes = kUnit / box_rows * across;   // at most 16 per tensor
         const int which = lane / boxes, block = lane % across, row = lane % boxes / across * box_rows;
-        const CUtensorMap* map = it.causal ? &maps.own[which & 1] : &maps.prefix[which & 1];
-        PageStream pages(view, it.slot, it.keys.begin + row, kUnit, which < 2 ? it.keys.end : 0);
-        int issued = 0;
-        for (; issued < steps; ++issued) {
-            const int stage = issued % S::stages, y = pages.next(it.kv_head, outside);
-            wait(&empty[stage], ((issued / S::stages) & 1) ^ 1);
-            if (!__all_sync(0xffffffffu, *alive != 0)) break;
-            if (lane == 0) mbar_expect_tx(&full[stage], 2 * S::tile_bytes);
-            __syncwarp();
-            unsigned char* to = ring + (stage * 2 + which) * S::tile_bytes;
-            if (which < 2) {
-                if (across < S::blocks) tma_load_3d(to, map, 0, y, 0, &full[stage]);
-                else tma_load_2d(to + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
+        int issued = 0, found = 0;
+        for (int index = blockIdx.x;; index += gridDim.x) {
+            Item it{};
+            const bool any = index < p.items;
+            if (any) {
+                it = find_item(p, first_item(p) + index);
+                if (!it.live) continue;
+            } else {
+                it.m_count = -1;   // no more
             }
+            wait(&item_empty[found & 1], ((found >> 1) & 1) ^ 1);
+            if (lane == 0) {
+                item_of[found & 1] = it;
+                mbar_arrive(&item_full[found & 1]);
+            }
+            ++found;
+            if (!any || !__all_sync(0xffffffffu, *alive != 0)) break;
+            const PagesView& view = it.causal ? p.own : p.prefix;
+            const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
+            const CUtensorMap* map = it.causal ? &maps.own[which & 1] : &maps.prefix[which & 1];
+            const int end = issued + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+            PageStream pages(view, it.slot, it.keys.begin + row, kUnit, which < 2 ? it.keys.end : 0);
+            for (; issued < end; ++issued) {
+                const int stage = issued % kStages, y = pages.next(it.kv_head, outside);
+                wait(&empty[stage], ((issued / kStages) & 1) ^ 1);
+                if (!__all_sync(0xffffffffu, *alive != 0)) break;
+                if (lane == 0) mbar_expect_tx(&full[stage], 2 * S::tile_bytes);
+                __syncwarp();
+                unsigned char* to = ring + (stage * 2 + which) * S::tile_bytes;
+                if (which < 2) {
+                    if (across < S::blocks) tma_load_3d(to, map, 0, y, 0, &full[stage]);
+                    else tma_load_2d(to + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
+                }
+            }
+            if (issued < end) break;
         }
-        if (issued < steps)   // no copy is in flight when the CTA leaves
-            for (int j = max(0, issued - S::stages); j < issued; ++j) mbar_wait(&full[j % S::stages], (j / S::stages) & 1);
+        if (!*alive)   // no copy is in flight when the CTA leaves
+            for (int j = max(0, issued - kStages); j < issued; ++j) mbar_wait(&full[j % kStages], (j / kStages) & 1);
         return end_items(p);
     }
-    // query fragments
-    const int quad = lane & 3, row_group = warp % kRowGroups, m0 = it.m_begin + row_group * 16 + (lane >> 2);
-    uint32_t q[kSteps][4];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int m = m0 + 8 * r;
-        const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.query)
-                                   + pair_row(p, it, m) * p.dim;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int d = 16 * k + 8 * h + 2 * quad;
-                q[k][2 * h + r] = m < it.m_count && d < p.dim ? __ldg(reinterpret_cast<const uint32_t*>(row + d)) : 0u;
-            }
-    }
-    int seen[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) seen[r] = it.causal ? min(it.keys.end, it.visible + divide(m0 + 8 * r, p.by_group)) : it.keys.end;
-    float acc[kColumns][4] = {}, most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    const int warp_key = warp / kRowGroups * kKeys;
-    const int first_limit = it.causal ? it.visible + divide(it.m_begin, p.by_group) : it.keys.end;   // keys that the tile's first pair sees
-    for (int step = 0; step < steps; ++step) {
-        const int stage = step % S::stages, begin = it.keys.begin + step * kUnit;
-        wait(&full[stage], (step / S::stages) & 1);
-        unsigned char* values = ring + (stage * 2 + 1) * S::tile_bytes;
-        const uint32_t key = smem_u32(ring) + stage * 2 * S::tile_bytes, value = key + S::tile_bytes;
-        if (begin + kUnit > it.keys.end && it.keys.end % box_rows) {
-            // rows of the last box behind the keys may hold anything
-            const int from = it.keys.end - begin, behind = (from + box_rows - 1) / box_rows * box_rows - from;
-            for (int i = thread; i < behind * 8 * S::blocks; i += kMmaWarps * 32)
-                *reinterpret_cast<uint4*>(values + i / (behind * 8) * S::block_bytes + from * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
-            mma_barrier();
-        }
-        float score[kTiles][4] = {};
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int n = 0; n < kTiles; n += 2) {
-                uint32_t b[4];   // keys n*8 .. +7 and +8 .. +15, both halves of the 16 values
-                ldsm_x4(b, key + piece_offset(warp_key + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-                mma_16816(score[n], q[k], b[0], b[1]);
-                mma_16816(score[n + 1], q[k], b[2], b[3]);
-            }
-        const int first_key = begin + warp_key + 2 * quad;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float top = most[r];
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float& x = score[n][2 * r + u];
-                    x = first_key + n * 8 + u < seen[r] ? x * p.scale : -INFINITY;
-                    top = fmaxf(top, x);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(most[r] - base);
-            float here = 0.0f;
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float& x = score[n][2 * r + u];
-                    x = exp2_fast(x - base);
-                    here += x;
-                }
-            sum[r] = sum[r] * shrink + here;   // of this lane's keys; the quad's are added at the end
-            most[r] = top;
-#pragma unroll
-            for (int n = 0; n < kColumns; ++n) {
-                acc[n][2 * r] *= shrink;
-                acc[n][2 * r + 1] *= shrink;
-            }
-        }
-        if (min(it.keys.end, begin + kUnit) > first_limit) guard_values<HD>(values, p.dim / 8, begin, warp_key, kKeys, seen, acc);
-#pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k) {
-            const uint32_t a[4] = {pack_bf16(score[2 * k][0], score[2 * k][1]), pack_bf16(score[2 * k][2], score[2 * k][3]),
-                                   pack_bf16(score[2 * k + 1][0], score[2 * k + 1][1]), pack_bf16(score[2 * k + 1][2], score[2 * k + 1][3])};
-#pragma unroll
-            for (int n = 0; n < kColumns; n += 2) {
-                uint32_t b[4];
-                ldsm_x4_trans(b, value + piece_offset(warp_key + 16 * k + (lane & 15), n + (lane >> 4)));
-                mma_16816(acc[n], a, b[0], b[1]);
-                mma_16816(acc[n + 1], a, b[2], b[3]);
-            }
-        }
+    int taken = 0;   // steps of the items before
+    for (int number = 0;; ++number) {
+        wait(&item_full[number & 1], (number >> 1) & 1);
+        const Item it = item_of[number & 1];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[stage]);
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-    }
-    if constexpr (PARTS > 1) {
-        // join the warps, in the ring that nothing is copied to any more: [part][rows][HD] accumulators behind [part][rows][2] maxima and sums
-        mma_barrier();
-        constexpr int kRows = 64 / PARTS, kPitch = HD + 4;
-        float* joined = reinterpret_cast<float*>(ring);
-        float* rows_of = joined + 4 * 16 * 2;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int at = warp / kRowGroups * kRows + row_group * 16 + (lane >> 2) + 8 * r;
-            if (quad == 0) {
-                joined[at * 2] = most[r];
-                joined[at * 2 + 1] = sum[r];
-            }
-#pragma unroll
-            for (int n = 0; n < kColumns; ++n) *reinterpret_cast<float2*>(rows_of + at * kPitch + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
-        }
-        mma_barrier();
-        const int live = min(kRows, it.m_count - it.m_begin);
-        for (int i = thread; i < live * (HD / 4); i += kMmaWarps * 32) {
-            const int m = i / (HD / 4), d = i % (HD / 4) * 4;
-            float top = -INFINITY, total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < PARTS; ++w) top = fmaxf(top, joined[(w * kRows + m) * 2]);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < PARTS; ++w) {
-                const float f = exp2_fast(joined[(w * kRows + m) * 2] - base);
-                const float4 v = *reinterpret_cast<const float4*>(rows_of + (w * kRows + m) * kPitch + d);
-                total += f * joined[(w * kRows + m) * 2 + 1];
-                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
-            }
-            const int64_t to = partial_row(p, it, it.m_begin + m);
-            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(top, total);
-            if (d < p.dim) *reinterpret_cast<float4*>(p.part_o + to * p.dim + d) = o;
-        }
-    } else {
+        if (lane == 0) mbar_arrive(&item_empty[number & 1]);
+        if (mma_any(!*alive) || it.m_count < 0) return end_items(p);
+        const int steps = (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+        // query fragments
+        const int quad = lane & 3, row_group = warp % kRowGroups, m0 = it.m_begin + row_group * 16 + (lane >> 2);
+        uint32_t q[kSteps][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int m = m0 + 8 * r;
-            if (m >= it.m_count) continue;
-            const int64_t to = partial_row(p, it, m);
-            if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most[r], sum[r]);
+            const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.query) + pair_row(p, it, m) * p.dim;
 #pragma unroll
-            for (int n = 0; n < kColumns; ++n)
-                if (8 * n < p.dim) *reinterpret_cast<float2*>(p.part_o + to * p.dim + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int d = 16 * k + 8 * h + 2 * quad;
+                    q[k][2 * h + r] = m < it.m_count && d < p.dim ? __ldg(reinterpret_cast<const uint32_t*>(row + d)) : 0u;
+                }
         }
+        int seen[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) seen[r] = it.causal ? min(it.keys.end, it.visible + divide(m0 + 8 * r, p.by_group)) : it.keys.end;
+        float acc[kColumns][4] = {}, most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        const int warp_key = warp / kRowGroups * kKeys;
+        const int first_limit = it.causal ? it.visible + divide(it.m_begin, p.by_group) : it.keys.end;   // keys that the tile's first pair sees
+        for (int step = 0; step < steps; ++step) {
+            const int stage = (taken + step) % kStages, begin = it.keys.begin + step * kUnit;
+            wait(&full[stage], ((taken + step) / kStages) & 1);
+            unsigned char* values = ring + (stage * 2 + 1) * S::tile_bytes;
+            const uint32_t key = smem_u32(ring) + stage * 2 * S::tile_bytes, value = key + S::tile_bytes;
+            if (begin + kUnit > it.keys.end && it.keys.end % box_rows) {
+                // rows of the last box behind the keys may hold anything
+                const int from = it.keys.end - begin, behind = (from + box_rows - 1) / box_rows * box_rows - from;
+                for (int i = thread; i < behind * 8 * S::blocks; i += kMmaWarps * 32)
+                    *reinterpret_cast<uint4*>(values + i / (behind * 8) * S::block_bytes + from * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
+                own_writes_done();
+                mma_barrier();
+            }
+            float score[kTiles][4] = {};
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int n = 0; n < kTiles; n += 2) {
+                    uint32_t b[4];   // keys n*8 .. +7 and +8 .. +15, both halves of the 16 values
+                    ldsm_x4(b, key + piece_offset(warp_key + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                    mma_16816(score[n], q[k], b[0], b[1]);
+                    mma_16816(score[n + 1], q[k], b[2], b[3]);
+                }
+            const int first_key = begin + warp_key + 2 * quad;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float top = most[r];
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float& x = score[n][2 * r + u];
+                        x = first_key + n * 8 + u < seen[r] ? x * p.scale : -INFINITY;
+                        top = fmaxf(top, x);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(most[r] - base);
+                float here = 0.0f;
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float& x = score[n][2 * r + u];
+                        x = exp2_fast(x - base);
+                        here += x;
+                    }
+                sum[r] = sum[r] * shrink + here;   // of this lane's keys; the quad's are added at the end
+                most[r] = top;
+#pragma unroll
+                for (int n = 0; n < kColumns; ++n) {
+                    acc[n][2 * r] *= shrink;
+                    acc[n][2 * r + 1] *= shrink;
+                }
+            }
+            if (min(it.keys.end, begin + kUnit) > first_limit) guard_values<HD>(values, p.dim / 8, begin, warp_key, kKeys, seen, acc);
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k) {
+                const uint32_t a[4] = {pack_bf16(score[2 * k][0], score[2 * k][1]), pack_bf16(score[2 * k][2], score[2 * k][3]),
+                                       pack_bf16(score[2 * k + 1][0], score[2 * k + 1][1]), pack_bf16(score[2 * k + 1][2], score[2 * k + 1][3])};
+#pragma unroll
+                for (int n = 0; n < kColumns; n += 2) {
+                    uint32_t b[4];
+                    ldsm_x4_trans(b, value + piece_offset(warp_key + 16 * k + (lane & 15), n + (lane >> 4)));
+                    mma_16816(acc[n], a, b[0], b[1]);
+                    mma_16816(acc[n + 1], a, b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        }
+        if constexpr (PARTS > 1) {
+            // join the warps: [part][rows][HD] accumulators behind [part][rows][2] maxima and sums
+            constexpr int kRows = 64 / PARTS, kPitch = HD + 4;
+            float* rows_of = joined + 64 * 2;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int at = warp / kRowGroups * kRows + row_group * 16 + (lane >> 2) + 8 * r;
+                if (quad == 0) {
+                    joined[at * 2] = most[r];
+                    joined[at * 2 + 1] = sum[r];
+                }
+#pragma unroll
+                for (int n = 0; n < kColumns; ++n) *reinterpret_cast<float2*>(rows_of + at * kPitch + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+            }
+            mma_barrier();
+            const int live = min(kRows, it.m_count - it.m_begin);
+            for (int i = thread; i < live * (HD / 4); i += kMmaWarps * 32) {
+                const int m = i / (HD / 4), d = i % (HD / 4) * 4;
+                float top = -INFINITY, total = 0.0f;
+#pragma unroll
+                for (int w = 0; w < PARTS; ++w) top = fmaxf(top, joined[(w * kRows + m) * 2]);
+                const float base = top == -INFINITY ? 0.0f : top;
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < PARTS; ++w) {
+                    const float f = exp2_fast(joined[(w * kRows + m) * 2] - base);
+                    const float4 v = *reinterpret_cast<const float4*>(rows_of + (w * kRows + m) * kPitch + d);
+                    total += f * joined[(w * kRows + m) * 2 + 1];
+                    o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+                }
+                const int64_t to = partial_row(p, it, it.m_begin + m);
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(top, total);
+                if (d < p.dim) *reinterpret_cast<float4*>(p.part_o + to * p.dim + d) = o;
+            }
+            mma_barrier();   // the next item's results may be written
+        } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int m = m0 + 8 * r;
+                if (m >= it.m_count) continue;
+                const int64_t to = partial_row(p, it, m);
+                if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most[r], sum[r]);
+#pragma unroll
+                for (int n = 0; n < kColumns; ++n)
+                    if (8 * n < p.dim) *reinterpret_cast<float2*>(p.part_o + to * p.dim + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+            }
+        }
+        taken += steps;
     }
-    end_items(p);
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------------------------
@@ -479,6 +519,7 @@ struct Plan {
     Form form;
     bool tensor;               // the prefix's items are the tcgen05 kernel's
     int prefix_rows, own_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
+    int own_ctas;              // beside the tcgen05 kernel, 0: as many as there are items for
 };
 
 bool mma_takes(const b200_kv_pages& pages) {
@@ -489,24 +530,27 @@ int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Splits of the prefix's keys for the tcgen05 kernel.  Its CTAs have an SM each, and the own tokens' CTAs, which are bound by memory, run on the SMs that
-// it leaves: few splits leave more of them and fewer partial results, many shorten the prefix's own time.  In us: a CTA takes 9 and 0.8 per step; an SM
-// streams up to 60 KB of own keys and values, all of them together 5.5 MB; partial results go out and back at 5 MB.
-int tensor_splits(int64_t items, int max_prefix, double own_bytes, double part_bytes) {
+// How the tcgen05 kernel and the own tokens' kernel share the SMs.  A CTA of the first has an SM to itself; the other's CTAs run on the SMs that its last wave
+// leaves: few splits of the prefix leave more of them and fewer partial results, many shorten the prefix's own time.  Measured, in us: a CTA of the prefix takes
+// 10 and 0.75 (heads of 64: 0.6) per step; a step of own keys takes an SM 0.8, 1.0, 1.7 (0.5, 0.65, 0.9) with tiles of 16, 32 and 64 pairs; partial results go
+// out and back at 5 MB per us.
+struct Share { int splits, own_ctas; };   // own_ctas: 0: as many as there are items for
+Share share_sms(int64_t items, int max_prefix, int dim, int own_rows, double own_steps, double part_bytes, int sms) {
     const int steps = ceil_div(max_prefix, kTensorKeys);
-    int best = 1;
+    const double step = dim > 64 ? 0.75 : 0.6;
+    const double own_step = own_rows == 16 ? (dim > 64 ? 0.8 : 0.5) : own_rows == 32 ? (dim > 64 ? 1.0 : 0.65) : dim > 64 ? 1.7 : 0.9;
+    const double own = own_steps * own_step;
+    Share best{1, 0};
     double least = 1e30;
     for (int n = 1; n <= kMostSplits && n <= steps; ++n) {
-        const int64_t ctas = items * n, waves = ceil_div64(ctas, 148);
-        const double prefix = static_cast<double>(waves) * (9.0 + 0.8 * ceil_div(steps, n));
-        const double rest = static_cast<double>(waves * 148 - ctas);   // SMs that the last wave leaves
-        const double rate = std::min(5.5e6, std::max(rest, 1.0) * 6e4), own = own_bytes / 5.5e6;
-        const double last = 9.0 + 0.8 * ceil_div(steps, n);            // the last wave, beside which own tokens run
-        const double beside = std::min(last, own_bytes / rate);
-        const double time = prefix + std::max(0.0, own - beside * rate / 5.5e6) + n * part_bytes / 5e6;
+        const int64_t ctas = items * n, waves = ceil_div64(ctas, sms);
+        const double wave = 10.0 + step * ceil_div(steps, n);
+        const double rest = static_cast<double>(waves * sms - ctas), prefix = static_cast<double>(waves) * wave;
+        const double free_only = rest > 0 ? std::max(prefix, prefix - wave + own / rest) : 1e30, all = prefix + std::max(0.0, own - rest * wave) / sms;
+        const double time = std::min(free_only, all) + n * part_bytes / 5e6;
         if (time < least) {
             least = time;
-            best = n;
+            best = {n, free_only <= all ? static_cast<int>(2 * rest) : 0};
         }
     }
     return best;
@@ -546,7 +590,10 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
         plan.prefix_splits = splits(filled, max_prefix, 2 * 148);
         return plan;
     }
-    plan.prefix_splits = tensor_splits(filled, max_prefix, static_cast<double>(pass.sequences) * kv_heads * max_length * a.cache.head_dim * 4, static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8);
+    const double own_steps = static_cast<double>(plan.own_tiles == 1 ? pass.sequences : ceil_div64(pairs, plan.own_rows) + pass.sequences / 2) * kv_heads * ceil_div(max_length, kUnit);
+    const Share share = share_sms(filled, max_prefix, a.cache.head_dim, plan.own_rows, own_steps, static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8, 148);
+    plan.prefix_splits = share.splits;
+    plan.own_ctas = share.own_ctas;
     return plan;
 }
 
@@ -579,9 +626,9 @@ template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned item
     return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p);
 }
 
-template <int HD> int launch_mma(const PrefixParams& p, unsigned items, cudaStream_t stream) {
+template <int HD> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
     auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, 4> : p.own_rows == 32 ? prefix_mma_kernel<HD, 2> : prefix_mma_kernel<HD, 1>;
-    constexpr int smem = MmaShape<HD>::smem_bytes;
+    const int smem = MmaShape<HD>::smem_bytes(p.own_rows == 16 ? 4 : p.own_rows == 32 ? 2 : 1);
     MmaMaps maps;
     int box_rows = page_box_rows(p.own.page_size);
     if (p.groups && !p.beside) box_rows = std::min(box_rows, page_box_rows(p.prefix.page_size));   // powers of two
@@ -589,7 +636,7 @@ template <int HD> int launch_mma(const PrefixParams& p, unsigned items, cudaStre
     if (status == B200_OK && p.groups && !p.beside) status = page_maps(p.prefix, box_rows, maps.prefix);
     if (status != B200_OK) return status;
     B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    return cuda_status(launch_dependent(kernel, dim3(items), dim3(kMmaThreads), static_cast<size_t>(smem), stream, maps, p, box_rows), "prefix_mma_kernel launch");
+    return cuda_status(launch_dependent(kernel, dim3(static_cast<unsigned>(std::min(p.items, ctas))), dim3(kMmaThreads), static_cast<size_t>(smem), stream, maps, p, box_rows), "prefix_mma_kernel launch");
 }
 
 }  // namespace
@@ -640,9 +687,11 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     }
     cudaStream_t s = as_stream(stream);
     int status;
+    int ctas = 2 * 148;
     if (plan.form == Form::mma) {
         int device = 0;
         B200_CUDA(cudaGetDevice(&device));
+        ctas = 2 * sm_count(device);
         p.status = device_status_word(device);
         if (!p.status) { set_error("b200_prefix_attention: the device status word could not be allocated"); return B200_NO_DEVICE; }
     }
@@ -651,11 +700,14 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
         if (status != B200_OK) return status;
         p.beside = 1;
     }
-    const unsigned items = static_cast<unsigned>(plan.tensor ? own_items : prefix_items + own_items);
+    p.items = static_cast<int>(plan.tensor ? own_items : prefix_items + own_items);
+    // beside the prefix: CTAs for the SMs that are free at once, or, where those do not suffice, two items per CTA, which begin as SMs become free
+    if (plan.tensor) ctas = plan.own_ctas ? plan.own_ctas : std::max(ctas, (p.items + 1) / 2);
+    const unsigned items = static_cast<unsigned>(p.items);
     if (plan.form == Form::plain)
         status = cuda_status(a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, s) : launch_plain<float>(p, items, s), "prefix_plain_kernel launch");
     else
-        status = p.dim <= 64 ? launch_mma<64>(p, items, s) : p.dim <= 96 ? launch_mma<96>(p, items, s) : launch_mma<128>(p, items, s);
+        status = p.dim <= 64 ? launch_mma<64>(p, ctas, s) : p.dim <= 96 ? launch_mma<96>(p, ctas, s) : launch_mma<128>(p, ctas, s);
     if (status != B200_OK) return status;
     auto merge = p.dim % 4 == 0 ? prefix_merge_kernel<4> : prefix_merge_kernel<1>;
     return cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(merges)), dim3(kMergeWarps * 32), 0, s, p), "prefix_merge_kernel launch");
