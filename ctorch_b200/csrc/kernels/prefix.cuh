@@ -78,52 +78,57 @@ struct Item {
     KeySpan keys;
 };
 
-// Items are numbered split-major inside a kind; the prefix's, which are longer, come first.  Every warp works this out for itself.
-__device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
+// Items are numbered split-major inside a kind; the prefix's, which are longer, come first.
+__device__ __forceinline__ int prefix_items(const PrefixParams& p) { return p.prefix_tiles * p.own.kv_heads * p.prefix_splits; }
+
+// Item `index` of the prefix, worked out by a whole warp.
+__device__ __forceinline__ Item find_prefix_item(const PrefixParams& p, int index) {
     Item it{};
-    const int kv_heads = p.own.kv_heads, prefix_items = p.prefix_tiles * kv_heads * p.prefix_splits;
-    const int lane = threadIdx.x & 31;
-    if (index < prefix_items) {
-        it.kv_head = index % kv_heads;
-        const int rest = index / kv_heads;
-        int tile = rest % p.prefix_tiles;
-        it.split = rest / p.prefix_tiles;
-        // tile -> group: the groups' tile counts are added up 32 at a time
-        for (int base = 0; base < p.groups; base += 32) {
-            const int g = base + lane;
-            int begin = 0, rows = 0, tiles = 0, slot = -1, keys = 0;
-            if (g < p.groups) {   // two rounds of loads that do not wait for one another
-                const int from = __ldg(p.group_first + g), to = __ldg(p.group_first + g + 1);
-                slot = __ldg(p.group_prefix + g);
-                begin = __ldg(p.rows.first + from);
-                rows = max(0, __ldg(p.rows.first + to) - begin);
-                keys = prefix_keys(p, slot);
-                tiles = (rows * p.group + p.prefix_rows - 1) / p.prefix_rows;
-            }
-            int up_to = tiles;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, up_to, o);
-                if (lane >= o) up_to += other;
-            }
-            const unsigned found = __ballot_sync(0xffffffffu, up_to > tile);
-            if (found) {
-                const int from = __ffs(found) - 1;
-                it.row = __shfl_sync(0xffffffffu, begin, from);
-                it.m_count = __shfl_sync(0xffffffffu, rows, from) * p.group;
-                it.m_begin = (tile - __shfl_sync(0xffffffffu, up_to - tiles, from)) * p.prefix_rows;
-                it.slot = __shfl_sync(0xffffffffu, slot, from);
-                keys = __shfl_sync(0xffffffffu, keys, from);
-                it.keys = split_span(keys, p.prefix_splits, it.split);
-                it.visible = keys;
-                it.live = it.keys.begin < it.keys.end;
-                return it;
-            }
-            tile -= __shfl_sync(0xffffffffu, up_to, 31);
+    const int kv_heads = p.own.kv_heads, lane = threadIdx.x & 31;
+    it.kv_head = index % kv_heads;
+    const int rest = index / kv_heads;
+    int tile = rest % p.prefix_tiles;
+    it.split = rest / p.prefix_tiles;
+    // tile -> group: the groups' tile counts are added up 32 at a time
+    for (int base = 0; base < p.groups; base += 32) {
+        const int g = base + lane;
+        int begin = 0, rows = 0, tiles = 0, slot = -1, keys = 0;
+        if (g < p.groups) {   // two rounds of loads that do not wait for one another
+            const int from = __ldg(p.group_first + g), to = __ldg(p.group_first + g + 1);
+            slot = __ldg(p.group_prefix + g);
+            begin = __ldg(p.rows.first + from);
+            rows = max(0, __ldg(p.rows.first + to) - begin);
+            keys = prefix_keys(p, slot);
+            tiles = (rows * p.group + p.prefix_rows - 1) / p.prefix_rows;
         }
-        return it;
+        int up_to = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, up_to, o);
+            if (lane >= o) up_to += other;
+        }
+        const unsigned found = __ballot_sync(0xffffffffu, up_to > tile);
+        if (found) {
+            const int from = __ffs(found) - 1;
+            it.row = __shfl_sync(0xffffffffu, begin, from);
+            it.m_count = __shfl_sync(0xffffffffu, rows, from) * p.group;
+            it.m_begin = (tile - __shfl_sync(0xffffffffu, up_to - tiles, from)) * p.prefix_rows;
+            it.slot = __shfl_sync(0xffffffffu, slot, from);
+            keys = __shfl_sync(0xffffffffu, keys, from);
+            it.keys = split_span(keys, p.prefix_splits, it.split);
+            it.visible = keys;
+            it.live = it.keys.begin < it.keys.end;
+            return it;
+        }
+        tile -= __shfl_sync(0xffffffffu, up_to, 31);
     }
-    index -= prefix_items;
+    return it;
+}
+
+// Item `index` of the own tokens, by any one thread.
+__device__ __forceinline__ Item find_own_item(const PrefixParams& p, int index) {
+    Item it{};
+    const int kv_heads = p.own.kv_heads;
     it.kv_head = index % kv_heads;
     int rest = index / kv_heads;
     const int tile = rest % p.own_tiles;
@@ -145,6 +150,24 @@ __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
     it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
     return it;
 }
+__device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
+    return index < prefix_items(p) ? find_prefix_item(p, index) : find_own_item(p, index - prefix_items(p));
+}
+__device__ __forceinline__ Item item_of_lane(const Item& it, int lane) {
+    Item r;
+    r.live = __shfl_sync(0xffffffffu, it.live, lane);
+    r.causal = __shfl_sync(0xffffffffu, it.causal, lane);
+    r.row = __shfl_sync(0xffffffffu, it.row, lane);
+    r.m_begin = __shfl_sync(0xffffffffu, it.m_begin, lane);
+    r.m_count = __shfl_sync(0xffffffffu, it.m_count, lane);
+    r.kv_head = __shfl_sync(0xffffffffu, it.kv_head, lane);
+    r.slot = __shfl_sync(0xffffffffu, it.slot, lane);
+    r.split = __shfl_sync(0xffffffffu, it.split, lane);
+    r.visible = __shfl_sync(0xffffffffu, it.visible, lane);
+    r.keys.begin = __shfl_sync(0xffffffffu, it.keys.begin, lane);
+    r.keys.end = __shfl_sync(0xffffffffu, it.keys.end, lane);
+    return r;
+}
 
 // A kernel that runs beside the prefix's: that one let it start when everything before both was complete, so it need not wait to begin; its first CTA waits
 // before it ends, so that the kernel is complete no earlier than the other and the merge can wait for this one alone.
@@ -155,7 +178,7 @@ __device__ __forceinline__ void begin_items(const PrefixParams& p) {
 __device__ __forceinline__ void end_items(const PrefixParams& p) {
     if (p.beside && blockIdx.x == 0) grid_dependency_wait();
 }
-__device__ __forceinline__ int first_item(const PrefixParams& p) { return p.beside ? p.prefix_tiles * p.own.kv_heads * p.prefix_splits : 0; }
+__device__ __forceinline__ int first_item(const PrefixParams& p) { return p.beside ? prefix_items(p) : 0; }
 
 // Pair m of an item among the pass's rows * heads, and where it leaves its partial result, a row of [rows * heads][splits].
 __device__ __forceinline__ int64_t pair_row(const PrefixParams& p, const Item& it, int m) {

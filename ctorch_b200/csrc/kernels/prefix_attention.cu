@@ -23,9 +23,23 @@ __host__ __device__ constexpr int plain_smem(int dim) {
     return (kPlainRows * plain_width(dim) + 2 * kPlainKeys * (plain_width(dim) + 4) + kPlainRows * (kPlainKeys + 1)) * static_cast<int>(sizeof(float));
 }
 
+template <class T> __device__ __forceinline__ float4 load_four(const T* p);
+template <> __device__ __forceinline__ float4 load_four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <> __device__ __forceinline__ float4 load_four(const __nv_bfloat16* p) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    return make_float4(bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y));
+}
+// Values d .. d + 3 of a row, zeros past its end.  `whole`: head sizes of 4 n in aligned pools.
+template <class T> __device__ __forceinline__ float4 load_piece(const T* row, int d, int dim, bool whole) {
+    if (whole) return d < dim ? load_four<T>(row + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(d < dim ? load_as_f32(row, d) : 0.0f, d + 1 < dim ? load_as_f32(row, d + 1) : 0.0f, d + 2 < dim ? load_as_f32(row, d + 2) : 0.0f,
+                       d + 3 < dim ? load_as_f32(row, d + 3) : 0.0f);
+}
+
 // A tile of 32 pairs x 32 keys: thread (ty, tx) has the scores of rows 2 ty, 2 ty + 1 with the keys tx + 8 j, and the columns 4 tx + 32 c of their
-// accumulators.
-template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) prefix_plain_kernel(const PrefixParams p) {
+// accumulators; it brings the same columns of the keys ty and ty + 16, up to 128 wide a step ahead.  Bound by the chain of a step (shared memory, f32
+// products) with few CTAs, which the splits are for.
+template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) prefix_plain_kernel(const PrefixParams p, const bool whole) {
     extern __shared__ __align__(16) float plain_shared[];
     begin_items(p);
     const Item it = find_item(p, first_item(p) + blockIdx.x);
@@ -37,11 +51,27 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
     float* weight = value + kPlainKeys * pitch;
     const int thread = threadIdx.x, ty = thread / 8, tx = thread % 8;
     const PagesView& view = it.causal ? p.own : p.prefix;
-    for (int i = thread; i < kPlainRows * width; i += kPlainThreads) {
-        const int m = it.m_begin + i / width, d = i % width;
-        query[i] = m < it.m_count && d < p.dim
-                       ? load_as_f32(static_cast<const T*>(p.query), pair_row(p, it, m) * p.dim + d)
-                       : 0.0f;
+    constexpr bool kAhead = BLOCKS <= 4;
+    float4 next[2][2][BLOCKS];   // [key or value][row][columns]
+    auto fetch = [&](int begin) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int position = begin + ty + 16 * r;
+            int page = -1;
+            if (position < it.keys.end) page = page_of(view, it.slot, position / view.page_size);
+            const int64_t at = page >= 0 ? page_row(view, page, it.kv_head, position % view.page_size) : 0;
+#pragma unroll
+            for (int which = 0; which < 2; ++which)
+#pragma unroll
+                for (int c = 0; c < BLOCKS; ++c)
+                    next[which][r][c] = page >= 0 ? load_piece(static_cast<const T*>(view.pool[which]) + at, 32 * c + 4 * tx, p.dim, whole) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    if (kAhead) fetch(it.keys.begin);
+    for (int i = thread; i < kPlainRows * (width / 4); i += kPlainThreads) {
+        const int m = it.m_begin + i / (width / 4), d = i % (width / 4) * 4;
+        *reinterpret_cast<float4*>(query + 4 * i) =
+            m < it.m_count ? load_piece(static_cast<const T*>(p.query) + pair_row(p, it, m) * p.dim, d, p.dim, whole) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, acc[2][BLOCKS][4] = {};
     int limit[2];
@@ -49,20 +79,16 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
     for (int r = 0; r < 2; ++r) limit[r] = it.causal ? min(it.keys.end, it.visible + divide(it.m_begin + 2 * ty + r, p.by_group)) : it.keys.end;
     for (int begin = it.keys.begin; begin < it.keys.end; begin += kPlainKeys) {
         __syncthreads();
-        for (int i = thread; i < kPlainKeys * width; i += kPlainThreads) {
-            const int r = i / width, d = i % width, position = begin + r;
-            float k = 0.0f, v = 0.0f;
-            if (position < it.keys.end && d < p.dim) {
-                const int page = page_of(view, it.slot, position / view.page_size);
-                if (page >= 0) {
-                    const int64_t at = page_row(view, page, it.kv_head, position % view.page_size) + d;
-                    k = load_as_f32(static_cast<const T*>(view.pool[0]), at);
-                    v = load_as_f32(static_cast<const T*>(view.pool[1]), at);
+        if (!kAhead) fetch(begin);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < BLOCKS; ++c)
+                if (32 * c + 4 * tx < width) {
+                    *reinterpret_cast<float4*>(key + (ty + 16 * r) * pitch + 32 * c + 4 * tx) = next[0][r][c];
+                    *reinterpret_cast<float4*>(value + (ty + 16 * r) * pitch + 32 * c + 4 * tx) = next[1][r][c];
                 }
-            }
-            key[r * pitch + d] = k;
-            value[r * pitch + d] = v;
-        }
+        if (kAhead && begin + kPlainKeys < it.keys.end) fetch(begin + kPlainKeys);
         __syncthreads();
         float score[2][4] = {};
         for (int d = 0; d < width; d += 4) {
@@ -236,15 +262,32 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
         const int across = boxes_per_row(box_rows, p.dim), boxes = kUnit / box_rows * across;   // at most 16 per tensor
         const int which = lane / boxes, block = lane % across, row = lane % boxes / across * box_rows;
         int issued = 0, found = 0;
-        for (int index = blockIdx.x;; index += gridDim.x) {
+        const int shared_items = p.beside ? 0 : prefix_items(p), stride = static_cast<int>(gridDim.x);
+        int index = blockIdx.x, batch = 0;   // own items are found 32 at a time, one per lane, from `batch` on
+        unsigned waiting = 0;                // those of the batch that have work and are still to come
+        Item mine{};
+        while (true) {
             Item it{};
-            const bool any = index < p.items;
-            if (any) {
-                it = find_item(p, first_item(p) + index);
-                if (!it.live) continue;
-            } else {
-                it.m_count = -1;   // no more
+            bool any = false;
+            for (; index < shared_items && !any; index += stride) {
+                it = find_prefix_item(p, index);
+                any = it.live;
             }
+            while (!any) {
+                if (!waiting) {
+                    const int64_t at = index + static_cast<int64_t>(batch + lane) * stride;
+                    if (index + static_cast<int64_t>(batch) * stride >= p.items) break;
+                    mine.live = false;
+                    if (at < p.items) mine = find_own_item(p, static_cast<int>(at) - shared_items);
+                    waiting = __ballot_sync(0xffffffffu, mine.live);
+                    batch += 32;
+                    continue;
+                }
+                it = item_of_lane(mine, __ffs(waiting) - 1);
+                waiting &= waiting - 1;
+                any = true;
+            }
+            if (!any) it.m_count = -1;   // no more
             wait(&item_empty[found & 1], ((found >> 1) & 1) ^ 1);
             if (lane == 0) {
                 item_of[found & 1] = it;
@@ -517,6 +560,7 @@ constexpr int kMostDim = 256;
 enum class Form { plain, mma };
 struct Plan {
     Form form;
+    bool aligned;              // 16-byte addresses, head sizes of 4 n
     bool tensor;               // the prefix's items are the tcgen05 kernel's
     int prefix_rows, own_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
     int own_ctas;              // beside the tcgen05 kernel, 0: as many as there are items for
@@ -532,13 +576,13 @@ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How the tcgen05 kernel and the own tokens' kernel share the SMs.  A CTA of the first has an SM to itself; the other's CTAs run on the SMs that its last wave
 // leaves: few splits of the prefix leave more of them and fewer partial results, many shorten the prefix's own time.  Measured, in us: a CTA of the prefix takes
-// 10 and 0.75 (heads of 64: 0.6) per step; a step of own keys takes an SM 0.8, 1.0, 1.7 (0.5, 0.65, 0.9) with tiles of 16, 32 and 64 pairs; partial results go
+// 10 and 0.75 (heads of 64: 0.6) per step; a step of own keys takes an SM 0.6, 1.0, 1.7 (0.4, 0.65, 0.9) with tiles of 16, 32 and 64 pairs; partial results go
 // out and back at 5 MB per us.
 struct Share { int splits, own_ctas; };   // own_ctas: 0: as many as there are items for
 Share share_sms(int64_t items, int max_prefix, int dim, int own_rows, double own_steps, double part_bytes, int sms) {
     const int steps = ceil_div(max_prefix, kTensorKeys);
     const double step = dim > 64 ? 0.75 : 0.6;
-    const double own_step = own_rows == 16 ? (dim > 64 ? 0.8 : 0.5) : own_rows == 32 ? (dim > 64 ? 1.0 : 0.65) : dim > 64 ? 1.7 : 0.9;
+    const double own_step = own_rows == 16 ? (dim > 64 ? 0.6 : 0.4) : own_rows == 32 ? (dim > 64 ? 1.0 : 0.65) : dim > 64 ? 1.7 : 0.9;
     const double own = own_steps * own_step;
     Share best{1, 0};
     double least = 1e30;
@@ -562,6 +606,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     uintptr_t bits = reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.cache.key) | reinterpret_cast<uintptr_t>(a.cache.value);
     if (a.groups) bits |= reinterpret_cast<uintptr_t>(a.prefix.key) | reinterpret_cast<uintptr_t>(a.prefix.value);
     const bool mma = a.cache.dtype == B200_BF16 && mma_takes(a.cache) && (!a.groups || mma_takes(a.prefix)) && bits % 16 == 0;
+    plan.aligned = bits % 16 == 0 && a.cache.head_dim % 4 == 0;
     const int64_t pairs = pass.rows * group;
     const int groups = a.groups < pass.sequences ? a.groups : pass.sequences;
     const bool prefix = a.groups > 0 && max_prefix > 0;
@@ -575,7 +620,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.prefix_rows) + groups : 0;
     plan.own_tiles = ceil_div(own_pairs, plan.own_rows);
     auto splits = [&](int64_t items, int keys, int ctas) {
-        const int most = ceil_div(keys, 4 * kUnit);
+        const int most = ceil_div(keys, mma ? 4 * kUnit : kUnit);   // the plain kernel takes longer over a step than a partial result costs
         int n = static_cast<int>(ctas / (items > 0 ? items : 1));
         if (n > most) n = most;
         if (n > kMostSplits) n = kMostSplits;
@@ -616,14 +661,14 @@ int check_prefix(const b200_prefix_args* a, const b200_rows* pass, PrefixParams&
     return B200_OK;
 }
 
-template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned items, cudaStream_t stream) {
+template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned items, bool whole, cudaStream_t stream) {
     auto kernel = p.dim <= 64 ? prefix_plain_kernel<T, 2> : p.dim <= 128 ? prefix_plain_kernel<T, 4> : prefix_plain_kernel<T, 8>;
     const int smem = plain_smem(p.dim);
     if (smem > 48 * 1024) {
         const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (status != cudaSuccess) return status;
     }
-    return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p);
+    return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p, whole);
 }
 
 template <int HD> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
@@ -705,7 +750,8 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     if (plan.tensor) ctas = plan.own_ctas ? plan.own_ctas : std::max(ctas, (p.items + 1) / 2);
     const unsigned items = static_cast<unsigned>(p.items);
     if (plan.form == Form::plain)
-        status = cuda_status(a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, s) : launch_plain<float>(p, items, s), "prefix_plain_kernel launch");
+        status = cuda_status(a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, plan.aligned, s) : launch_plain<float>(p, items, plan.aligned, s),
+                             "prefix_plain_kernel launch");
     else
         status = p.dim <= 64 ? launch_mma<64>(p, ctas, s) : p.dim <= 96 ? launch_mma<96>(p, ctas, s) : launch_mma<128>(p, ctas, s);
     if (status != B200_OK) return status;

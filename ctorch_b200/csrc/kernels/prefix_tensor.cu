@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     begin_items(p);
-    const Item it = find_item(p, blockIdx.x);
+    const Item it = find_prefix_item(p, blockIdx.x);
     if (!it.live) return;
     const int tiles = it.m_count - it.m_begin > 128 ? 2 : 1;
     const int steps = (it.keys.end - it.keys.begin + kTensorKeys - 1) / kTensorKeys;

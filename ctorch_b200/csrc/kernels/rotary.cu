@@ -27,14 +27,12 @@ struct TableParams {
     float *cosine, *sine;
 };
 
-// A thread owns one frequency and `run` consecutive positions.
+// A thread owns one frequency and `run` consecutive positions: sine and cosine of the first angle and of the step, then one complex product per position
+// (a few 2^-53 each).  Bound by the stores: 64 k positions and more x 64 frequencies at 5 TB/s (sines and cosines of every single angle: 2 TB/s).
 __global__ void __launch_bounds__(256) rotary_tables_kernel(const TableParams p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int64_t at = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
     const int i = static_cast<int>(at % p.half);
     const int64_t begin = at / p.half * p.run, end = min(begin + p.run, p.positions);
-    if (begin >= end) return;
     double frequency = exp(-static_cast<double>(i) / p.half * p.log_base);
     if (p.kind == B200_ROTARY_LINEAR) frequency /= p.factor;
     if (p.kind == B200_ROTARY_PARTS) {
@@ -42,11 +40,19 @@ __global__ void __launch_bounds__(256) rotary_tables_kernel(const TableParams p)
         const double kept = fmin(1.0, fmax(0.0, (turns - p.low) / (p.high - p.low)));
         frequency *= kept + (1.0 - kept) / p.factor;
     }
+    double s, c, step_s, step_c;
+    sincos(static_cast<double>(p.first + begin) * frequency, &s, &c);
+    sincos(frequency, &step_s, &step_c);
+    s *= p.magnitude;
+    c *= p.magnitude;
+    grid_dependency_wait();   // the tables may still be read
+    grid_launch_dependents();
     for (int64_t q = begin; q < end; ++q) {
-        double s, c;
-        sincos(static_cast<double>(p.first + q) * frequency, &s, &c);
-        p.cosine[q * p.half + i] = static_cast<float>(p.magnitude * c);
-        p.sine[q * p.half + i] = static_cast<float>(p.magnitude * s);
+        p.cosine[q * p.half + i] = static_cast<float>(c);
+        p.sine[q * p.half + i] = static_cast<float>(s);
+        const double next = c * step_c - s * step_s;
+        s = s * step_c + c * step_s;
+        c = next;
     }
 }
 
@@ -74,72 +80,103 @@ template <int V> __device__ __forceinline__ void store_values(void* base, int bf
     }
 }
 
-// An item is 2 V values of one head of one row: entries d .. d + V - 1 and e .. e + V - 1, which turn together in the rotating part.  grid
-// (rows, blocks of items).
+// Where the two quarters of an item lie in its head: d .. d + V - 1 and e .. e + V - 1, which turn together in the rotating part.
+template <int V> __device__ __forceinline__ void item_places(const AppendParams& p, int j, int& d, int& e) {
+    d = j * 2 * V;
+    e = d + V;
+    if (!p.pairs && d < p.rot) {
+        d = j * V;
+        e = d + p.rot / 2;
+    }
+}
+
+// An item is 2 V values of one head of one row.  grid (rows, blocks of items): a block has a whole row where there are rows for every SM, since each block
+// walks from the row to its page (four dependent loads); it asks for the row's values before that.  Bound by memory with many rows, by this chain with few.
+constexpr int kItemsHeld = 4;
 template <int V> __global__ void __launch_bounds__(256) rotary_append_kernel(const AppendParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
     const int row = blockIdx.x;
-    if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
     const int dim = p.cache.head_dim, per_head = dim / (2 * V), kv_heads = p.cache.kv_heads;
-    const int items = (p.heads + 2 * kv_heads) * per_head;
-    const RowPlace place = row_place(p.rows, row);
-    const int64_t turn = static_cast<int64_t>(place.position) + (p.offset ? __ldg(p.offset + place.sequence) : 0);
-    const bool turns = p.rot > 0 && turn >= 0 && turn < p.positions;
-    int page = -1, entry = 0;
-    if (place.slot >= 0 && place.slot < p.cache.sequences && place.position >= 0 && place.position < p.cache.capacity()) {
-        page = page_of(p.cache, place.slot, place.position / p.cache.page_size);
-        entry = place.position % p.cache.page_size;
-    }
+    const int items = (p.heads + 2 * kv_heads) * per_head, stride = gridDim.y * blockDim.x;
     const float* source = p.projected + row * p.stride;
-    const int half = p.rot / 2;
-    const float* cosine = p.cosine + turn * half;
-    const float* sine = p.sine + turn * half;
-    for (int item = blockIdx.y * blockDim.x + threadIdx.x; item < items; item += gridDim.y * blockDim.x) {
-        const int head = item / per_head, j = item % per_head;
-        const bool rotates = turns && head < p.heads + kv_heads && j * 2 * V < p.rot;
-        int d, e;
-        if (!p.pairs && j * 2 * V < p.rot) {
-            d = j * V;
-            e = d + half;
-        } else {
-            d = j * 2 * V;
-            e = d + V;
+    if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
+    bool placed = false, turns = false;
+    int page = -1, entry = 0;
+    const float *cosine = nullptr, *sine = nullptr;
+    for (int first = blockIdx.y * blockDim.x + threadIdx.x; first < items; first += kItemsHeld * stride) {
+        Lanes<V> a[kItemsHeld], b[kItemsHeld];
+#pragma unroll
+        for (int k = 0; k < kItemsHeld; ++k) {
+            const int item = first + k * stride;
+            if (item >= items) break;
+            int d, e;
+            item_places<V>(p, item % per_head, d, e);
+            if (item / per_head >= p.heads + kv_heads) {   // values do not turn
+                d = item % per_head * 2 * V;
+                e = d + V;
+            }
+            a[k] = load_lanes<V>(source + item / per_head * dim + d);
+            b[k] = load_lanes<V>(source + item / per_head * dim + e);
         }
-        Lanes<V> a = load_lanes<V>(source + head * dim + d), b = load_lanes<V>(source + head * dim + e);
-        if (rotates) {
-            if (!p.pairs) {
-                const Lanes<V> c = load_lanes<V>(cosine + d), s = load_lanes<V>(sine + d);
-#pragma unroll
-                for (int u = 0; u < V; ++u) {
-                    const float x = a.v[u], y = b.v[u];
-                    a.v[u] = x * c.v[u] - y * s.v[u];
-                    b.v[u] = y * c.v[u] + x * s.v[u];
-                }
-            } else if constexpr (V == 4) {
-                const Lanes<4> c = load_lanes<4>(cosine + d / 2), s = load_lanes<4>(sine + d / 2);
-                const float x[4] = {a.v[0], a.v[2], b.v[0], b.v[2]}, y[4] = {a.v[1], a.v[3], b.v[1], b.v[3]};
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    Lanes<4>& to = u < 2 ? a : b;
-                    to.v[(u & 1) * 2] = x[u] * c.v[u] - y[u] * s.v[u];
-                    to.v[(u & 1) * 2 + 1] = y[u] * c.v[u] + x[u] * s.v[u];
-                }
-            } else {
-                const float c = cosine[d / 2], s = sine[d / 2], x = a.v[0], y = b.v[0];
-                a.v[0] = x * c - y * s;
-                b.v[0] = y * c + x * s;
+        if (!placed) {
+            placed = true;
+            const RowPlace place = row_place(p.rows, row);
+            const int64_t turn = static_cast<int64_t>(place.position) + (p.offset ? __ldg(p.offset + place.sequence) : 0);
+            turns = p.rot > 0 && turn >= 0 && turn < p.positions;
+            if (place.slot >= 0 && place.slot < p.cache.sequences && place.position >= 0 && place.position < p.cache.capacity()) {
+                page = page_of(p.cache, place.slot, place.position / p.cache.page_size);
+                entry = place.position % p.cache.page_size;
+            }
+            if (turns) {
+                cosine = p.cosine + turn * (p.rot / 2);
+                sine = p.sine + turn * (p.rot / 2);
             }
         }
-        if (head < p.heads) {
-            const int64_t at = (static_cast<int64_t>(row) * p.heads + head) * dim;
-            store_values<V>(p.query, p.query_bf16, at + d, a);
-            store_values<V>(p.query, p.query_bf16, at + e, b);
-        } else if (page >= 0) {
-            const bool value = head >= p.heads + kv_heads;
-            const int64_t at = page_row(p.cache, page, head - p.heads - (value ? kv_heads : 0), entry);
-            store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + d, a);
-            store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + e, b);
+#pragma unroll
+        for (int k = 0; k < kItemsHeld; ++k) {
+            const int item = first + k * stride;
+            if (item >= items) break;
+            const int head = item / per_head, j = item % per_head;
+            int d, e;
+            item_places<V>(p, j, d, e);
+            if (head >= p.heads + kv_heads) {
+                d = j * 2 * V;
+                e = d + V;
+            } else if (turns && j * 2 * V < p.rot) {
+                if (!p.pairs) {
+                    const Lanes<V> c = load_lanes<V>(cosine + d), s = load_lanes<V>(sine + d);
+#pragma unroll
+                    for (int u = 0; u < V; ++u) {
+                        const float x = a[k].v[u], y = b[k].v[u];
+                        a[k].v[u] = x * c.v[u] - y * s.v[u];
+                        b[k].v[u] = y * c.v[u] + x * s.v[u];
+                    }
+                } else if constexpr (V == 4) {
+                    const Lanes<4> c = load_lanes<4>(cosine + d / 2), s = load_lanes<4>(sine + d / 2);
+                    const float x[4] = {a[k].v[0], a[k].v[2], b[k].v[0], b[k].v[2]}, y[4] = {a[k].v[1], a[k].v[3], b[k].v[1], b[k].v[3]};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        Lanes<4>& to = u < 2 ? a[k] : b[k];
+                        to.v[(u & 1) * 2] = x[u] * c.v[u] - y[u] * s.v[u];
+                        to.v[(u & 1) * 2 + 1] = y[u] * c.v[u] + x[u] * s.v[u];
+                    }
+                } else {
+                    const float c = cosine[d / 2], s = sine[d / 2], x = a[k].v[0], y = b[k].v[0];
+                    a[k].v[0] = x * c - y * s;
+                    b[k].v[0] = y * c + x * s;
+                }
+            }
+            if (head < p.heads) {
+                const int64_t at = (static_cast<int64_t>(row) * p.heads + head) * dim;
+                store_values<V>(p.query, p.query_bf16, at + d, a[k]);
+                store_values<V>(p.query, p.query_bf16, at + e, b[k]);
+            } else if (page >= 0) {
+                const bool value = head >= p.heads + kv_heads;
+                const int64_t at = page_row(p.cache, page, head - p.heads - (value ? kv_heads : 0), entry);
+                store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + d, a[k]);
+                store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + e, b[k]);
+            }
         }
     }
 }
@@ -170,8 +207,11 @@ extern "C" int b200_rotary_tables(const b200_rotary_scaling* s, int32_t rot_dims
     if (s->kind == B200_ROTARY_BASE && rot_dims > 2) p.log_base += std::log(s->factor) * rot_dims / (rot_dims - 2);
     p.factor = s->factor; p.original = s->original; p.low = s->low; p.high = s->high;
     p.magnitude = s->magnitude == 0.0 ? 1.0 : s->magnitude;
-    p.kind = s->kind; p.half = rot_dims / 2; p.run = 8;
+    p.kind = s->kind; p.half = rot_dims / 2;
     p.first = first; p.positions = positions; p.cosine = cosine; p.sine = sine;
+    // enough threads for every SM before the runs get longer than a few positions; 32 positions make two pairs of sines and cosines cheap
+    p.run = static_cast<int>(positions * p.half / (148 * 1024));
+    p.run = p.run < 2 ? 2 : p.run > 32 ? 32 : p.run;
     const int64_t threads = (positions + p.run - 1) / p.run * p.half;
     if ((threads + 255) / 256 > INT32_MAX) { set_error("b200_rotary_tables: the tables are too large"); return B200_UNSUPPORTED; }
     return cuda_status(launch_dependent(rotary_tables_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, as_stream(stream), p),
@@ -201,7 +241,8 @@ extern "C" int b200_rotary_append(const b200_rotary_append_args* a, const b200_r
     if (a->rot_dims) bits |= reinterpret_cast<uintptr_t>(a->cosine) | reinterpret_cast<uintptr_t>(a->sine);
     const bool wide = dim % 8 == 0 && a->rot_dims % 8 == 0 && stride % 4 == 0 && bits % 16 == 0;
     const int64_t items = width / (wide ? 8 : 2);
-    const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>((items + 255) / 256 < 65535 ? (items + 255) / 256 : 65535));
+    const int64_t blocks = p.rows.rows >= 148 ? 1 : (items + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>(blocks < 65535 ? blocks : 65535));
     return cuda_status(wide ? launch_dependent(rotary_append_kernel<4>, grid, dim3(256), 0, as_stream(stream), p)
                             : launch_dependent(rotary_append_kernel<1>, grid, dim3(256), 0, as_stream(stream), p),
                        "rotary_append_kernel launch");

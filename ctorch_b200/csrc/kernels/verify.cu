@@ -35,6 +35,12 @@ struct VerifyParams {
 
 __device__ __forceinline__ float weight_of(float x, float most, float inverse) { return expf(__fmul_rn(__fsub_rn(x, most), inverse)); }
 
+// A weight in f64 by its bits (conversions share the exponential's unit, at a quarter of the rate of these operations); weights below 2^-126 count as 0.
+__device__ __forceinline__ double widen(float w) {
+    const uint32_t bits = __float_as_uint(w);   // not negative
+    return bits < 0x00800000u ? 0.0 : __hiloint2double(static_cast<int>((bits >> 3) + (bits < 0x7f800000u ? 0x38000000u : 0x70000000u)), static_cast<int>(bits << 29));
+}
+
 // One CTA's part of a row, in vectors of four values on 16-byte boundaries: vector v holds the values 4 v - shift .. + 3 of the part.
 struct RowPart {
     const float* base;
@@ -151,10 +157,10 @@ template <bool GREEDY> __global__ void __launch_bounds__(kVerifyThreads) verify_
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
             if ((t * kHeld + j) * kVerifyThreads >= own.vectors) break;
-            sum += static_cast<double>(weight_of(held[j].x, most, p.inverse));
-            sum += static_cast<double>(weight_of(held[j].y, most, p.inverse));
-            sum += static_cast<double>(weight_of(held[j].z, most, p.inverse));
-            sum += static_cast<double>(weight_of(held[j].w, most, p.inverse));
+            sum += widen(weight_of(held[j].x, most, p.inverse));
+            sum += widen(weight_of(held[j].y, most, p.inverse));
+            sum += widen(weight_of(held[j].z, most, p.inverse));
+            sum += widen(weight_of(held[j].w, most, p.inverse));
         }
     }
     // values outside the part weigh nothing; where the row's maximum is itself -inf every weight is NaN, as for the values inside
@@ -179,7 +185,11 @@ struct RowStats {
 __device__ __forceinline__ RowStats row_stats(const VerifyParams& p, int row, int side) {
     const int64_t at = 2 * static_cast<int64_t>(row) + side;
     RowStats r{p.row_max[at], 0.0, false};
-    for (int c = 0; c < p.parts; ++c) r.sum += p.row_sum[at * p.parts + c];
+    double part[kVerifyMostParts];
+#pragma unroll
+    for (int c = 0; c < kVerifyMostParts; ++c) part[c] = c < p.parts ? p.row_sum[at * p.parts + c] : 0.0;
+#pragma unroll
+    for (int c = 0; c < kVerifyMostParts; ++c) r.sum += part[c];
     r.good = r.sum > 0.0 && r.sum < INFINITY;
     return r;
 }
@@ -191,11 +201,29 @@ struct Residual {
     int without;                 // the draft that counts as certain, or -1
     bool minus;                  // the draft's probabilities are taken off
     __device__ __forceinline__ double value(float x, float y, int index) const {
-        double left = static_cast<double>(weight_of(x, most, inverse)) * scale;
-        if (minus) left -= static_cast<double>(weight_of(y, draft_most, inverse)) * draft_scale;
+        double left = widen(weight_of(x, most, inverse)) * scale;
+        if (minus) left -= widen(weight_of(y, draft_most, inverse)) * draft_scale;
         return index == without || !(left > 0.0) ? 0.0 : left;
     }
 };
+
+// What the test of a row's draft needs besides the row's sums.
+struct Test {
+    bool valid;
+    float target, draft;
+    double accept;
+};
+__device__ __forceinline__ Test fetch_test(const VerifyParams& p, int row) {
+    Test t{};
+    const int64_t x = __ldg(p.ids + row + 1);
+    t.accept = p.accept[row];
+    t.valid = x >= 0 && x < p.vocab;
+    if (t.valid) {
+        t.target = __ldg(p.logits + row * p.stride + x);
+        if (p.draft) t.draft = __ldg(p.draft + row * p.stride + x);
+    }
+    return t;
+}
 
 // grid: a cluster of `parts` CTAs per sequence.  Dynamic shared memory: the sums of the part's segments of 128 values.
 __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const VerifyParams p) {
@@ -204,11 +232,15 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
     __shared__ double part_total;
     __shared__ Candidate warp_best[kVerifyWarps];
     __shared__ Candidate part_best;
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int part = cluster_part(), s = blockIdx.x / p.parts;
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    // The pass's arrays and the logits were complete before verify_rows_kernel began: what the first tests need is fetched while that still runs.
     const int first = __ldg(p.rows.first + s), last = __ldg(p.rows.first + s + 1) - 1;
+    const double draw = last >= first ? p.draw[s] : 0.0;
+    Test test{};
+    if (warp == 0 && first + lane < last) test = fetch_test(p, first + lane);
+    grid_dependency_wait();
+    grid_launch_dependents();
     if (last < first) {
         if (part == 0 && thread == 0) {
             p.accepted[s] = 0;
@@ -221,19 +253,19 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
         int stop = last;
         for (int base = first; base < last; base += 32) {
             const int row = base + lane;
+            if (base > first && row < last) test = fetch_test(p, row);
             bool refused = false;
             if (row < last) {
-                const int64_t x = __ldg(p.ids + row + 1);
                 refused = true;
-                if (x >= 0 && x < p.vocab) {
+                if (test.valid) {
                     const RowStats t = row_stats(p, row, 0);
                     double q = 1.0;
                     if (p.draft) {
                         const RowStats d = row_stats(p, row, 1);
-                        q = d.good ? static_cast<double>(weight_of(p.draft[row * p.stride + x], d.most, p.inverse)) / d.sum : NAN;
+                        q = d.good ? widen(weight_of(test.draft, d.most, p.inverse)) / d.sum : NAN;
                     }
-                    const double share = t.good ? static_cast<double>(weight_of(p.logits[row * p.stride + x], t.most, p.inverse)) / t.sum : NAN;
-                    refused = !(p.accept[row] * q < share);
+                    const double share = t.good ? widen(weight_of(test.target, t.most, p.inverse)) / t.sum : NAN;
+                    refused = !(test.accept * q < share);
                 }
             }
             const unsigned found = __ballot_sync(0xffffffffu, refused);
@@ -296,18 +328,25 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
         const int run = (segments + 31) / 32;   // segments that a lane of the first warp adds up
         double total, before, lane_before, mine;
         while (true) {
-            for (int g = warp; g < segments; g += kVerifyWarps) {
-                const int v = g * 32 + lane, at = begin + 4 * v - target.shift;
-                double sum = 0.0;
-                if (v < target.vectors) {
-                    const float4 x = target.load(v), y = residual.minus ? draft.load(v, target.shift) : x;
-                    sum = residual.value(x.x, y.x, at);
-                    sum += residual.value(x.y, y.y, at + 1);
-                    sum += residual.value(x.z, y.z, at + 2);
-                    sum += residual.value(x.w, y.w, at + 3);
+            constexpr int kBatch = 4;   // segments of a warp whose values are requested together
+            for (int begin_g = warp; begin_g < segments; begin_g += kBatch * kVerifyWarps) {
+                float4 x[kBatch], y[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int v = (begin_g + k * kVerifyWarps) * 32 + lane;
+                    x[k] = v < target.vectors ? target.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    y[k] = residual.minus && v < target.vectors ? draft.load(v, target.shift) : x[k];
                 }
-                sum = warp_sum(sum);
-                if (lane == 0) segment_sum[g] = sum;
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int g = begin_g + k * kVerifyWarps, at = begin + 4 * (g * 32 + lane) - target.shift;
+                    double sum = residual.value(x[k].x, y[k].x, at);
+                    sum += residual.value(x[k].y, y[k].y, at + 1);
+                    sum += residual.value(x[k].z, y[k].z, at + 2);
+                    sum += residual.value(x[k].w, y[k].w, at + 3);
+                    sum = warp_sum(sum);
+                    if (lane == 0 && g < segments) segment_sum[g] = sum;
+                }
             }
             __syncthreads();
             if (warp == 0) {
@@ -335,7 +374,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
             residual.without = -1;
             cluster_sync_all();
         }
-        const double wanted = p.draw[s] * total;
+        const double wanted = draw * total;
         // the first part whose running sum exceeds what is wanted; by rounding there may be none, then the last with any weight
         int chosen = -1, heavy = 0;
         double running = 0.0;
