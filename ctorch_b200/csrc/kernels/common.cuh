@@ -62,6 +62,30 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 __device__ __forceinline__ int warp_max_int(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
+// Two f32 at a time: each half is rounded as the scalar operation would.
+struct Two { uint64_t bits; };
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits)); }
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+__device__ __forceinline__ Two mul_two(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Two add_two(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+
 // SiLU exactly as the reference states it: v * sigmoid(v), sigmoid through exp(-|v|) in two branches
 // (src/kernels/cpu/pointwise.cpp:31-34,57 of the reference).
 __device__ __forceinline__ float silu_reference(float v) {

@@ -33,24 +33,6 @@ template <int HD> struct TensorShape {
 __device__ __forceinline__ int key_item(int step) { return step ? 2 * step - 1 : 0; }
 __device__ __forceinline__ int value_item(int step, int steps) { return step + 1 < steps ? 2 * step + 2 : 2 * steps - 1; }
 
-// Two f32 at a time.
-struct Two { uint64_t bits; };
-__device__ __forceinline__ Two two(float a, float b) {
-    Two r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void split(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits)); }
-__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
-    Two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-    return r;
-}
-__device__ __forceinline__ Two add_two(Two a, Two b) {
-    Two r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
-    return r;
-}
 // 2^x for x <= 8 on the FMA units: 2^x = 2^n 2^f with n the nearest integer and |f| <= 1/2, 2^f by a polynomial whose relative error is the smallest one
 // of degree 5 (fitted on Chebyshev points; 2.3e-7 as evaluated in f32), 2^n by its exponent.  Below 2^-126 the result is 2^-126.  `odd` becomes NaN where x is.
 __device__ __forceinline__ Two exp2_polynomial(Two x, Two& odd) {

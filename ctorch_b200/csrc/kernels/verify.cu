@@ -1,11 +1,14 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers.
 //
 // Two launches.  verify_rows_kernel: for every row of target and draft logits the maximum and the sum of its weights exp((x - max) / T); a row is
-// split over a cluster of CTAs that hold their part in registers, so the row is read once although the weights need the maximum first.
+// split over a cluster of CTAs that hold their part in shared memory, so the row is read once although the weights need the maximum first.
 // verify_finish_kernel: one cluster per sequence walks the acceptance tests, then draws from the residual of the row that refused: running sums
-// over segments of 128 values, in index order.  All sums are f64 and added in a fixed order, so the choice does not depend on the launch.
+// over segments of 128 values, in index order.  All sums are as good as f64 and added in a fixed order.
 #include "linear_common.cuh"
+#include "mma.cuh"
 #include "rows.cuh"
+
+#include <algorithm>
 
 #include <cmath>
 
@@ -14,7 +17,11 @@ namespace {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kHeld = 16;                                    // 16-byte vectors of a row that a thread keeps in registers
+constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
+constexpr int kPieceVectors = 1024, kTilePieces = 4;
+constexpr int kTileVectors = kTilePieces * kPieceVectors;    // 16-byte vectors of a row that a CTA holds
+constexpr int kSweeps = kPieceVectors / kRowThreads;         // of the block's threads over a piece
+static_assert(kTileVectors / kRowThreads * 4 / 2 <= 64);     // see add_weights: values of a thread per half of a sum
 constexpr int kVerifyMostParts = 8;
 
 struct VerifyParams {
@@ -22,6 +29,7 @@ struct VerifyParams {
     const float *logits, *draft;
     int64_t stride;
     int vocab, parts, chunk;      // CTAs per row, values per CTA (a multiple of 4)
+    int draw_parts, draw_chunk;   // the same of the drawing clusters
     float inverse;
     const int64_t* ids;
     const double *accept, *draw;
@@ -31,6 +39,7 @@ struct VerifyParams {
     float* row_max;               // [2 * rows]: target and draft of each row
     double* row_sum;              // [2 * rows][parts]
     Candidate* best;              // greedy: [rows][parts]
+    int32_t* status;
 };
 
 __device__ __forceinline__ float weight_of(float x, float most, float inverse) { return expf(__fmul_rn(__fsub_rn(x, most), inverse)); }
@@ -41,14 +50,26 @@ __device__ __forceinline__ double widen(float w) {
     return bits < 0x00800000u ? 0.0 : __hiloint2double(static_cast<int>((bits >> 3) + (bits < 0x7f800000u ? 0x38000000u : 0x70000000u)), static_cast<int>(bits << 29));
 }
 
+// Adds the weights of two values to a sum in two parts: multiples of 2^-17, of which the at most 64 that a thread adds are exact in f32, and what is left of each
+// weight, at most 2^-18, whose sum is off by 2^-36 at most: together as good as f64 sums, at four packed operations for two values (a conversion to
+// f64 for each value takes the exponential's unit).
+__device__ __forceinline__ void add_weights(Two x, Two minus_most, Two inverse, Two& coarse, Two& fine) {
+    float a, b;
+    split(mul_two(add_two(x, minus_most), inverse), a, b);
+    const Two w = two(expf(a), expf(b));
+    const Two high = add_two(add_two(w, two(96.0f, 96.0f)), two(-96.0f, -96.0f));
+    coarse = add_two(coarse, high);
+    fine = add_two(fine, fma_two(high, two(-1.0f, -1.0f), w));
+}
+
 // One CTA's part of a row, in vectors of four values on 16-byte boundaries: vector v holds the values 4 v - shift .. + 3 of the part.
 struct RowPart {
     const float* base;
     int length, shift, vectors;
-    __device__ __forceinline__ RowPart(const VerifyParams& p, const float* row, int part) {
-        const int begin = min(p.vocab, part * p.chunk);
+    __device__ __forceinline__ RowPart(int vocab, int chunk, const float* row, int part) {
+        const int begin = min(vocab, part * chunk);
         base = row + begin;
-        length = min(p.vocab, begin + p.chunk) - begin;
+        length = min(vocab, begin + chunk) - begin;
         shift = static_cast<int>((reinterpret_cast<uintptr_t>(base) >> 2) & 3);
         vectors = length > 0 ? (length + shift + 3) / 4 : 0;
     }
@@ -62,6 +83,17 @@ struct RowPart {
         return make_float4(r[0], r[1], r[2], r[3]);
     }
     __device__ __forceinline__ float4 load(int v) const { return load(v, shift); }
+    __device__ __forceinline__ float4 load_or_none(int v) const { return v < vectors ? load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
+    // A vector as it lies in memory, without what lies outside the part.
+    __device__ __forceinline__ float4 inside(float4 x, int v) const {
+        const int at = 4 * v - shift;
+        if (at >= 0 && at + 4 <= length) return x;
+        x.x = at >= 0 && at < length ? x.x : -INFINITY;
+        x.y = at + 1 >= 0 && at + 1 < length ? x.y : -INFINITY;
+        x.z = at + 2 >= 0 && at + 2 < length ? x.z : -INFINITY;
+        x.w = at + 3 >= 0 && at + 3 < length ? x.w : -INFINITY;
+        return x;
+    }
 };
 
 __device__ __forceinline__ int cluster_part() {
@@ -75,93 +107,110 @@ __device__ __forceinline__ double load_cluster_double(uint32_t address) {
     return value;
 }
 
-// grid: clusters of `parts` CTAs, two (target, draft) or one per row.
-template <bool GREEDY> __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const VerifyParams p) {
-    __shared__ float warp_max_of[kVerifyWarps];
-    __shared__ double warp_sum_of[kVerifyWarps];
-    __shared__ Candidate warp_best[kVerifyWarps];
+__device__ __forceinline__ float most_of(float4 x) { return fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)); }
+
+// grid: clusters of `parts` CTAs, two (target, draft) or one per row.  A part's first kTileVectors come to shared memory with bulk copies and stay for the
+// second pass; longer parts are read twice.  Bound by the chain of a CTA (9 us: launch of the cluster, its row's place, copy, the cluster's barrier, 14 instructions
+// per value), of which an SM holds three with 64 KB each: 825 rows of 128256 take 124 us, 3 TB/s.  What did not help: several rows per cluster with the next one's
+// copies under way (+15%), a cluster per sequence that stops at the first refusal (+50%), 512 threads (+10%).
+__global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const VerifyParams p) {
+    extern __shared__ __align__(128) float4 tile[];
+    __shared__ uint64_t full[kTilePieces];
+    __shared__ float warp_max_of[kRowWarps];
+    __shared__ double warp_sum_of[kRowWarps];
     __shared__ float part_max;
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    if (thread == 0) {
+        for (int i = 0; i < kTilePieces; ++i) mbar_init(&full[i], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
     const int part = cluster_part(), unit = blockIdx.x / p.parts;
-    const int sides = p.draft && !GREEDY ? 2 : 1;
+    const int sides = p.draft ? 2 : 1;
     const int row = unit / sides, side = unit % sides;
     // (the whole cluster leaves together)
     if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
     if (side == 1 && row + 1 == __ldg(p.rows.first + __ldg(p.rows.sequence + row) + 1)) return;
-    const RowPart own(p, (side ? p.draft : p.logits) + row * p.stride, part);
-    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
-    const int tiles = max(1, (own.vectors + kVerifyThreads * kHeld - 1) / (kVerifyThreads * kHeld));
-    float4 held[kHeld];
-    if constexpr (GREEDY) {
-        Candidate best{-INFINITY, INT32_MAX};
-        for (int t = 0; t < tiles; ++t) {
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int v = (t * kHeld + j) * kVerifyThreads + thread;
-                held[j] = v < own.vectors ? own.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const RowPart own(p.vocab, p.chunk, (side ? p.draft : p.logits) + row * p.stride, part);
+    const int tiled = min(own.vectors, kTileVectors);
+    if (thread == 0)
+        for (int piece = 0; piece * kPieceVectors < tiled; ++piece) {
+            int begin = piece * kPieceVectors, end = min(begin + kPieceVectors, tiled);
+            // The vectors at the part's ends may reach into its neighbours, which are in the buffer but for the first row's begin and the last row's end.
+            if (begin == 0 && own.shift && row == 0 && part == 0) {
+                for (int u = own.shift; u < 4; ++u) reinterpret_cast<float*>(tile)[u] = u - own.shift < own.length ? __ldg(own.base + u - own.shift) : 0.0f;
+                ++begin;
             }
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int at = 4 * ((t * kHeld + j) * kVerifyThreads + thread) - own.shift;
-                const float x[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
-#pragma unroll
+            if (begin < end && 4 * end - own.shift > own.length && row == p.rows.rows - 1) {
+                --end;
                 for (int u = 0; u < 4; ++u) {
-                    const Candidate other{x[u], part * p.chunk + at + u};
-                    if (at + u >= 0 && at + u < own.length && preferred(other, best)) best = other;
+                    const int at = 4 * end - own.shift + u;
+                    reinterpret_cast<float*>(tile + end)[u] = at >= 0 && at < own.length ? __ldg(own.base + at) : 0.0f;
                 }
             }
+            mbar_expect_tx(&full[piece], begin < end ? (end - begin) * 16 : 0);
+            if (begin < end) bulk_load(tile + begin, own.base - own.shift + 4 * begin, (end - begin) * 16, &full[piece]);
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            const Candidate other{__shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.index, o)};
-            if (preferred(other, best)) best = other;
-        }
-        if (lane == 0) warp_best[warp] = best;
-        __syncthreads();
-        if (thread == 0) {
-            for (int w = 1; w < kVerifyWarps; ++w)
-                if (preferred(warp_best[w], best)) best = warp_best[w];
-            p.best[static_cast<int64_t>(row) * p.parts + part] = best;
-        }
-        return;
-    }
     float most = -INFINITY;
-    for (int t = tiles - 1; t >= 0; --t) {   // the first tile stays in the registers
+    for (int v = kTileVectors + thread; v < own.vectors; v += kPieceVectors) {
+        float4 x[kSweeps];
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int v = (t * kHeld + j) * kVerifyThreads + thread;
-            held[j] = v < own.vectors ? own.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (int j = 0; j < kSweeps; ++j) x[j] = own.load_or_none(v + j * kRowThreads);
+#pragma unroll
+        for (int j = 0; j < kSweeps; ++j) most = fmaxf(most, most_of(x[j]));
+    }
+    const int sweeps = max(0, tiled - 1) / kRowThreads;   // whole ones, before the part's last vector
+    const float4* mine = tile + thread;
+    for (int piece = 0; piece * kPieceVectors < tiled; ++piece) {
+        if (!mbar_wait(&full[piece], 0)) atomicExch(p.status, B200_DEVICE_TIMEOUT);
+        if (piece == 0 && thread == 0 && own.shift) tile[0] = own.inside(tile[0], 0);
+        if (kSweeps * (piece + 1) <= sweeps) {
+#pragma unroll
+            for (int j = 0; j < kSweeps; ++j) most = fmaxf(most, most_of(mine[(kSweeps * piece + j) * kRowThreads]));
+            continue;
         }
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j) most = fmaxf(most, fmaxf(fmaxf(held[j].x, held[j].y), fmaxf(held[j].z, held[j].w)));
+        for (int v = piece * kPieceVectors + thread; v < min(tiled, (piece + 1) * kPieceVectors); v += kRowThreads) {
+            if (v == own.vectors - 1) tile[v] = own.inside(tile[v], v);
+            most = fmaxf(most, most_of(tile[v]));
+        }
     }
     most = warp_max(most);
     if (lane == 0) warp_max_of[warp] = most;
     __syncthreads();
-    if (thread == 0) {
-        for (int w = 1; w < kVerifyWarps; ++w) most = fmaxf(most, warp_max_of[w]);
-        part_max = most;
+    most = warp_max(lane < kRowWarps ? warp_max_of[lane] : -INFINITY);
+    if (p.parts > 1) {
+        if (thread == 0) part_max = most;
+        cluster_sync_all();
+        most = warp_max(lane < p.parts ? load_cluster_float(map_peer_shared(smem_u32(&part_max), static_cast<uint32_t>(lane))) : -INFINITY);
     }
-    cluster_sync_all();
-    most = -INFINITY;
-    for (int c = 0; c < p.parts; ++c) most = fmaxf(most, load_cluster_float(map_peer_shared(smem_u32(&part_max), static_cast<uint32_t>(c))));
     double sum = 0.0;
-    for (int t = 0; t < tiles; ++t) {
-        if (t > 0) {
+    Two coarse = two(0.0f, 0.0f), fine = two(0.0f, 0.0f);
+    const Two minus_most = two(-most, -most), inverse = two(p.inverse, p.inverse);
+    auto fold = [&] {
+        float a, b, c, d;
+        split(coarse, a, b);
+        split(fine, c, d);
+        sum += (static_cast<double>(a) + static_cast<double>(b)) + (static_cast<double>(c) + static_cast<double>(d));
+    };
+    auto add = [&](float4 x) {
+        add_weights(two(x.x, x.y), minus_most, inverse, coarse, fine);
+        add_weights(two(x.z, x.w), minus_most, inverse, coarse, fine);
+    };
+    for (int sweep = 0; sweep + 4 <= sweeps; sweep += 4)
 #pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int v = (t * kHeld + j) * kVerifyThreads + thread;
-                held[j] = v < own.vectors ? own.load(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            }
-        }
+        for (int j = 0; j < 4; ++j) add(mine[(sweep + j) * kRowThreads]);
+    for (int v = sweeps / 4 * 4 * kRowThreads + thread; v < tiled; v += kRowThreads) add(tile[v]);
+    fold();
+    for (int v = kTileVectors + thread; v < own.vectors; v += kPieceVectors) {
+        float4 x[kSweeps];
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            if ((t * kHeld + j) * kVerifyThreads >= own.vectors) break;
-            sum += widen(weight_of(held[j].x, most, p.inverse));
-            sum += widen(weight_of(held[j].y, most, p.inverse));
-            sum += widen(weight_of(held[j].z, most, p.inverse));
-            sum += widen(weight_of(held[j].w, most, p.inverse));
-        }
+        for (int j = 0; j < kSweeps; ++j) x[j] = own.load_or_none(v + j * kRowThreads);
+        coarse = fine = two(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < kSweeps; ++j) add(x[j]);
+        fold();
     }
     // values outside the part weigh nothing; where the row's maximum is itself -inf every weight is NaN, as for the values inside
     sum = warp_sum(sum);
@@ -169,12 +218,51 @@ template <bool GREEDY> __global__ void __launch_bounds__(kVerifyThreads) verify_
     __syncthreads();
     if (thread == 0) {
         sum = 0.0;
-        for (int w = 0; w < kVerifyWarps; ++w) sum += warp_sum_of[w];
+        for (int w = 0; w < kRowWarps; ++w) sum += warp_sum_of[w];
         const int64_t at = 2 * static_cast<int64_t>(row) + side;
         p.row_sum[at * p.parts + part] = sum;
         if (part == 0) p.row_max[at] = most;
     }
-    cluster_sync_all();   // the peers have read this CTA's maximum
+    if (p.parts > 1) cluster_sync_all();   // the peers have read this CTA's maximum
+}
+
+// Temperature 0: the first maximum of every row.  grid: rows * parts.
+__global__ void __launch_bounds__(kVerifyThreads) verify_best_kernel(const VerifyParams p) {
+    __shared__ Candidate warp_best[kVerifyWarps];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
+    const RowPart own(p.vocab, p.chunk, p.logits + row * p.stride, part);
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    constexpr int kBatch = 8;
+    Candidate best{-INFINITY, INT32_MAX};
+    for (int begin = thread; begin < own.vectors; begin += kBatch * kVerifyThreads) {
+        float4 x[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) x[j] = own.load_or_none(begin + j * kVerifyThreads);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int at = 4 * (begin + j * kVerifyThreads) - own.shift;
+            const float values[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const Candidate other{values[u], part * p.chunk + at + u};
+                if (at + u >= 0 && at + u < own.length && preferred(other, best)) best = other;
+            }
+        }
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        const Candidate other{__shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.index, o)};
+        if (preferred(other, best)) best = other;
+    }
+    if (lane == 0) warp_best[warp] = best;
+    __syncthreads();
+    if (thread == 0) {
+        for (int w = 1; w < kVerifyWarps; ++w)
+            if (preferred(warp_best[w], best)) best = warp_best[w];
+        p.best[static_cast<int64_t>(row) * p.parts + part] = best;
+    }
 }
 
 struct RowStats {
@@ -225,14 +313,14 @@ __device__ __forceinline__ Test fetch_test(const VerifyParams& p, int row) {
     return t;
 }
 
-// grid: a cluster of `parts` CTAs per sequence.  Dynamic shared memory: the sums of the part's segments of 128 values.
+// grid: a cluster of `draw_parts` CTAs per sequence.  Dynamic shared memory: the sums of the part's segments of 128 values.
 __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const VerifyParams p) {
     extern __shared__ double segment_sum[];
     __shared__ int stop_row;
     __shared__ double part_total;
     __shared__ Candidate warp_best[kVerifyWarps];
     __shared__ Candidate part_best;
-    const int part = cluster_part(), s = blockIdx.x / p.parts;
+    const int part = cluster_part(), s = blockIdx.x / p.draw_parts;
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
     // The pass's arrays and the logits were complete before verify_rows_kernel began: what the first tests need is fetched while that still runs.
     const int first = __ldg(p.rows.first + s), last = __ldg(p.rows.first + s + 1) - 1;
@@ -293,9 +381,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
             }
         }
     }
-    const RowPart target(p, p.logits + row * p.stride, part);
-    const RowPart draft(p, (p.draft ? p.draft : p.logits) + row * p.stride, part);
-    const int begin = part * p.chunk;
+    const RowPart target(p.vocab, p.draw_chunk, p.logits + row * p.stride, part);
+    const RowPart draft(p.vocab, p.draw_chunk, (p.draft ? p.draft : p.logits) + row * p.stride, part);
+    const int begin = part * p.draw_chunk;
     if (!stats.good) {   // no distribution: the argmax, as b200_argmax has it
         Candidate best{-INFINITY, INT32_MAX};
         for (int i = thread; i < target.length; i += kVerifyThreads) {
@@ -315,7 +403,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
         }
         cluster_sync_all();
         if (part == 0 && thread == 0) {
-            for (int c = 1; c < p.parts; ++c) {
+            for (int c = 1; c < p.draw_parts; ++c) {
                 const float2 raw = load_cluster_float2(map_peer_shared(smem_u32(&part_best), static_cast<uint32_t>(c)));
                 const Candidate other{raw.x, __float_as_int(raw.y)};
                 if (preferred(other, best)) best = other;
@@ -364,7 +452,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
             }
             cluster_sync_all();
             total = before = 0.0;
-            for (int c = 0; c < p.parts; ++c) {
+            for (int c = 0; c < p.draw_parts; ++c) {
                 if (c == part) before = total;
                 total += load_cluster_double(map_peer_shared(smem_u32(&part_total), static_cast<uint32_t>(c)));
             }
@@ -378,7 +466,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
         // the first part whose running sum exceeds what is wanted; by rounding there may be none, then the last with any weight
         int chosen = -1, heavy = 0;
         double running = 0.0;
-        for (int c = 0; c < p.parts; ++c) {
+        for (int c = 0; c < p.draw_parts; ++c) {
             const double here = load_cluster_double(map_peer_shared(smem_u32(&part_total), static_cast<uint32_t>(c)));
             running += here;
             if (here > 0.0) heavy = c;
@@ -476,12 +564,15 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyParams p
     }
 }
 
-// CTAs per row: a CTA keeps its part of a row in registers.
-int verify_parts(int64_t vocab) {
+// CTAs per row: parts that a CTA can hold, and more, of 2048 values at least, where there are fewer CTAs than wanted.  Parts of a size cost a cluster's launch and
+// barriers each: 64 x 7 rows of 32000 take 43 us with two parts per row, 60 with eight; 15 rows of 50257 take 31 us with four parts and 29 with eight.
+int split_rows(int64_t vocab, int64_t rows, int64_t ctas) {
+    constexpr int kLeast = 2048;
     int parts = 1;
-    while (parts < kVerifyMostParts && vocab > static_cast<int64_t>(parts) * 4096) parts *= 2;
+    while (parts < kVerifyMostParts && (vocab > static_cast<int64_t>(parts) * (4 * kTileVectors - 8) || (rows * parts < ctas && vocab >= 2 * parts * kLeast))) parts *= 2;
     return parts;
 }
+int chunk_of(int vocab, int parts) { return ((vocab + parts - 1) / parts + 3) / 4 * 4; }
 
 }  // namespace
 }  // namespace b200
@@ -512,8 +603,11 @@ extern "C" int b200_verify_drafts(const b200_verify_args* a, const b200_rows* pa
     }
     const bool greedy = a->temperature == 0.0;
     p.logits = a->logits; p.draft = greedy ? nullptr : a->draft_logits; p.stride = a->stride ? a->stride : a->vocab;
-    p.vocab = static_cast<int>(a->vocab); p.parts = verify_parts(a->vocab);
-    p.chunk = ((p.vocab + p.parts - 1) / p.parts + 3) / 4 * 4;
+    p.vocab = static_cast<int>(a->vocab);
+    p.parts = split_rows(p.vocab, static_cast<int64_t>(p.rows.rows) * (p.draft ? 2 : 1), 2 * 148);
+    p.chunk = chunk_of(p.vocab, p.parts);
+    p.draw_parts = split_rows(p.vocab, p.rows.sequences, 4 * 148);
+    p.draw_chunk = chunk_of(p.vocab, p.draw_parts);
     p.inverse = inverse; p.ids = a->ids; p.accept = a->accept; p.draw = a->draw; p.accepted = a->accepted; p.next = a->next; p.advance = a->advance != 0;
     const size_t units = 2 * static_cast<size_t>(p.rows.rows);
     p.row_sum = static_cast<double*>(scratch);
@@ -522,19 +616,23 @@ extern "C" int b200_verify_drafts(const b200_verify_args* a, const b200_rows* pa
     cudaStream_t st = as_stream(stream);
     const int64_t ctas = static_cast<int64_t>(p.rows.rows) * (p.draft ? 2 : 1) * p.parts;
     if (ctas > INT32_MAX) { set_error("b200_verify_drafts: too many rows"); return B200_UNSUPPORTED; }
-    const dim3 cluster(static_cast<unsigned>(p.parts), 1, 1);
     if (greedy) {
-        int status = cuda_status(launch_dependent_cluster(verify_rows_kernel<true>, dim3(static_cast<unsigned>(ctas)), dim3(kVerifyThreads), 0, st, cluster, p),
-                                 "verify_rows_kernel launch");
+        const int status = cuda_status(launch_dependent(verify_best_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kVerifyThreads), 0, st, p), "verify_best_kernel launch");
         if (status != B200_OK) return status;
         return cuda_status(launch_dependent(verify_greedy_kernel, dim3(static_cast<unsigned>((p.rows.sequences + 3) / 4)), dim3(128), 0, st, p),
                            "verify_greedy_kernel launch");
     }
-    const int status = cuda_status(launch_dependent_cluster(verify_rows_kernel<false>, dim3(static_cast<unsigned>(ctas)), dim3(kVerifyThreads), 0, st, cluster, p),
-                                   "verify_rows_kernel launch");
+    int device = 0;
+    B200_CUDA(cudaGetDevice(&device));
+    p.status = device_status_word(device);
+    if (!p.status) { set_error("b200_verify_drafts: the device status word could not be allocated"); return B200_NO_DEVICE; }
+    const size_t held = static_cast<size_t>(std::min((p.chunk + 6) / 4, kTileVectors)) * 16;
+    B200_CUDA(cudaFuncSetAttribute(verify_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileVectors * 16));
+    const int status = cuda_status(launch_dependent_cluster(verify_rows_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kRowThreads), held, st,
+                                                            dim3(static_cast<unsigned>(p.parts), 1, 1), p), "verify_rows_kernel launch");
     if (status != B200_OK) return status;
-    const size_t smem = static_cast<size_t>((p.chunk + 3) / 4 + 1 + 31) / 32 * sizeof(double);
+    const size_t smem = static_cast<size_t>((p.draw_chunk + 3) / 4 + 1 + 31) / 32 * sizeof(double);
     if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(verify_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    return cuda_status(launch_dependent_cluster(verify_finish_kernel, dim3(static_cast<unsigned>(p.rows.sequences * p.parts)), dim3(kVerifyThreads), smem, st, cluster, p),
-                       "verify_finish_kernel launch");
+    return cuda_status(launch_dependent_cluster(verify_finish_kernel, dim3(static_cast<unsigned>(p.rows.sequences * p.draw_parts)), dim3(kVerifyThreads), smem, st,
+                                                dim3(static_cast<unsigned>(p.draw_parts), 1, 1), p), "verify_finish_kernel launch");
 }
