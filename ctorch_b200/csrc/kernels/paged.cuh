@@ -5,6 +5,20 @@
 
 namespace b200 {
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^k the power of two from d on and f = ceil(2^(31 + k) / d) < 2^32, f d - 2^(31 + k) < d <= 2^k, so
+// n f / 2^(31 + k) exceeds n / d by less than n 2^k / (d 2^(31 + k)) < 1 / d.
+struct Divider {
+    uint32_t factor;
+    int shift;   // -1: d = 1
+};
+inline Divider divider(int d) {
+    int k = 0;
+    while ((1 << k) < d) ++k;
+    if (k == 0) return {0, -1};
+    return {static_cast<uint32_t>(((uint64_t{1} << (31 + k)) + d - 1) / d), k - 1};
+}
+__device__ __forceinline__ int divide(int n, Divider d) { return d.shift < 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.factor) >> d.shift); }
+
 struct PagesView {
     void* pool[2];  // 0 = K, 1 = V
     const int32_t* table;

@@ -1,8 +1,10 @@
 // Rotary positions: tables of cosines and sines, scaled for long contexts, and the rotation of the queries and keys of a packed pass with
 // the append of its keys and values to paged caches.
+#include "mma.cuh"
 #include "paged.cuh"
 #include "rows.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace b200 {
@@ -66,6 +68,7 @@ struct AppendParams {
     int64_t stride;
     int query_bf16;
     void* query;
+    Divider by_head;   // items of a head
 };
 
 template <int V> __device__ __forceinline__ void store_values(void* base, int bf16, int64_t at, const Lanes<V>& v) {
@@ -90,93 +93,112 @@ template <int V> __device__ __forceinline__ void item_places(const AppendParams&
     }
 }
 
-// An item is 2 V values of one head of one row.  grid (rows, blocks of items): a block has a whole row where there are rows for every SM, since each block
-// walks from the row to its page (four dependent loads); it asks for the row's values before that.  Bound by memory with many rows, by this chain with few.
+// Where a row's keys and values go, and the row of the tables that turns it; -1 for none.
+struct AppendPlace { int page, entry, turn; };
+__device__ __forceinline__ AppendPlace append_place(const AppendParams& p, int row) {
+    AppendPlace at{-1, 0, -1};
+    const int s = __ldg(p.rows.sequence + row), slot = __ldg(p.rows.slot + s);
+    if (slot < 0 || slot >= p.cache.sequences) return at;
+    const int position = p.rows.lengths[slot] + row - __ldg(p.rows.first + s);
+    const int64_t turn = static_cast<int64_t>(position) + (p.offset ? __ldg(p.offset + s) : 0);
+    if (p.rot > 0 && turn >= 0 && turn < p.positions) at.turn = static_cast<int>(turn);
+    if (position >= 0 && position < p.cache.capacity()) {
+        at.page = page_of(p.cache, slot, position / p.cache.page_size);
+        at.entry = position % p.cache.page_size;
+    }
+    return at;
+}
+
+// Turns an item by its row's cosines and sines.
+template <int V> __device__ __forceinline__ void turn_item(const AppendParams& p, int d, const float* cosine, const float* sine, Lanes<V>& a, Lanes<V>& b) {
+    if (!p.pairs) {
+        const Lanes<V> c = load_lanes<V>(cosine + d), s = load_lanes<V>(sine + d);
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            const float x = a.v[u], y = b.v[u];
+            a.v[u] = x * c.v[u] - y * s.v[u];
+            b.v[u] = y * c.v[u] + x * s.v[u];
+        }
+    } else if constexpr (V == 4) {
+        const Lanes<4> c = load_lanes<4>(cosine + d / 2), s = load_lanes<4>(sine + d / 2);
+        const float x[4] = {a.v[0], a.v[2], b.v[0], b.v[2]}, y[4] = {a.v[1], a.v[3], b.v[1], b.v[3]};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            Lanes<4>& to = u < 2 ? a : b;
+            to.v[(u & 1) * 2] = x[u] * c.v[u] - y[u] * s.v[u];
+            to.v[(u & 1) * 2 + 1] = y[u] * c.v[u] + x[u] * s.v[u];
+        }
+    } else {
+        const float c = cosine[d / 2], s = sine[d / 2], x = a.v[0], y = b.v[0];
+        a.v[0] = x * c - y * s;
+        b.v[0] = y * c + x * s;
+    }
+}
+
+template <int V> __device__ __forceinline__ void store_item(void* base, int bf16, int64_t to, int d, int e, const Lanes<V>& a, const Lanes<V>& b) {
+    if (V == 4 && bf16 && e == d + V) {
+        const uint4 x = make_uint4(pack_bf16(a.v[0], a.v[1 % V]), pack_bf16(a.v[2 % V], a.v[3 % V]), pack_bf16(b.v[0], b.v[1 % V]), pack_bf16(b.v[2 % V], b.v[3 % V]));
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + to + d) = x;
+        return;
+    }
+    store_values<V>(base, bf16, to + d, a);
+    store_values<V>(base, bf16, to + e, b);
+}
+
+// Turns the item j of a row's head and stores it.
+template <int V> __device__ __forceinline__ void finish_item(const AppendParams& p, int row, const AppendPlace& at, int head, int d, int e, bool turns, const float* cosine,
+                                                             const float* sine, Lanes<V>& a, Lanes<V>& b) {
+    const int kv_heads = p.cache.kv_heads;
+    if (turns) turn_item<V>(p, d, cosine, sine, a, b);
+    if (head < p.heads) {
+        store_item<V>(p.query, p.query_bf16, (static_cast<int64_t>(row) * p.heads + head) * p.cache.head_dim, d, e, a, b);
+    } else if (at.page >= 0) {
+        const bool value = head >= p.heads + kv_heads;
+        store_item<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, page_row(p.cache, at.page, head - p.heads - (value ? kv_heads : 0), at.entry), d, e, a, b);
+    }
+}
+
+// An item is 2 V values of one head of one row.  grid (rows, blocks of items): a block has one or more whole rows where there are rows for every SM, since it
+// walks from the row to its page (four dependent loads); it asks for the row's values before that, and before it knows whether the row is one of a sequence.
+// Bound by this chain with few rows, by memory with many: 670 MB (18 k rows of 48 heads of 128 to bf16) at 5.8 TB/s.
 constexpr int kItemsHeld = 4;
 template <int V> __global__ void __launch_bounds__(256) rotary_append_kernel(const AppendParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
-    const int row = blockIdx.x;
-    const int dim = p.cache.head_dim, per_head = dim / (2 * V), kv_heads = p.cache.kv_heads;
-    const int items = (p.heads + 2 * kv_heads) * per_head, stride = gridDim.y * blockDim.x;
+    const int row = blockIdx.x * blockDim.y + threadIdx.y;
+    if (row >= p.rows.rows) return;
+    const int dim = p.cache.head_dim, per_head = dim / (2 * V), turning = p.heads + p.cache.kv_heads;
+    const int items = (p.heads + 2 * p.cache.kv_heads) * per_head, stride = gridDim.y * blockDim.x;
     const float* source = p.projected + row * p.stride;
-    if (row >= __ldg(p.rows.first + p.rows.sequences)) return;
-    bool placed = false, turns = false;
-    int page = -1, entry = 0;
-    const float *cosine = nullptr, *sine = nullptr;
+    const int live = __ldg(p.rows.first + p.rows.sequences);
+    AppendPlace at{};
+    bool placed = false;
     for (int first = blockIdx.y * blockDim.x + threadIdx.x; first < items; first += kItemsHeld * stride) {
         Lanes<V> a[kItemsHeld], b[kItemsHeld];
 #pragma unroll
         for (int k = 0; k < kItemsHeld; ++k) {
             const int item = first + k * stride;
             if (item >= items) break;
-            int d, e;
-            item_places<V>(p, item % per_head, d, e);
-            if (item / per_head >= p.heads + kv_heads) {   // values do not turn
-                d = item % per_head * 2 * V;
-                e = d + V;
-            }
-            a[k] = load_lanes<V>(source + item / per_head * dim + d);
-            b[k] = load_lanes<V>(source + item / per_head * dim + e);
+            const int head = divide(item, p.by_head), j = item - head * per_head;
+            int d = j * 2 * V, e = d + V;
+            if (head < turning) item_places<V>(p, j, d, e);   // values do not turn
+            a[k] = load_lanes<V>(source + head * dim + d);
+            b[k] = load_lanes<V>(source + head * dim + e);
         }
         if (!placed) {
             placed = true;
-            const RowPlace place = row_place(p.rows, row);
-            const int64_t turn = static_cast<int64_t>(place.position) + (p.offset ? __ldg(p.offset + place.sequence) : 0);
-            turns = p.rot > 0 && turn >= 0 && turn < p.positions;
-            if (place.slot >= 0 && place.slot < p.cache.sequences && place.position >= 0 && place.position < p.cache.capacity()) {
-                page = page_of(p.cache, place.slot, place.position / p.cache.page_size);
-                entry = place.position % p.cache.page_size;
-            }
-            if (turns) {
-                cosine = p.cosine + turn * (p.rot / 2);
-                sine = p.sine + turn * (p.rot / 2);
-            }
+            if (row >= live) return;
+            at = append_place(p, row);
         }
+        const int64_t table = static_cast<int64_t>(at.turn) * (p.rot / 2);
 #pragma unroll
         for (int k = 0; k < kItemsHeld; ++k) {
             const int item = first + k * stride;
             if (item >= items) break;
-            const int head = item / per_head, j = item % per_head;
-            int d, e;
-            item_places<V>(p, j, d, e);
-            if (head >= p.heads + kv_heads) {
-                d = j * 2 * V;
-                e = d + V;
-            } else if (turns && j * 2 * V < p.rot) {
-                if (!p.pairs) {
-                    const Lanes<V> c = load_lanes<V>(cosine + d), s = load_lanes<V>(sine + d);
-#pragma unroll
-                    for (int u = 0; u < V; ++u) {
-                        const float x = a[k].v[u], y = b[k].v[u];
-                        a[k].v[u] = x * c.v[u] - y * s.v[u];
-                        b[k].v[u] = y * c.v[u] + x * s.v[u];
-                    }
-                } else if constexpr (V == 4) {
-                    const Lanes<4> c = load_lanes<4>(cosine + d / 2), s = load_lanes<4>(sine + d / 2);
-                    const float x[4] = {a[k].v[0], a[k].v[2], b[k].v[0], b[k].v[2]}, y[4] = {a[k].v[1], a[k].v[3], b[k].v[1], b[k].v[3]};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        Lanes<4>& to = u < 2 ? a[k] : b[k];
-                        to.v[(u & 1) * 2] = x[u] * c.v[u] - y[u] * s.v[u];
-                        to.v[(u & 1) * 2 + 1] = y[u] * c.v[u] + x[u] * s.v[u];
-                    }
-                } else {
-                    const float c = cosine[d / 2], s = sine[d / 2], x = a[k].v[0], y = b[k].v[0];
-                    a[k].v[0] = x * c - y * s;
-                    b[k].v[0] = y * c + x * s;
-                }
-            }
-            if (head < p.heads) {
-                const int64_t at = (static_cast<int64_t>(row) * p.heads + head) * dim;
-                store_values<V>(p.query, p.query_bf16, at + d, a[k]);
-                store_values<V>(p.query, p.query_bf16, at + e, b[k]);
-            } else if (page >= 0) {
-                const bool value = head >= p.heads + kv_heads;
-                const int64_t at = page_row(p.cache, page, head - p.heads - (value ? kv_heads : 0), entry);
-                store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + d, a[k]);
-                store_values<V>(p.cache.pool[value], p.cache.dtype == B200_BF16, at + e, b[k]);
-            }
+            const int head = divide(item, p.by_head), j = item - head * per_head;
+            int d = j * 2 * V, e = d + V;
+            if (head < turning) item_places<V>(p, j, d, e);
+            finish_item<V>(p, row, at, head, d, e, at.turn >= 0 && head < turning && j * 2 * V < p.rot, p.cosine + table, p.sine + table, a[k], b[k]);
         }
     }
 }
@@ -240,10 +262,20 @@ extern "C" int b200_rotary_append(const b200_rotary_append_args* a, const b200_r
                      | reinterpret_cast<uintptr_t>(a->cache.value);
     if (a->rot_dims) bits |= reinterpret_cast<uintptr_t>(a->cosine) | reinterpret_cast<uintptr_t>(a->sine);
     const bool wide = dim % 8 == 0 && a->rot_dims % 8 == 0 && stride % 4 == 0 && bits % 16 == 0;
+    p.by_head = divider(dim / (wide ? 8 : 2));
     const int64_t items = width / (wide ? 8 : 2);
-    const int64_t blocks = p.rows.rows >= 148 ? 1 : (items + 255) / 256;
-    const dim3 grid(static_cast<unsigned>(p.rows.rows), static_cast<unsigned>(blocks < 65535 ? blocks : 65535));
-    return cuda_status(wide ? launch_dependent(rotary_append_kernel<4>, grid, dim3(256), 0, as_stream(stream), p)
-                            : launch_dependent(rotary_append_kernel<1>, grid, dim3(256), 0, as_stream(stream), p),
+    // Many rows: four items per thread and no thread without, so that as many rows as there is room for have their values on the way.  18 k rows of 48 heads
+    // of 128 (of 64, 10 heads of 128): 116 us (62, 30), with 256 threads whatever the row's length 121 (82, 46).  Short rows share blocks of up to 128 threads:
+    // with rows of 3 heads of 64 10 us, with a block each 20.
+    int64_t threads = 256, blocks = (items + 255) / 256, rows = 1;
+    if (p.rows.rows >= 148) {
+        threads = std::clamp<int64_t>((items + 32 * kItemsHeld - 1) / (32 * kItemsHeld) * 32, 32, 256);
+        if (p.rows.rows >= 8 * 148) rows = std::max<int64_t>(1, 128 / threads);
+        blocks = 1;
+    }
+    const dim3 grid(static_cast<unsigned>((p.rows.rows + rows - 1) / rows), static_cast<unsigned>(blocks < 65535 ? blocks : 65535));
+    const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(rows));
+    return cuda_status(wide ? launch_dependent(rotary_append_kernel<4>, grid, block, 0, as_stream(stream), p)
+                            : launch_dependent(rotary_append_kernel<1>, grid, block, 0, as_stream(stream), p),
                        "rotary_append_kernel launch");
 }

@@ -656,7 +656,7 @@ B200_API int b200_rotary_tables(const b200_rotary_scaling* scaling, int32_t rot_
  * row's angle, keys and values are appended to the sequence's slot of the cache at positions lengths[slot] + r - first[s] (lengths do not move
  * on: b200_rows_advance), queries are written out.  The angle is that of the position plus offset[s]: the length of the prefix that the slot's
  * tokens stand behind.  Rows whose angle lies past the tables do not turn (as with b200_chunk_prepare); rows past the slot's pages are not
- * appended. */
+ * appended; rows of a slot outside the cache neither turn nor are appended. */
 typedef struct b200_rotary_append_args {
     int32_t heads;
     int32_t rot_dims;              /* even, 0 .. head_dim */
