@@ -611,7 +611,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     const int groups = a.groups < pass.sequences ? a.groups : pass.sequences;
     const bool prefix = a.groups > 0 && max_prefix > 0;
     plan.form = mma ? Form::mma : Form::plain;
-    plan.tensor = mma && prefix && pairs > 32 * static_cast<int64_t>(groups) && prefix_tensor_takes(a.prefix, a.scale);
+    plan.tensor = mma && prefix && pairs > 32 * static_cast<int64_t>(groups) && a.scale != 0.0f;
     // tiles of 16, 32 or 64 pairs: the smallest that holds the most that a sequence (or, with the prefix's items among them, a group) has
     const int64_t own_pairs = static_cast<int64_t>(pass.max_count) * group;
     const int64_t most_pairs = prefix && !plan.tensor ? std::max(own_pairs, ceil_div64(pairs, groups)) : own_pairs;

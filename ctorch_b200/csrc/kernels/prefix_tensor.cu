@@ -19,6 +19,7 @@ namespace {
 constexpr int kTensorThreads = 352;
 constexpr float kLazy = 8.0f;
 
+// HD: the head size rounded up to 64 or 128; what is behind the head's end is zeros.
 template <int HD> struct TensorShape {
     static constexpr int blocks = HD / 64;                          // 64 values: one swizzled row of 128 bytes
     static constexpr int query_block = 128 * 128, key_block = kTensorKeys * 128;
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
 
     if (warp == 8) {
         const int outside = static_cast<int>(p.prefix.pages) * p.prefix.kv_heads * p.prefix.page_size;   // a row past the pools: zeros
-        const int across = boxes_per_row(box_rows, HD), boxes = kTensorKeys / box_rows * across;   // at most 16
+        const int across = boxes_per_row(box_rows, p.dim), boxes = kTensorKeys / box_rows * across;   // at most 16
         const int block = lane % across, row = lane / across * box_rows;
         PageStream pages(p.prefix, it.slot, it.keys.begin + row, kTensorKeys, lane < boxes ? it.keys.end : 0);
         int issued = 0, key_row = outside, value_row = outside;
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             for (int u = 0; u < kPieces; ++u) {
                 const int m = m_tile + row / kPieces + u * (128 / kPieces);
                 x[u] = make_uint4(0, 0, 0, 0);
-                if (m < it.m_count) x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query) + pair_row(p, it, m) * HD + 8 * c));
+                if (m < it.m_count && 8 * c < p.dim) x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.query) + pair_row(p, it, m) * p.dim + 8 * c));
             }
 #pragma unroll
             for (int u = 0; u < kPieces; ++u) {
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
                 for (int i = 0; i < kPieces; ++i) {
                     const int r = i * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
                     const int64_t at = __shfl_sync(0xffffffffu, to, r);
-                    if (at >= 0) *reinterpret_cast<uint4*>(p.part_o + at * HD + first + 4 * c) = *reinterpret_cast<const uint4*>(rows + r * kPieces * 16 + ((c ^ (r & 7)) << 4));
+                    if (at >= 0 && first + 4 * c < p.dim) *reinterpret_cast<uint4*>(p.part_o + at * p.dim + first + 4 * c) = *reinterpret_cast<const uint4*>(rows + r * kPieces * 16 + ((c ^ (r & 7)) << 4));
                 }
                 __syncwarp();
             }
@@ -385,12 +386,8 @@ int page_maps(const PagesView& pages, int box_rows, CUtensorMap* maps) {
     return B200_OK;
 }
 
-bool prefix_tensor_takes(const b200_kv_pages& prefix, float scale) {
-    return (prefix.head_dim == 64 || prefix.head_dim == 128) && scale != 0.0f;
-}
-
 int launch_prefix_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
-    return p.dim == 128 ? launch_tensor<128>(p, items, stream) : launch_tensor<64>(p, items, stream);
+    return p.dim > 64 ? launch_tensor<128>(p, items, stream) : launch_tensor<64>(p, items, stream);
 }
 
 }  // namespace b200
