@@ -1,6 +1,7 @@
 // Work items of the attention over a shared prefix and own tokens: what its kernels share.
 #pragma once
 
+#include "mma.cuh"
 #include "paged.cuh"
 #include "rows.cuh"
 
@@ -22,6 +23,8 @@ struct PrefixParams {
     int prefix_rows, own_rows; // pairs of a row tile
     int items;                 // of this launch
     int beside;                // 1: the prefix's items are another kernel's, launched just before, beside which this one runs
+    int joined;                // 1: the own tokens' items go over the keys of their sequence's prefix first and leave results, not partial ones
+    int wide_out;              // results on 16-byte boundaries
     int32_t* status;
     float* part_o;             // [rows * heads][splits][dim]
     float* part_ml;            // [rows * heads][splits][2]
@@ -62,6 +65,7 @@ struct Item {
     int kv_head, slot, split;    // split: which partial result
     int visible;                 // keys that pair 0 sees (causal: pair m sees m / group more)
     KeySpan keys;
+    int shared_slot, shared;     // joined: the prefix and its keys, which are seen before `keys`
 };
 
 // Items are numbered split-major inside a kind; the prefix's, which are longer, come first.
@@ -111,6 +115,18 @@ __device__ __forceinline__ Item find_prefix_item(const PrefixParams& p, int inde
     return it;
 }
 
+// The group of sequence s, -1 for none: groups own consecutive sequences.
+__device__ __forceinline__ int group_of(const PrefixParams& p, int s) {
+    if (p.groups == 0 || s < __ldg(p.group_first)) return -1;
+    int low = 0, high = p.groups;   // group_first[low] <= s, and s < group_first[high] unless high is the end
+    while (high - low > 1) {
+        const int middle = (low + high) / 2;
+        if (__ldg(p.group_first + middle) <= s) low = middle;
+        else high = middle;
+    }
+    return s < __ldg(p.group_first + low + 1) ? low : -1;
+}
+
 // Item `index` of the own tokens, by any one thread.
 __device__ __forceinline__ Item find_own_item(const PrefixParams& p, int index) {
     Item it{};
@@ -134,6 +150,15 @@ __device__ __forceinline__ Item find_own_item(const PrefixParams& p, int index) 
     // no further than the tile's last pair sees
     it.keys.end = min(it.keys.end, it.visible + divide(max(0, min(it.m_begin + p.own_rows, it.m_count) - 1), p.by_group));
     it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
+    if (p.joined) {
+        it.keys.end = max(0, it.keys.end);
+        it.live = it.m_begin < it.m_count;
+        const int g = group_of(p, s);
+        if (g >= 0) {
+            it.shared_slot = __ldg(p.group_prefix + g);
+            it.shared = prefix_keys(p, it.shared_slot);
+        }
+    }
     return it;
 }
 __device__ __forceinline__ Item find_item(const PrefixParams& p, int index) {
@@ -152,6 +177,8 @@ __device__ __forceinline__ Item item_of_lane(const Item& it, int lane) {
     r.visible = __shfl_sync(0xffffffffu, it.visible, lane);
     r.keys.begin = __shfl_sync(0xffffffffu, it.keys.begin, lane);
     r.keys.end = __shfl_sync(0xffffffffu, it.keys.end, lane);
+    r.shared_slot = __shfl_sync(0xffffffffu, it.shared_slot, lane);
+    r.shared = __shfl_sync(0xffffffffu, it.shared, lane);
     return r;
 }
 
@@ -169,6 +196,36 @@ __device__ __forceinline__ int first_item(const PrefixParams& p) { return p.besi
 // Pair m of an item among the pass's rows * heads, and where it leaves its partial result, a row of [rows * heads][splits].
 __device__ __forceinline__ int64_t pair_row(const PrefixParams& p, const Item& it, int m) {
     return static_cast<int64_t>(it.row) * p.heads + it.kv_head * p.group + static_cast<int64_t>(divide(m, p.by_group)) * (p.heads - p.group) + m;
+}
+// Where the results of a pair begin.
+__device__ __forceinline__ int64_t result_at(const PrefixParams& p, const Item& it, int m) {
+    const int of_row = divide(m, p.by_group);
+    return (it.row + of_row) * p.out_stride + static_cast<int64_t>(it.kv_head * p.group + m - of_row * p.group) * p.dim;
+}
+// N adjacent results, 2 or 4, at a multiple of N values behind a pair's begin.
+template <int N> __device__ __forceinline__ void store_results(const PrefixParams& p, int64_t at, const float (&v)[N]) {
+    if (!p.wide_out) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) store_forms(v[u], at + u, p.out, p.out_hi, p.out_lo);
+        return;
+    }
+    if (p.out) {
+        if constexpr (N == 4) *reinterpret_cast<float4*>(p.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<float2*>(p.out + at) = make_float2(v[0], v[1]);
+    }
+    if (p.out_hi) {
+        uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+        for (int u = 0; u < N / 2; ++u) pack_planes(v[2 * u], v[2 * u + 1], hi[u], lo[u]);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __nv_bfloat16* to = which ? p.out_lo : p.out_hi;
+            const uint32_t(&x)[N / 2] = which ? lo : hi;
+            if (!to) continue;
+            if constexpr (N == 4) *reinterpret_cast<uint2*>(to + at) = make_uint2(x[0], x[1]);
+            else *reinterpret_cast<uint32_t*>(to + at) = x[0];
+        }
+    }
 }
 __device__ __forceinline__ int64_t partial_row(const PrefixParams& p, const Item& it, int m) {
     return pair_row(p, it, m) * (p.prefix_splits + p.own_splits) + it.split;

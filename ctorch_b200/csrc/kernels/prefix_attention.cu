@@ -295,22 +295,28 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
             }
             ++found;
             if (!any || !__all_sync(0xffffffffu, *alive != 0)) break;
-            const PagesView& view = it.causal ? p.own : p.prefix;
-            const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
-            const CUtensorMap* map = it.causal ? &maps.own[which & 1] : &maps.prefix[which & 1];
-            const int end = issued + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
-            PageStream pages(view, it.slot, it.keys.begin + row, kUnit, which < 2 ? it.keys.end : 0);
-            for (; issued < end; ++issued) {
-                const int stage = issued % kStages, y = pages.next(it.kv_head, outside);
-                wait(&empty[stage], ((issued / kStages) & 1) ^ 1);
-                if (!__all_sync(0xffffffffu, *alive != 0)) break;
-                if (lane == 0) mbar_expect_tx(&full[stage], 2 * S::tile_bytes);
-                __syncwarp();
-                unsigned char* to = ring + (stage * 2 + which) * S::tile_bytes;
-                if (which < 2) {
-                    if (across < S::blocks) tma_load_3d(to, map, 0, y, 0, &full[stage]);
-                    else tma_load_2d(to + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
+            // the prefix of a joined item, then the item's own span
+            const int shared_steps = (it.shared + kUnit - 1) / kUnit, end = issued + shared_steps + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+            for (int span = shared_steps ? 0 : 1; span < 2; ++span) {
+                const PagesView& view = span && it.causal ? p.own : p.prefix;
+                const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
+                const CUtensorMap* map = span && it.causal ? &maps.own[which & 1] : &maps.prefix[which & 1];
+                const int until = span ? end : issued + shared_steps, last_key = span ? it.keys.end : it.shared;
+                if (issued >= until) break;
+                PageStream pages(view, span ? it.slot : it.shared_slot, (span ? it.keys.begin : 0) + row, kUnit, which < 2 ? last_key : 0);
+                for (; issued < until; ++issued) {
+                    const int stage = issued % kStages, y = pages.next(it.kv_head, outside);
+                    wait(&empty[stage], ((issued / kStages) & 1) ^ 1);
+                    if (!__all_sync(0xffffffffu, *alive != 0)) break;
+                    if (lane == 0) mbar_expect_tx(&full[stage], 2 * S::tile_bytes);
+                    __syncwarp();
+                    unsigned char* to = ring + (stage * 2 + which) * S::tile_bytes;
+                    if (which < 2) {
+                        if (across < S::blocks) tma_load_3d(to, map, 0, y, 0, &full[stage]);
+                        else tma_load_2d(to + block * S::block_bytes + row * 128, map, block * 64, y, &full[stage]);
+                    }
                 }
+                if (issued < until) break;
             }
             if (issued < end) break;
         }
@@ -325,7 +331,7 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_empty[number & 1]);
         if (mma_any(!*alive) || it.m_count < 0) return end_items(p);
-        const int steps = (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+        const int shared_steps = (it.shared + kUnit - 1) / kUnit, steps = shared_steps + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
         // query fragments
         const int quad = lane & 3, row_group = warp % kRowGroups, m0 = it.m_begin + row_group * 16 + (lane >> 2);
         uint32_t q[kSteps][4];
@@ -341,20 +347,22 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
                     q[k][2 * h + r] = m < it.m_count && d < p.dim ? __ldg(reinterpret_cast<const uint32_t*>(row + d)) : 0u;
                 }
         }
-        int seen[2];
+        int own_seen[2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) seen[r] = it.causal ? min(it.keys.end, it.visible + divide(m0 + 8 * r, p.by_group)) : it.keys.end;
+        for (int r = 0; r < 2; ++r) own_seen[r] = it.causal ? min(it.keys.end, it.visible + divide(m0 + 8 * r, p.by_group)) : it.keys.end;
         float acc[kColumns][4] = {}, most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
         const int warp_key = warp / kRowGroups * kKeys;
         const int first_limit = it.causal ? it.visible + divide(it.m_begin, p.by_group) : it.keys.end;   // keys that the tile's first pair sees
         for (int step = 0; step < steps; ++step) {
-            const int stage = (taken + step) % kStages, begin = it.keys.begin + step * kUnit;
+            const bool shared = step < shared_steps;   // everyone sees these
+            const int stage = (taken + step) % kStages, begin = shared ? step * kUnit : it.keys.begin + (step - shared_steps) * kUnit, end = shared ? it.shared : it.keys.end;
+            const int seen[2] = {shared ? end : own_seen[0], shared ? end : own_seen[1]};
             wait(&full[stage], ((taken + step) / kStages) & 1);
             unsigned char* values = ring + (stage * 2 + 1) * S::tile_bytes;
             const uint32_t key = smem_u32(ring) + stage * 2 * S::tile_bytes, value = key + S::tile_bytes;
-            if (begin + kUnit > it.keys.end && it.keys.end % box_rows) {
+            if (begin + kUnit > end && end % box_rows) {
                 // rows of the last box behind the keys may hold anything
-                const int from = it.keys.end - begin, behind = (from + box_rows - 1) / box_rows * box_rows - from;
+                const int from = end - begin, behind = (from + box_rows - 1) / box_rows * box_rows - from;
                 for (int i = thread; i < behind * 8 * S::blocks; i += kMmaWarps * 32)
                     *reinterpret_cast<uint4*>(values + i / (behind * 8) * S::block_bytes + from * 128 + i % (behind * 8) * 16) = make_uint4(0, 0, 0, 0);
                 own_writes_done();
@@ -402,7 +410,7 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
                     acc[n][2 * r + 1] *= shrink;
                 }
             }
-            if (min(it.keys.end, begin + kUnit) > first_limit) guard_values<HD>(values, p.dim / 8, begin, warp_key, kKeys, seen, acc);
+            if (!shared && min(end, begin + kUnit) > first_limit) guard_values<HD>(values, p.dim / 8, begin, warp_key, kKeys, seen, acc);
 #pragma unroll
             for (int k = 0; k < kKeys / 16; ++k) {
                 const uint32_t a[4] = {pack_bf16(score[2 * k][0], score[2 * k][1]), pack_bf16(score[2 * k][2], score[2 * k][3]),
@@ -453,6 +461,11 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
                     total += f * joined[(w * kRows + m) * 2 + 1];
                     o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
                 }
+                if (p.joined) {
+                    const float inverse = total == 0.0f ? 0.0f : 1.0f / total, v[4] = {o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse};
+                    if (d < p.dim) store_results<4>(p, result_at(p, it, it.m_begin + m) + d, v);
+                    continue;
+                }
                 const int64_t to = partial_row(p, it, it.m_begin + m);
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(top, total);
                 if (d < p.dim) *reinterpret_cast<float4*>(p.part_o + to * p.dim + d) = o;
@@ -463,6 +476,16 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
             for (int r = 0; r < 2; ++r) {
                 const int m = m0 + 8 * r;
                 if (m >= it.m_count) continue;
+                if (p.joined) {
+                    const float inverse = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+                    const int64_t to = result_at(p, it, m);
+#pragma unroll
+                    for (int n = 0; n < kColumns; ++n) {
+                        const float v[2] = {acc[n][2 * r] * inverse, acc[n][2 * r + 1] * inverse};
+                        if (8 * n < p.dim) store_results<2>(p, to + 8 * n + 2 * quad, v);
+                    }
+                    continue;
+                }
                 const int64_t to = partial_row(p, it, m);
                 if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most[r], sum[r]);
 #pragma unroll
@@ -562,6 +585,7 @@ struct Plan {
     Form form;
     bool aligned;              // 16-byte addresses, head sizes of 4 n
     bool tensor;               // the prefix's items are the tcgen05 kernel's
+    bool joined;               // one item per tile of own rows goes over prefix and own tokens: no partial results
     int prefix_rows, own_rows, prefix_tiles, own_tiles, prefix_splits, own_splits;
     int own_ctas;              // beside the tcgen05 kernel, 0: as many as there are items for
 };
@@ -574,28 +598,25 @@ int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// us that a step of prefix_mma_kernel takes an SM, measured, and a CTA that has an SM to itself.
+double step_time(int rows, int dim) { return rows == 16 ? (dim > 64 ? 0.6 : 0.4) : rows == 32 ? (dim > 64 ? 1.0 : 0.65) : dim > 64 ? 1.7 : 0.9; }
+
 // How the tcgen05 kernel and the own tokens' kernel share the SMs.  A CTA of the first has an SM to itself; the other's CTAs run on the SMs that its last wave
 // leaves: few splits of the prefix leave more of them and fewer partial results, many shorten the prefix's own time.  Measured, in us: a CTA of the prefix takes
-// 10 and 0.75 (heads of 64: 0.6) per step; a step of own keys takes an SM 0.6, 1.0, 1.7 (0.4, 0.65, 0.9) with tiles of 16, 32 and 64 pairs; partial results go
-// out and back at 5 MB per us.
-struct Share { int splits, own_ctas; };   // own_ctas: 0: as many as there are items for
+// 10 and 0.75 (heads of 64: 0.6) per step; partial results go out and back at 5 MB per us.
+struct Share { int splits, own_ctas; double time; };   // own_ctas: 0: as many as there are items for
 Share share_sms(int64_t items, int max_prefix, int dim, int own_rows, double own_steps, double part_bytes, int sms) {
     const int steps = ceil_div(max_prefix, kTensorKeys);
     const double step = dim > 64 ? 0.75 : 0.6;
-    const double own_step = own_rows == 16 ? (dim > 64 ? 0.6 : 0.4) : own_rows == 32 ? (dim > 64 ? 1.0 : 0.65) : dim > 64 ? 1.7 : 0.9;
-    const double own = own_steps * own_step;
-    Share best{1, 0};
-    double least = 1e30;
+    const double own = own_steps * step_time(own_rows, dim);
+    Share best{1, 0, 1e30};
     for (int n = 1; n <= kMostSplits && n <= steps; ++n) {
         const int64_t ctas = items * n, waves = ceil_div64(ctas, sms);
         const double wave = 10.0 + step * ceil_div(steps, n);
         const double rest = static_cast<double>(waves * sms - ctas), prefix = static_cast<double>(waves) * wave;
         const double free_only = rest > 0 ? std::max(prefix, prefix - wave + own / rest) : 1e30, all = prefix + std::max(0.0, own - rest * wave) / sms;
         const double time = std::min(free_only, all) + n * part_bytes / 5e6;
-        if (time < least) {
-            least = time;
-            best = {n, free_only <= all ? static_cast<int>(2 * rest) : 0};
-        }
+        if (time < best.time) best = {n, free_only <= all ? static_cast<int>(2 * rest) : 0, time};
     }
     return best;
 }
@@ -611,7 +632,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     const int groups = a.groups < pass.sequences ? a.groups : pass.sequences;
     const bool prefix = a.groups > 0 && max_prefix > 0;
     plan.form = mma ? Form::mma : Form::plain;
-    plan.tensor = mma && prefix && pairs > 32 * static_cast<int64_t>(groups) && a.scale != 0.0f;
+    plan.tensor = mma && prefix && pairs > 32 * static_cast<int64_t>(groups);
     // tiles of 16, 32 or 64 pairs: the smallest that holds the most that a sequence (or, with the prefix's items among them, a group) has
     const int64_t own_pairs = static_cast<int64_t>(pass.max_count) * group;
     const int64_t most_pairs = prefix && !plan.tensor ? std::max(own_pairs, ceil_div64(pairs, groups)) : own_pairs;
@@ -628,17 +649,35 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     };
     const int64_t own_items = static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads;
     plan.own_splits = splits(own_items, max_length, 2 * 148);
-    if (!prefix) return plan;
+    const int prefix_steps = prefix ? ceil_div(max_prefix, kUnit) : 0, length_steps = ceil_div(max_length, kUnit);
     // tiles that the rows fill: the last tile of every group is half empty
-    const int64_t filled = std::max<int64_t>(ceil_div(pairs, plan.prefix_rows), groups) * kv_heads;
-    if (!plan.tensor) {
-        plan.prefix_splits = splits(filled, max_prefix, 2 * 148);
-        return plan;
+    const int64_t filled = prefix ? std::max<int64_t>(ceil_div(pairs, plan.prefix_rows), groups) * kv_heads : 0;
+    const int64_t own_filled = plan.own_tiles == 1 ? own_items : (ceil_div64(pairs, plan.own_rows) + pass.sequences / 2) * kv_heads;
+    double time;   // of the split work, its launches and merge, in us
+    if (plan.tensor) {
+        const Share share = share_sms(filled, max_prefix, a.cache.head_dim, plan.own_rows, static_cast<double>(own_filled) * length_steps,
+                                      static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8, 148);
+        plan.prefix_splits = share.splits;
+        plan.own_ctas = share.own_ctas;
+        time = 5.0 + share.time;
+    } else {
+        if (prefix) plan.prefix_splits = splits(filled, max_prefix, 2 * 148);
+        const double longest = std::max(prefix ? ceil_div(prefix_steps, plan.prefix_splits) : 0, ceil_div(length_steps, plan.own_splits));
+        time = 10.0 + step_time(plan.own_rows, a.cache.head_dim) * std::max(longest, (static_cast<double>(filled) * prefix_steps + static_cast<double>(own_filled) * length_steps) / 148);
     }
-    const double own_steps = static_cast<double>(plan.own_tiles == 1 ? pass.sequences : ceil_div64(pairs, plan.own_rows) + pass.sequences / 2) * kv_heads * ceil_div(max_length, kUnit);
-    const Share share = share_sms(filled, max_prefix, a.cache.head_dim, plan.own_rows, own_steps, static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8, 148);
-    plan.prefix_splits = share.splits;
-    plan.own_ctas = share.own_ctas;
+    if (!mma) return plan;
+    // Short prefixes, whose keys come from L2 each time: one item per tile of own rows goes over both and leaves the result.  Measured: 34 sequences of up to 5 tokens
+    // behind 221 and 329 keys 27 us joined, 29 split; 52 single tokens behind 165 8.8 and 14.9; 9 single tokens behind 5755 61 and 24.
+    const int rows = own_pairs <= 16 ? 16 : own_pairs <= 32 ? 32 : 64, tiles = ceil_div(own_pairs, rows);
+    const int64_t items = (tiles == 1 ? pass.sequences : ceil_div64(pairs, rows) + pass.sequences / 2) * kv_heads;
+    const double step = step_time(rows, a.cache.head_dim);
+    if (6.0 + step * (2.5 + (prefix_steps + length_steps) * std::max(1.0, static_cast<double>(items) / 148)) > time) return plan;
+    plan.joined = true;
+    plan.tensor = false;
+    plan.own_rows = plan.prefix_rows = rows;
+    plan.own_tiles = tiles;
+    plan.own_splits = 1;
+    plan.prefix_tiles = plan.prefix_splits = plan.own_ctas = 0;
     return plan;
 }
 
@@ -713,7 +752,8 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     }
     const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
     p.heads = a->heads; p.group = a->heads / a->cache.kv_heads; p.by_group = divider(p.group); p.dim = a->cache.head_dim;
-    p.groups = plan.prefix_splits ? a->groups : 0;
+    p.groups = plan.prefix_splits || (plan.joined && max_prefix > 0) ? a->groups : 0;
+    p.joined = plan.joined;
     p.group_first = a->group_first; p.group_prefix = a->group_prefix; p.prefix_length = a->prefix_length;
     p.query = a->query;
     p.scale = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
@@ -723,6 +763,7 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     p.part_ml = p.part_o + static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * p.dim;
     p.out = out; p.out_hi = static_cast<__nv_bfloat16*>(out_hi); p.out_lo = static_cast<__nv_bfloat16*>(out_lo);
     p.out_stride = out_stride ? out_stride : width;
+    p.wide_out = (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_hi) | reinterpret_cast<uintptr_t>(out_lo)) % 16 == 0 && p.out_stride % 8 == 0 && p.dim % 8 == 0;
     const int64_t prefix_items = static_cast<int64_t>(plan.prefix_tiles) * plan.prefix_splits * a->cache.kv_heads;
     const int64_t own_items = static_cast<int64_t>(pass->sequences) * plan.own_tiles * plan.own_splits * a->cache.kv_heads;
     const int64_t merges = (pass->rows * a->heads + kMergeWarps - 1) / kMergeWarps;
@@ -754,7 +795,7 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
                              "prefix_plain_kernel launch");
     else
         status = p.dim <= 64 ? launch_mma<64>(p, ctas, s) : p.dim <= 96 ? launch_mma<96>(p, ctas, s) : launch_mma<128>(p, ctas, s);
-    if (status != B200_OK) return status;
+    if (status != B200_OK || plan.joined) return status;
     auto merge = p.dim % 4 == 0 ? prefix_merge_kernel<4> : prefix_merge_kernel<1>;
     return cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(merges)), dim3(kMergeWarps * 32), 0, s, p), "prefix_merge_kernel launch");
 }

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_ready[t]);
         }
-        const float scale = fabsf(p.scale);
+        const float scale = fmaxf(fabsf(p.scale), 0x1p-149f);   // 0 times the -inf of hidden scores would be no number
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * HD;
         float most = -INFINITY, sum = 0.0f;   // the maximum that the weights are relative to

@@ -14,7 +14,7 @@ int page_box_rows(int page_size);
 int page_maps(const PagesView& pages, int box_rows, CUtensorMap* maps);
 __host__ __device__ inline int boxes_per_row(int box_rows, int dim) { return box_rows == 64 && dim % 64 == 0 ? 1 : (dim + 63) / 64; }
 
-// Items of the prefix alone, of pages that prefix_mma_kernel takes; p.prefix_rows is kTensorRows, the scale not 0.
+// Items of the prefix alone, of pages that prefix_mma_kernel takes; p.prefix_rows is kTensorRows.
 int launch_prefix_tensor(const PrefixParams& p, int items, cudaStream_t stream);
 
 }  // namespace b200
