@@ -16,11 +16,12 @@ namespace b200 {
 namespace {
 
 // ---- any type and head size: f32 products on the CUDA cores --------------------------------------------------------------------------------
-constexpr int kPlainRows = 32, kPlainKeys = 32, kPlainThreads = 128;
+constexpr int kPlainKeys = 32, kPlainThreads = 128;
 
 __host__ __device__ constexpr int plain_width(int dim) { return (dim + 3) / 4 * 4; }
-__host__ __device__ constexpr int plain_smem(int dim) {
-    return (kPlainRows * plain_width(dim) + 2 * kPlainKeys * (plain_width(dim) + 4) + kPlainRows * (kPlainKeys + 1)) * static_cast<int>(sizeof(float));
+// Rows four floats longer than a multiple of 32 at most: neighbouring rows begin in other banks.
+__host__ __device__ constexpr int plain_smem(int dim, int rows) {
+    return ((rows + 2 * kPlainKeys) * (plain_width(dim) + 4) + rows * (kPlainKeys + 1)) * static_cast<int>(sizeof(float));
 }
 
 template <class T> __device__ __forceinline__ float4 load_four(const T* p);
@@ -36,17 +37,18 @@ template <class T> __device__ __forceinline__ float4 load_piece(const T* row, in
                        d + 3 < dim ? load_as_f32(row, d + 3) : 0.0f);
 }
 
-// A tile of 32 pairs x 32 keys: thread (ty, tx) has the scores of rows 2 ty, 2 ty + 1 with the keys tx + 8 j, and the columns 4 tx + 32 c of their
+// A tile of 16 ROWS pairs x 32 keys: thread (ty, tx) has the scores of rows ROWS ty .. + ROWS - 1 with the keys tx + 8 j, and the columns 4 tx + 32 c of their
 // accumulators; it brings the same columns of the keys ty and ty + 16, up to 128 wide a step ahead.  Bound by the chain of a step (shared memory, f32
 // products) with few CTAs, which the splits are for.
-template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) prefix_plain_kernel(const PrefixParams p, const bool whole) {
+template <class T, int BLOCKS, int ROWS> __global__ void __launch_bounds__(kPlainThreads, BLOCKS == 2 ? 4 : BLOCKS == 4 ? 3 : 2) prefix_plain_kernel(const PrefixParams p, const bool whole) {
     extern __shared__ __align__(16) float plain_shared[];
     begin_items(p);
     const Item it = find_item(p, first_item(p) + blockIdx.x);
     if (!it.live) return end_items(p);
     const int width = plain_width(p.dim), pitch = width + 4;
     float* query = plain_shared;
-    float* key = query + kPlainRows * width;
+    constexpr int kRows = 16 * ROWS;
+    float* key = query + kRows * pitch;
     float* value = key + kPlainKeys * pitch;
     float* weight = value + kPlainKeys * pitch;
     const int thread = threadIdx.x, ty = thread / 8, tx = thread % 8;
@@ -68,15 +70,18 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
         }
     };
     if (kAhead) fetch(it.keys.begin);
-    for (int i = thread; i < kPlainRows * (width / 4); i += kPlainThreads) {
-        const int m = it.m_begin + i / (width / 4), d = i % (width / 4) * 4;
-        *reinterpret_cast<float4*>(query + 4 * i) =
+    for (int i = thread; i < kRows * (width / 4); i += kPlainThreads) {
+        const int r = i / (width / 4), m = it.m_begin + r, d = i % (width / 4) * 4;
+        *reinterpret_cast<float4*>(query + r * pitch + d) =
             m < it.m_count ? load_piece(static_cast<const T*>(p.query) + pair_row(p, it, m) * p.dim, d, p.dim, whole) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, acc[2][BLOCKS][4] = {};
-    int limit[2];
+    float most[ROWS], sum[ROWS] = {}, acc[ROWS][BLOCKS][4] = {};
+    int limit[ROWS];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) limit[r] = it.causal ? min(it.keys.end, it.visible + divide(it.m_begin + 2 * ty + r, p.by_group)) : it.keys.end;
+    for (int r = 0; r < ROWS; ++r) {
+        most[r] = -INFINITY;
+        limit[r] = it.causal ? min(it.keys.end, it.visible + divide(it.m_begin + ROWS * ty + r, p.by_group)) : it.keys.end;
+    }
     for (int begin = it.keys.begin; begin < it.keys.end; begin += kPlainKeys) {
         __syncthreads();
         if (!kAhead) fetch(begin);
@@ -90,18 +95,21 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
                 }
         if (kAhead && begin + kPlainKeys < it.keys.end) fetch(begin + kPlainKeys);
         __syncthreads();
-        float score[2][4] = {};
+        float score[ROWS][4] = {};
+#pragma unroll 4
         for (int d = 0; d < width; d += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(query + 2 * ty * width + d), b = *reinterpret_cast<const float4*>(query + (2 * ty + 1) * width + d);
+            float4 a[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) a[r] = *reinterpret_cast<const float4*>(query + (ROWS * ty + r) * pitch + d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float4 k = *reinterpret_cast<const float4*>(key + (tx + 8 * j) * pitch + d);
-                score[0][j] += a.x * k.x + a.y * k.y + a.z * k.z + a.w * k.w;
-                score[1][j] += b.x * k.x + b.y * k.y + b.z * k.z + b.w * k.w;
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) score[r][j] += a[r].x * k.x + a[r].y * k.y + a[r].z * k.z + a[r].w * k.w;
             }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < ROWS; ++r) {
             float top = most[r];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -116,7 +124,7 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
             for (int j = 0; j < 4; ++j) {
                 const float w = exp2f(score[r][j] - base);
                 here += w;
-                weight[(2 * ty + r) * (kPlainKeys + 1) + tx + 8 * j] = w;
+                weight[(ROWS * ty + r) * (kPlainKeys + 1) + tx + 8 * j] = w;
             }
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) here += __shfl_xor_sync(0xffffffffu, here, o);
@@ -127,23 +135,30 @@ template <class T, int BLOCKS> __global__ void __launch_bounds__(kPlainThreads) 
 #pragma unroll
                 for (int u = 0; u < 4; ++u) acc[r][c][u] *= shrink;
         }
-        __syncwarp();   // the weights of two rows are written and read by the same eight lanes
-        // row 2 ty sees no more than row 2 ty + 1; what a row does not see is not multiplied, since it may be no number
-        const int both = min(kPlainKeys, limit[0] - begin), one = min(kPlainKeys, limit[1] - begin);
-        for (int k = 0; k < one; ++k) {
-            const float a = weight[2 * ty * (kPlainKeys + 1) + k], b = weight[(2 * ty + 1) * (kPlainKeys + 1) + k];
+        __syncwarp();   // the weights of a row are written and read by the same eight lanes
+        // A row sees no more than the next one; what a row does not see is not multiplied, since it may be no number.
+        auto add_values = [&](int keys, auto&& sees) {
+#pragma unroll 4
+            for (int k = 0; k < keys; ++k) {
+                float w[ROWS];
 #pragma unroll
-            for (int c = 0; c < BLOCKS; ++c) {
-                if (32 * c + 4 * tx >= width) continue;
-                const float4 v = *reinterpret_cast<const float4*>(value + k * pitch + 32 * c + 4 * tx);
-                if (k < both) { acc[0][c][0] += a * v.x; acc[0][c][1] += a * v.y; acc[0][c][2] += a * v.z; acc[0][c][3] += a * v.w; }
-                acc[1][c][0] += b * v.x; acc[1][c][1] += b * v.y; acc[1][c][2] += b * v.z; acc[1][c][3] += b * v.w;
+                for (int r = 0; r < ROWS; ++r) w[r] = weight[(ROWS * ty + r) * (kPlainKeys + 1) + k];
+#pragma unroll
+                for (int c = 0; c < BLOCKS; ++c) {
+                    if (32 * c + 4 * tx >= width) continue;
+                    const float4 v = *reinterpret_cast<const float4*>(value + k * pitch + 32 * c + 4 * tx);
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r)
+                        if (sees(r, k)) { acc[r][c][0] += w[r] * v.x; acc[r][c][1] += w[r] * v.y; acc[r][c][2] += w[r] * v.z; acc[r][c][3] += w[r] * v.w; }
+                }
             }
-        }
+        };
+        if (limit[0] >= begin + kPlainKeys) add_values(kPlainKeys, [](int, int) { return true; });
+        else add_values(min(kPlainKeys, limit[ROWS - 1] - begin), [&](int r, int k) { return begin + k < limit[r]; });
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int m = it.m_begin + 2 * ty + r;
+    for (int r = 0; r < ROWS; ++r) {
+        const int m = it.m_begin + ROWS * ty + r;
         if (m >= it.m_count) continue;
         const int64_t at = partial_row(p, it, m);
         if (tx == 0) {
@@ -222,7 +237,7 @@ struct MmaMaps { CUtensorMap own[2], prefix[2]; };   // K and V
 // A tile has 64 / PARTS pairs, 16 per warp: PARTS warps share the 64 keys of a step, and their results are joined at the end.  Tiles of 16 pairs (PARTS 4) for
 // single tokens, of 64 where there are as many pairs, so that no warp multiplies rows that are not there.  A CTA takes item after item; the copying warp finds
 // them and runs ahead of the products, so that keys of the next item are on their way while the last one's results are written.
-template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
+template <int HD, int PARTS, bool JOINED> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
     using S = MmaShape<HD>;
     extern __shared__ unsigned char mma_shared[];
     constexpr int kStages = S::stages(PARTS);
@@ -296,7 +311,7 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
             ++found;
             if (!any || !__all_sync(0xffffffffu, *alive != 0)) break;
             // the prefix of a joined item, then the item's own span
-            const int shared_steps = (it.shared + kUnit - 1) / kUnit, end = issued + shared_steps + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+            const int shared_steps = JOINED ? (it.shared + kUnit - 1) / kUnit : 0, end = issued + shared_steps + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
             for (int span = shared_steps ? 0 : 1; span < 2; ++span) {
                 const PagesView& view = span && it.causal ? p.own : p.prefix;
                 const int outside = static_cast<int>(view.pages) * view.kv_heads * view.page_size;   // a row past the pools: zeros
@@ -331,7 +346,7 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_empty[number & 1]);
         if (mma_any(!*alive) || it.m_count < 0) return end_items(p);
-        const int shared_steps = (it.shared + kUnit - 1) / kUnit, steps = shared_steps + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
+        const int shared_steps = JOINED ? (it.shared + kUnit - 1) / kUnit : 0, steps = shared_steps + (it.keys.end - it.keys.begin + kUnit - 1) / kUnit;
         // query fragments
         const int quad = lane & 3, row_group = warp % kRowGroups, m0 = it.m_begin + row_group * 16 + (lane >> 2);
         uint32_t q[kSteps][4];
@@ -354,7 +369,7 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
         const int warp_key = warp / kRowGroups * kKeys;
         const int first_limit = it.causal ? it.visible + divide(it.m_begin, p.by_group) : it.keys.end;   // keys that the tile's first pair sees
         for (int step = 0; step < steps; ++step) {
-            const bool shared = step < shared_steps;   // everyone sees these
+            const bool shared = JOINED && step < shared_steps;   // everyone sees these
             const int stage = (taken + step) % kStages, begin = shared ? step * kUnit : it.keys.begin + (step - shared_steps) * kUnit, end = shared ? it.shared : it.keys.end;
             const int seen[2] = {shared ? end : own_seen[0], shared ? end : own_seen[1]};
             wait(&full[stage], ((taken + step) / kStages) & 1);
@@ -461,14 +476,14 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
                     total += f * joined[(w * kRows + m) * 2 + 1];
                     o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
                 }
-                if (p.joined) {
+                if constexpr (JOINED) {
                     const float inverse = total == 0.0f ? 0.0f : 1.0f / total, v[4] = {o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse};
                     if (d < p.dim) store_results<4>(p, result_at(p, it, it.m_begin + m) + d, v);
-                    continue;
+                } else {
+                    const int64_t to = partial_row(p, it, it.m_begin + m);
+                    if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(top, total);
+                    if (d < p.dim) *reinterpret_cast<float4*>(p.part_o + to * p.dim + d) = o;
                 }
-                const int64_t to = partial_row(p, it, it.m_begin + m);
-                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(top, total);
-                if (d < p.dim) *reinterpret_cast<float4*>(p.part_o + to * p.dim + d) = o;
             }
             mma_barrier();   // the next item's results may be written
         } else {
@@ -476,7 +491,7 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
             for (int r = 0; r < 2; ++r) {
                 const int m = m0 + 8 * r;
                 if (m >= it.m_count) continue;
-                if (p.joined) {
+                if constexpr (JOINED) {
                     const float inverse = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
                     const int64_t to = result_at(p, it, m);
 #pragma unroll
@@ -484,13 +499,13 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
                         const float v[2] = {acc[n][2 * r] * inverse, acc[n][2 * r + 1] * inverse};
                         if (8 * n < p.dim) store_results<2>(p, to + 8 * n + 2 * quad, v);
                     }
-                    continue;
-                }
-                const int64_t to = partial_row(p, it, m);
-                if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most[r], sum[r]);
+                } else {
+                    const int64_t to = partial_row(p, it, m);
+                    if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * to) = make_float2(most[r], sum[r]);
 #pragma unroll
-                for (int n = 0; n < kColumns; ++n)
-                    if (8 * n < p.dim) *reinterpret_cast<float2*>(p.part_o + to * p.dim + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+                    for (int n = 0; n < kColumns; ++n)
+                        if (8 * n < p.dim) *reinterpret_cast<float2*>(p.part_o + to * p.dim + 8 * n + 2 * quad) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+                }
             }
         }
         taken += steps;
@@ -500,12 +515,14 @@ template <int HD, int PARTS> __global__ void __launch_bounds__(kMmaThreads, 2) p
 // ---- merge ------------------------------------------------------------------------------------------------------------------------------
 constexpr int kMergeWarps = 4, kMostSplits = 64;
 
-// A warp per row and head.  V = 4 (head sizes of 4 n): a group of `lanes` lanes reads one partial result at 16 bytes per lane, the warp's groups take
+// A warp per row and head, or, SPREAD, a block: with many splits of few rows its warps share the partial results (57 splits of 6 rows and heads: 11 us, 24 with a warp each).
+// V = 4 (head sizes of 4 n): a group of `lanes` lanes reads one partial result at 16 bytes per lane, the warp's groups take
 // turns over the splits and are added at the end.
 // The pass's arrays were complete before the kernels that left the partial results began, so what is to be read is worked out while those still run.
-template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const PrefixParams p) {
-    const int64_t index = blockIdx.x * static_cast<int64_t>(kMergeWarps) + static_cast<int64_t>(threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+template <int V, bool SPREAD> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const PrefixParams p) {
+    __shared__ Lanes<V> shares[SPREAD ? kMergeWarps : 1][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t index = SPREAD ? blockIdx.x : blockIdx.x * static_cast<int64_t>(kMergeWarps) + warp;
     const int row = static_cast<int>(index / p.heads);
     if (row >= p.rows.rows || row >= __ldg(p.rows.first + p.rows.sequences)) {
         grid_dependency_wait();
@@ -557,21 +574,53 @@ template <int V> __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merg
         Lanes<V> o{};
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
-#pragma unroll 8
-            for (int i = 0; i < 32; i += groups) {
-                if (32 * j + i >= parts) break;
-                const int part = 32 * j + i + turn;
-                const float f = __shfl_sync(0xffffffffu, weight[j], i + turn);
-                if (part < parts && d < pieces && f != 0.0f) {
-                    const Lanes<V> v = load_lanes<V>(p.part_o + (base + part + (part < from_prefix ? 0 : skip)) * p.dim + d * V);
+            if constexpr (SPREAD) {
+                for (int begin = 0; begin < 32; begin += 4 * groups) {   // partial results that are requested together
+                    if (32 * j + begin >= parts) break;
+                    if ((32 * j + begin) / (4 * groups) % kMergeWarps != warp) continue;
+                    Lanes<V> v[4];
+                    float f[4];
 #pragma unroll
-                    for (int u = 0; u < V; ++u) o.v[u] += f * v.v[u];
+                    for (int k = 0; k < 4; ++k) {
+                        const int i = begin + k * groups + turn, part = 32 * j + i;
+                        f[k] = __shfl_sync(0xffffffffu, weight[j], i & 31);
+                        if (i >= 32 || part >= parts || d >= pieces) f[k] = 0.0f;
+                        v[k] = Lanes<V>{};
+                        if (f[k] != 0.0f) v[k] = load_lanes<V>(p.part_o + (base + part + (part < from_prefix ? 0 : skip)) * p.dim + d * V);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int u = 0; u < V; ++u) o.v[u] += f[k] * v[k].v[u];
+                }
+            } else {
+#pragma unroll 8
+                for (int i = 0; i < 32; i += groups) {
+                    if (32 * j + i >= parts) break;
+                    const int part = 32 * j + i + turn;
+                    const float f = __shfl_sync(0xffffffffu, weight[j], i + turn);
+                    if (part < parts && d < pieces && f != 0.0f) {
+                        const Lanes<V> v = load_lanes<V>(p.part_o + (base + part + (part < from_prefix ? 0 : skip)) * p.dim + d * V);
+#pragma unroll
+                        for (int u = 0; u < V; ++u) o.v[u] += f * v.v[u];
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int u = 0; u < V; ++u) {
+        for (int u = 0; u < V; ++u)
             for (int x = lanes; x < 32; x *= 2) o.v[u] += __shfl_xor_sync(0xffffffffu, o.v[u], x);
+        if constexpr (SPREAD) {
+            __syncthreads();
+            shares[warp][lane] = o;
+            __syncthreads();
+            if (warp) continue;
+            for (int w = 1; w < kMergeWarps; ++w)
+#pragma unroll
+                for (int u = 0; u < V; ++u) o.v[u] += shares[w][lane].v[u];
+        }
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
             if (turn == 0 && d < pieces) store_forms(o.v[u] * inverse, to + d * V + u, p.out, p.out_hi, p.out_lo);
         }
     }
@@ -636,7 +685,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     // tiles of 16, 32 or 64 pairs: the smallest that holds the most that a sequence (or, with the prefix's items among them, a group) has
     const int64_t own_pairs = static_cast<int64_t>(pass.max_count) * group;
     const int64_t most_pairs = prefix && !plan.tensor ? std::max(own_pairs, ceil_div64(pairs, groups)) : own_pairs;
-    plan.own_rows = !mma ? kPlainRows : most_pairs <= 16 ? 16 : most_pairs <= 32 ? 32 : 64;
+    plan.own_rows = !mma ? (most_pairs <= 16 ? 16 : 32) : most_pairs <= 16 ? 16 : most_pairs <= 32 ? 32 : 64;
     plan.prefix_rows = plan.tensor ? kTensorRows : plan.own_rows;
     plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.prefix_rows) + groups : 0;
     plan.own_tiles = ceil_div(own_pairs, plan.own_rows);
@@ -700,18 +749,21 @@ int check_prefix(const b200_prefix_args* a, const b200_rows* pass, PrefixParams&
     return B200_OK;
 }
 
-template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned items, bool whole, cudaStream_t stream) {
-    auto kernel = p.dim <= 64 ? prefix_plain_kernel<T, 2> : p.dim <= 128 ? prefix_plain_kernel<T, 4> : prefix_plain_kernel<T, 8>;
-    const int smem = plain_smem(p.dim);
+template <class T, int ROWS> cudaError_t launch_plain(const PrefixParams& p, unsigned items, bool whole, cudaStream_t stream) {
+    auto kernel = p.dim <= 64 ? prefix_plain_kernel<T, 2, ROWS> : p.dim <= 128 ? prefix_plain_kernel<T, 4, ROWS> : prefix_plain_kernel<T, 8, ROWS>;
+    const int smem = plain_smem(p.dim, 16 * ROWS);
     if (smem > 48 * 1024) {
         const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (status != cudaSuccess) return status;
     }
     return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p, whole);
 }
+template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned items, bool whole, cudaStream_t stream) {
+    return p.own_rows == 16 ? launch_plain<T, 1>(p, items, whole, stream) : launch_plain<T, 2>(p, items, whole, stream);
+}
 
-template <int HD> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
-    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, 4> : p.own_rows == 32 ? prefix_mma_kernel<HD, 2> : prefix_mma_kernel<HD, 1>;
+template <int HD, bool JOINED> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
+    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, 4, JOINED> : p.own_rows == 32 ? prefix_mma_kernel<HD, 2, JOINED> : prefix_mma_kernel<HD, 1, JOINED>;
     const int smem = MmaShape<HD>::smem_bytes(p.own_rows == 16 ? 4 : p.own_rows == 32 ? 2 : 1);
     MmaMaps maps;
     int box_rows = page_box_rows(p.own.page_size);
@@ -723,6 +775,10 @@ template <int HD> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t s
     return cuda_status(launch_dependent(kernel, dim3(static_cast<unsigned>(std::min(p.items, ctas))), dim3(kMmaThreads), static_cast<size_t>(smem), stream, maps, p, box_rows), "prefix_mma_kernel launch");
 }
 
+template <int HD> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
+    return p.joined ? launch_mma<HD, true>(p, ctas, stream) : launch_mma<HD, false>(p, ctas, stream);
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -732,7 +788,8 @@ extern "C" size_t b200_prefix_scratch_bytes(const b200_prefix_args* a, const b20
     PrefixParams p{};
     if (check_prefix(a, pass, p) != B200_OK || max_length <= 0 || max_prefix < 0) return 0;
     const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
-    return static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * (a->cache.head_dim + 2) * sizeof(float) + 256;
+    const size_t partials = plan.joined ? 0 : static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits);
+    return partials * (a->cache.head_dim + 2) * sizeof(float) + 256;
 }
 
 extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch, size_t scratch_bytes,
@@ -796,6 +853,8 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     else
         status = p.dim <= 64 ? launch_mma<64>(p, ctas, s) : p.dim <= 96 ? launch_mma<96>(p, ctas, s) : launch_mma<128>(p, ctas, s);
     if (status != B200_OK || plan.joined) return status;
-    auto merge = p.dim % 4 == 0 ? prefix_merge_kernel<4> : prefix_merge_kernel<1>;
-    return cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(merges)), dim3(kMergeWarps * 32), 0, s, p), "prefix_merge_kernel launch");
+    const bool spread = plan.prefix_splits + plan.own_splits > 8 && pass->rows * static_cast<int64_t>(a->heads) <= 8 * 148;
+    auto merge = spread ? (p.dim % 4 == 0 ? prefix_merge_kernel<4, true> : prefix_merge_kernel<1, true>)
+                        : (p.dim % 4 == 0 ? prefix_merge_kernel<4, false> : prefix_merge_kernel<1, false>);
+    return cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(spread ? pass->rows * a->heads : merges)), dim3(kMergeWarps * 32), 0, s, p), "prefix_merge_kernel launch");
 }
