@@ -788,8 +788,7 @@ extern "C" size_t b200_prefix_scratch_bytes(const b200_prefix_args* a, const b20
     PrefixParams p{};
     if (check_prefix(a, pass, p) != B200_OK || max_length <= 0 || max_prefix < 0) return 0;
     const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
-    const size_t partials = plan.joined ? 0 : static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits);
-    return partials * (a->cache.head_dim + 2) * sizeof(float) + 256;
+    return static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * (a->cache.head_dim + 2) * sizeof(float) + 256;
 }
 
 extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch, size_t scratch_bytes,
