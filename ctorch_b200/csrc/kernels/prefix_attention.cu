@@ -5,6 +5,7 @@
 // of that sequence.  Items are (prefix tile or sequence tile, KV head, split of the keys); each leaves an unnormalised partial result (maximum,
 // sum, accumulator) per row and head, and the merge kernel joins them under one softmax:
 //   m = max m_i,  out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i      (scores in units of log2 e).
+// Where the prefixes are short, an item is joined: the rows of a sequence tile with the prefix's keys and then the sequence's own, and it leaves the result.
 #include "mma.cuh"
 #include "prefix.cuh"
 #include "prefix_tensor.cuh"
