@@ -676,7 +676,7 @@ B200_API int b200_rotary_append(const b200_rotary_append_args* args, const b200_
 /* Grouped-query attention of a pass over a prefix that the sequences of a group share and over each sequence's own tokens: row r of
  * sequence s in group g sees the first prefix_length[group_prefix[g]] positions of that prefix and, in slot[s] of the cache, the positions 0 ..
  * lengths[slot[s]] + r - first[s], which the cache must already hold.  One softmax(scale q.k) over both.  A prefix's keys and values are read
- * once for all rows of a group.  Group g owns the sequences group_first[g] .. group_first[g + 1] - 1 of the pass; a sequence in no group has no
+ * once for all rows of a group (short ones once per sequence, from L2, where that takes less time).  Group g owns the sequences group_first[g] .. group_first[g + 1] - 1 of the pass; a sequence in no group has no
  * prefix, a prefix or slot number outside its table no positions; a row that sees nothing gives zeros.  Prefix and cache may be tables over the
  * same pools. */
 typedef struct b200_prefix_args {
