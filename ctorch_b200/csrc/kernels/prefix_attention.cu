@@ -731,6 +731,12 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     return plan;
 }
 
+// Floats of the partial accumulators: the maxima and sums behind them are read eight bytes at a time, and rows * heads * splits * head_dim may be odd.
+size_t part_floats(const b200_prefix_args& a, const b200_rows& pass, const Plan& plan) {
+    const size_t floats = static_cast<size_t>(pass.rows) * a.heads * (plan.prefix_splits + plan.own_splits) * a.cache.head_dim;
+    return (floats + 3) / 4 * 4;
+}
+
 bool same_heads(const b200_kv_pages& a, const b200_kv_pages& b) { return a.dtype == b.dtype && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim; }
 
 int check_prefix(const b200_prefix_args* a, const b200_rows* pass, PrefixParams& p) {
@@ -789,7 +795,7 @@ extern "C" size_t b200_prefix_scratch_bytes(const b200_prefix_args* a, const b20
     PrefixParams p{};
     if (check_prefix(a, pass, p) != B200_OK || max_length <= 0 || max_prefix < 0) return 0;
     const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
-    return static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * (a->cache.head_dim + 2) * sizeof(float) + 256;
+    return (part_floats(*a, *pass, plan) + static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * 2) * sizeof(float) + 256;
 }
 
 extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch, size_t scratch_bytes,
@@ -817,7 +823,7 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits; p.prefix_tiles = plan.prefix_tiles; p.own_tiles = plan.own_tiles;
     p.prefix_rows = plan.prefix_rows; p.own_rows = plan.own_rows;
     p.part_o = static_cast<float*>(scratch);
-    p.part_ml = p.part_o + static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * p.dim;
+    p.part_ml = p.part_o + part_floats(*a, *pass, plan);
     p.out = out; p.out_hi = static_cast<__nv_bfloat16*>(out_hi); p.out_lo = static_cast<__nv_bfloat16*>(out_lo);
     p.out_stride = out_stride ? out_stride : width;
     p.wide_out = (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_hi) | reinterpret_cast<uintptr_t>(out_lo)) % 16 == 0 && p.out_stride % 8 == 0 && p.dim % 8 == 0;
