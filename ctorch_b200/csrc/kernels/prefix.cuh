@@ -24,6 +24,7 @@ struct PrefixParams {
     int items;                 // of this launch
     int beside;                // 1: the prefix's items are another kernel's, launched just before, beside which this one runs
     int joined;                // 1: the own tokens' items go over the keys of their sequence's prefix first and leave results, not partial ones
+    int planes;                // 1: weights as two bf16 planes
     int wide_out;              // results on 16-byte boundaries
     int32_t* status;
     float* part_o;             // [rows * heads][splits][dim]
@@ -46,6 +47,19 @@ __device__ __forceinline__ int used_splits(int total, int splits, int seen) {
     if (steps == 0 || seen <= 0) return 0;
     const int per = (steps + splits - 1) / splits * kUnit;
     return (min(seen, total) + per - 1) / per;
+}
+
+// The weights of the softmax as the tensor cores take them.  What they are relative to, a running maximum, hangs on the split, the tile and the form, and these on
+// the batch, so it is a whole number of powers of two (whole_maximum): another one shifts a weight's exponent and leaves its rounding alone.  (Rounded relative to
+// the maximum itself, f32 results of peaked rows moved by up to 9e-3 from batch to batch, and a third of all bf16 results by a step.)
+//   PLANES, for results in f32 or two planes: two bf16 planes, 15 bits.  The first is cut off, not rounded, and the second larger by 2^-23 of the weight, so that
+//   both are positive where the weight is and an infinite value stays one.
+//   Otherwise, for bf16 results, one plane of 8 bits, and the sum is that of the rounded weights: rounding the largest ones cancels.  Half the products.
+__device__ __forceinline__ float whole_maximum(float top) { return top == -INFINITY ? 0.0f : ceilf(top); }
+__device__ __forceinline__ uint32_t first_plane(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+__device__ __forceinline__ uint32_t second_plane(float a, float b) {
+    const float high_a = __uint_as_float(__float_as_uint(a) & 0xffff0000u), high_b = __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    return pack_bf16(fmaf(a, 0x1.000002p0f, -high_a), fmaf(b, 0x1.000002p0f, -high_b));
 }
 
 // Keys of the prefix in a slot of its table.

@@ -238,7 +238,7 @@ struct MmaMaps { CUtensorMap own[2], prefix[2]; };   // K and V
 // A tile has 64 / PARTS pairs, 16 per warp: PARTS warps share the 64 keys of a step, and their results are joined at the end.  Tiles of 16 pairs (PARTS 4) for
 // single tokens, of 64 where there are as many pairs, so that no warp multiplies rows that are not there.  A CTA takes item after item; the copying warp finds
 // them and runs ahead of the products, so that keys of the next item are on their way while the last one's results are written.
-template <int HD, int PARTS, bool JOINED> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
+template <int HD, int PARTS, bool JOINED, bool PLANES> __global__ void __launch_bounds__(kMmaThreads, 2) prefix_mma_kernel(const __grid_constant__ MmaMaps maps, const PrefixParams p, const int box_rows) {
     using S = MmaShape<HD>;
     extern __shared__ unsigned char mma_shared[];
     constexpr int kStages = S::stages(PARTS);
@@ -408,18 +408,22 @@ template <int HD, int PARTS, bool JOINED> __global__ void __launch_bounds__(kMma
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(most[r] - base);
+                const float base = whole_maximum(top), shrink = exp2_fast(most[r] - base);
                 float here = 0.0f;
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float& x = score[n][2 * r + u];
-                        x = exp2_fast(x - base);
-                        here += x;
+                for (int n = 0; n < kTiles; ++n) {
+                    float &a = score[n][2 * r], &b = score[n][2 * r + 1];
+                    a = exp2_fast(a - base);
+                    b = exp2_fast(b - base);
+                    if constexpr (!PLANES) {
+                        const uint32_t rounded = pack_bf16(a, b);
+                        a = bf16_lo(rounded);
+                        b = bf16_hi(rounded);
                     }
+                    here += a + b;
+                }
                 sum[r] = sum[r] * shrink + here;   // of this lane's keys; the quad's are added at the end
-                most[r] = top;
+                if (top != -INFINITY) most[r] = base;
 #pragma unroll
                 for (int n = 0; n < kColumns; ++n) {
                     acc[n][2 * r] *= shrink;
@@ -429,14 +433,22 @@ template <int HD, int PARTS, bool JOINED> __global__ void __launch_bounds__(kMma
             if (!shared && min(end, begin + kUnit) > first_limit) guard_values<HD>(values, p.dim / 8, begin, warp_key, kKeys, seen, acc);
 #pragma unroll
             for (int k = 0; k < kKeys / 16; ++k) {
-                const uint32_t a[4] = {pack_bf16(score[2 * k][0], score[2 * k][1]), pack_bf16(score[2 * k][2], score[2 * k][3]),
-                                       pack_bf16(score[2 * k + 1][0], score[2 * k + 1][1]), pack_bf16(score[2 * k + 1][2], score[2 * k + 1][3])};
+                uint32_t weights[2][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = score[2 * k + i / 2][2 * (i % 2)], b = score[2 * k + i / 2][2 * (i % 2) + 1];
+                    weights[0][i] = first_plane(a, b);
+                    if constexpr (PLANES) weights[1][i] = second_plane(a, b);
+                }
 #pragma unroll
                 for (int n = 0; n < kColumns; n += 2) {
                     uint32_t b[4];
                     ldsm_x4_trans(b, value + piece_offset(warp_key + 16 * k + (lane & 15), n + (lane >> 4)));
-                    mma_16816(acc[n], a, b[0], b[1]);
-                    mma_16816(acc[n + 1], a, b[2], b[3]);
+#pragma unroll
+                    for (int plane = 0; plane < 1 + PLANES; ++plane) {
+                        mma_16816(acc[n], weights[plane], b[0], b[1]);
+                        mma_16816(acc[n + 1], weights[plane], b[2], b[3]);
+                    }
                 }
             }
             __syncwarp();
@@ -769,8 +781,8 @@ template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned item
     return p.own_rows == 16 ? launch_plain<T, 1>(p, items, whole, stream) : launch_plain<T, 2>(p, items, whole, stream);
 }
 
-template <int HD, bool JOINED> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
-    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, 4, JOINED> : p.own_rows == 32 ? prefix_mma_kernel<HD, 2, JOINED> : prefix_mma_kernel<HD, 1, JOINED>;
+template <int HD, bool JOINED, bool PLANES> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
+    auto kernel = p.own_rows == 16 ? prefix_mma_kernel<HD, 4, JOINED, PLANES> : p.own_rows == 32 ? prefix_mma_kernel<HD, 2, JOINED, PLANES> : prefix_mma_kernel<HD, 1, JOINED, PLANES>;
     const int smem = MmaShape<HD>::smem_bytes(p.own_rows == 16 ? 4 : p.own_rows == 32 ? 2 : 1);
     MmaMaps maps;
     int box_rows = page_box_rows(p.own.page_size);
@@ -783,7 +795,8 @@ template <int HD, bool JOINED> int launch_mma(const PrefixParams& p, int ctas, c
 }
 
 template <int HD> int launch_mma(const PrefixParams& p, int ctas, cudaStream_t stream) {
-    return p.joined ? launch_mma<HD, true>(p, ctas, stream) : launch_mma<HD, false>(p, ctas, stream);
+    if (p.joined) return p.planes ? launch_mma<HD, true, true>(p, ctas, stream) : launch_mma<HD, true, false>(p, ctas, stream);
+    return p.planes ? launch_mma<HD, false, true>(p, ctas, stream) : launch_mma<HD, false, false>(p, ctas, stream);
 }
 
 }  // namespace
@@ -817,6 +830,7 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     p.heads = a->heads; p.group = a->heads / a->cache.kv_heads; p.by_group = divider(p.group); p.dim = a->cache.head_dim;
     p.groups = plan.prefix_splits || (plan.joined && max_prefix > 0) ? a->groups : 0;
     p.joined = plan.joined;
+    p.planes = out || out_lo;
     p.group_first = a->group_first; p.group_prefix = a->group_prefix; p.prefix_length = a->prefix_length;
     p.query = a->query;
     p.scale = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);

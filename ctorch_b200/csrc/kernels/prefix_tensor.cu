@@ -8,6 +8,7 @@
 //   warps 9, 10      all products of tile 0 and 1 (a product keeps its issuing warp as long as the tensor cores); warp 9 also has the tensor memory
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the maximum its weights are relative to: they
 // are relative to the same one in the sum and in O, so the quotient is the softmax all the same, and weights up to 2^8 lose nothing in f32 and bf16.
+// With PLANES the second planes of the weights take the other half of the columns of S, and O += P V has twice the products.
 #include "mma.cuh"
 #include "prefix.cuh"
 #include "prefix_tensor.cuh"
@@ -67,7 +68,7 @@ __device__ __forceinline__ void hide_scores(uint32_t (&s)[2][32], int live) {
             if (32 * c + i >= live) s[c][i] = 0xff800000u;   // -inf
 }
 
-template <int HD>
+template <int HD, bool PLANES>
 __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                                                                           const PrefixParams p, const int box_rows) {
     using S = TensorShape<HD>;
@@ -201,8 +202,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             const uint64_t value = operand_descriptor_transposed(slots + v % S::slots * S::step_bytes, S::key_block), key = key_of(k);
             if (going && elect_one()) {
 #pragma unroll
-                for (int i = 0; i < kTensorKeys / 16; ++i)
-                    tc_mma_bf16_tmem(o_at, s_at + buffer * 64 + 8 * i, value + i * 128, S::sums, (step | i) != 0);
+                for (int i = 0; i < (1 + PLANES) * (kTensorKeys / 16); ++i)   // the weights' first planes, then the second ones
+                    tc_mma_bf16_tmem(o_at, s_at + buffer * 64 + 8 * i, value + i % (kTensorKeys / 16) * 128, S::sums, (step | i) != 0);
                 tc_commit(&o_done[2 * t + buffer]);
                 tc_commit(&empty[v % S::slots]);
                 if (more) scores(buffer, k, key);
@@ -263,8 +264,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
             const bool grows = here > most + kLazy;
             if (__any_sync(0xffffffffu, grows)) {
-                const float factor = grows ? exp2_fast(most - here) : 1.0f;
-                if (grows) most = here;
+                const float base = whole_maximum(here), factor = grows ? exp2_fast(most - base) : 1.0f;
+                if (grows) most = base;
                 sum *= factor;
                 if (step > 0) {
                     going = wait(&o_done[2 * t + ((step - 1) & 1)], ((step - 1) >> 1) & 1);
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
             // fourth pair is computed on the FMA units instead.
             const Two scales = two(scale, scale), bases = two(base, base);
             Two add[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)}, odd = two(0.0f, 0.0f);
-            uint32_t weights[32];
+            uint32_t weights[32], second[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
                 Two x = fma_two(two(__uint_as_float(s[i / 16][2 * (i % 16)]), __uint_as_float(s[i / 16][2 * (i % 16) + 1])), scales, bases);
@@ -297,12 +298,19 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
                     split(x, a, b);
                     a = exp2_fast(a);
                     b = exp2_fast(b);
-                    x = two(a, b);
                 }
-                add[i & 1] = add_two(add[i & 1], x);
-                weights[i] = pack_bf16(a, b);
+                if constexpr (PLANES) {
+                    weights[i] = first_plane(a, b);
+                    second[i] = second_plane(a, b);
+                } else {
+                    weights[i] = pack_bf16(a, b);
+                    a = bf16_lo(weights[i]);
+                    b = bf16_hi(weights[i]);
+                }
+                add[i & 1] = add_two(add[i & 1], two(a, b));
             }
             tmem_store_32(s_here, weights);
+            if constexpr (PLANES) tmem_store_32(s_here + 32, second);
             {
                 float a, b;
                 split(add_two(add_two(add[0], add[1]), odd), a, b);
@@ -351,12 +359,12 @@ __global__ void __launch_bounds__(kTensorThreads, 1) prefix_tensor_kernel(const 
     }
 }
 
-template <int HD> int launch_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
+template <int HD, bool PLANES> int launch_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
     const int box_rows = page_box_rows(p.prefix.page_size);
     CUtensorMap maps[2];
     const int status = page_maps(p.prefix, box_rows, maps);
     if (status != B200_OK) return status;
-    auto kernel = prefix_tensor_kernel<HD>;
+    auto kernel = prefix_tensor_kernel<HD, PLANES>;
     B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TensorShape<HD>::smem_bytes));
     return cuda_status(launch_dependent(kernel, dim3(static_cast<unsigned>(items)), dim3(kTensorThreads), TensorShape<HD>::smem_bytes, stream, maps[0], maps[1], p, box_rows),
                        "prefix_tensor_kernel launch");
@@ -387,7 +395,8 @@ int page_maps(const PagesView& pages, int box_rows, CUtensorMap* maps) {
 }
 
 int launch_prefix_tensor(const PrefixParams& p, int items, cudaStream_t stream) {
-    return p.dim > 64 ? launch_tensor<128>(p, items, stream) : launch_tensor<64>(p, items, stream);
+    if (p.planes) return p.dim > 64 ? launch_tensor<128, true>(p, items, stream) : launch_tensor<64, true>(p, items, stream);
+    return p.dim > 64 ? launch_tensor<128, false>(p, items, stream) : launch_tensor<64, false>(p, items, stream);
 }
 
 }  // namespace b200

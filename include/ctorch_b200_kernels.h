@@ -692,7 +692,9 @@ typedef struct b200_prefix_args {
 } b200_prefix_args;
 /* max_length and max_prefix: upper bounds of lengths[slot] + rows of a sequence and of a prefix's length, by which the work is split (the pages
  * of a table bound what is read).  The result [rows, heads*dim] in f32 (out) and / or as planes, out_stride elements between rows (0: heads*dim).
- * bf16 caches: products of bf16 queries, keys, weights and values with f32 sums, so a result is good to bf16. */
+ * bf16 caches: products of bf16 queries, keys and values with f32 sums.  Results in f32 or two planes take the softmax's weights with 15 bits (two bf16 planes),
+ * results in one plane with 8, rounded in product and sum alike.  The work is split by the whole pass, and the split sets the order of the f32 sums: between
+ * batches a sequence's f32 results differ by what f32 rounding gives, its bf16 results in the few that lie at a border.  Two equal calls give equal bits. */
 B200_API size_t b200_prefix_scratch_bytes(const b200_prefix_args* args, const b200_rows* pass, int32_t max_length, int32_t max_prefix);
 B200_API int b200_prefix_attention(const b200_prefix_args* args, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch,
                                    size_t scratch_bytes, float* out, void* out_hi, void* out_lo, int64_t out_stride, void* stream);

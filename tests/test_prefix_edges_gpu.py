@@ -31,3 +31,114 @@ def test_odd_numbers_of_everything(monkeypatch, name):
     T.Attention(state, cache, prefix, query, of)(out)
     want, mass, size, keys = T.wanted(state, cache, prefix, query, of)
     assert (np.abs(T.host(out).reshape(want.shape) - want) <= T.attention_bound(of, mass, size, keys)).all()
+
+
+# ---- weights: what they are rounded to, and that it does not hang on the batch -----------------------------------------------------------------------
+
+
+def weight_bound(of, mass, size, keys):
+    """Of f32 and two-plane results: the weights' two bf16 planes hold all but 2^-15 of a weight (the first is cut off, 2^-7, the second rounded, 2^-8 of that) and
+    are 2^-23 too large; the rest is what attention_bound says of f32."""
+    f32 = T.attention_bound({**of, "dtype": "f32"}, mass, size, keys)
+    return f32 + (2.0 ** -15 + 2.0 ** -23) * mass if of["dtype"] == "bf16" else f32
+
+
+def bf16_bound(of, want, mass, size, keys):
+    """Of bf16 results: weights w (1 + e) with |e| <= 2^-8 in the products and in their sum, so that out is off by sum w e v / sum w (1 + e) and by out times
+    sum w e / sum w (1 + e); then rounded."""
+    weights = 2.0 ** -8 / (1 - 2.0 ** -8) * (mass + np.abs(want)) if of["dtype"] == "bf16" else 0.0
+    off = T.attention_bound({**of, "dtype": "f32"}, mass, size, keys) + weights
+    return off + 2.0 ** -8 * (np.abs(want) + off)
+
+
+@pytest.mark.parametrize("loose", [False, True])
+@pytest.mark.parametrize("spread", [1.0, 6.0])
+@pytest.mark.parametrize("name", T.ATTENTIONS)
+def test_results_are_as_good_as_their_form(name, spread, loose):
+    """f32 results; two planes alone; one plane alone."""
+    state, cache, prefix, query, of = T.attention_state(name, spread, spare=2)
+    call = T.Attention(state, cache, prefix, query, of, **(dict(max_length=1 << 16, max_prefix=1 << 16) if loose else {}))
+    want, mass, size, keys = T.wanted(state, cache, prefix, query, of)
+    width = of["heads"] * of["dim"]
+    out, (hi, lo, one) = torch.full((state.rows, width), 9.0, device="cuda"), torch.full((3, state.rows, width), 9.0, dtype=torch.bfloat16, device="cuda")
+    call(out)
+    call(None, hi, lo)
+    call(None, one)
+    out, hi, lo, one = (T.host(x).astype(np.float64) for x in (out, hi, lo, one))
+    assert (out[state.live:] == 9.0).all() and (one[state.live:] == 9.0).all()
+    bound = weight_bound(of, mass, size, keys)
+    assert (np.abs(out[:state.live].reshape(want.shape) - want) <= bound).all()
+    # the second plane of a result is rounded to 2^-8 of at most 2^-8
+    assert (np.abs((hi + lo)[:state.live].reshape(want.shape) - want) <= bound + 2.0 ** -16 * (np.abs(want) + bound)).all()
+    assert (np.abs(one[:state.live].reshape(want.shape) - want) <= bf16_bound(of, want, mass, size, keys)).all()
+
+
+BATCHES = [  # dtype, heads, kv_heads, dim, page, prefix, sequences, rows and earlier tokens of each
+    ("bf16", 32, 8, 128, 64, 2000, 40, 1, 512),
+    ("bf16", 8, 2, 64, 32, 3001, 30, 5, 700),
+    ("bf16", 8, 1, 96, 16, 900, 50, 3, 90),
+    ("bf16", 4, 4, 72, 24, 1200, 64, 2, 300),
+    ("bf16", 4, 2, 64, 64, 0, 50, 4, 2000),
+    ("bf16", 4, 2, 160, 64, 300, 30, 4, 200),
+    ("f32", 8, 2, 64, 16, 700, 40, 2, 200),
+]
+
+
+@pytest.mark.parametrize("spread", [1.0, 2.0, 6.0])
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,length,sequences,count,earlier", BATCHES)
+def test_a_sequence_by_itself_and_among_others(dtype, heads, kv_heads, dim, page, length, sequences, count, earlier, spread):
+    """Other splits, tiles and kernels for the same sequence: what f32 results differ by is what f32 allows, and bf16 results are the same but where two such
+    f32 values lie on either side of a border.  These differ by some 2^-21 of mass (a few roundings of 2^-24, and of weights near a border 2^-8 once in
+    2^12 times) and borders are 2^-8 |out| apart: one result in 2^13 |out| / mass; |out| is a 30th of mass at the least here.  Below 1 % then; it
+    was a third with weights rounded relative to the maximum."""
+    rng = np.random.default_rng(dim + count)
+    prefix_span, span = max(1, -(-length // page)), -(-(earlier + count) // page)
+    pages = prefix_span + span * sequences
+    order = rng.permutation(pages)
+    cache, prefix = T.Paged(dtype, kv_heads, page, dim, 1, order[:span * sequences].reshape(sequences, span)), T.Paged(dtype, kv_heads, page, dim, 1, order[span * sequences:].reshape(1, -1))
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    cache.key, cache.value = prefix.key, prefix.value = torch.randn((2, pages, kv_heads, page, dim), generator=g, device="cuda").to(T.TORCH[dtype])
+    query = (spread * torch.randn((sequences * count, heads, dim), generator=g, device="cuda")).to(T.TORCH[dtype])
+    results = []
+    for n in (sequences, 1):
+        state = T.Pass([count] * n, list(range(n)), [earlier] * sequences)
+        of = dict(heads=heads, dim=dim, prefixes=[length], group_first=[0, n], group_prefix=[0], dtype=dtype, max_length=earlier + count, max_prefix=length)
+        call = T.Attention(state, cache, prefix, query, of)
+        out, one = torch.empty((n * count, heads, dim), device="cuda"), torch.empty((n * count, heads, dim), dtype=torch.bfloat16, device="cuda")
+        call(out)
+        call(None, one)
+        results.append((T.host(out[:count]).astype(np.float64), T.host(one[:count])))
+    # mass and size of the sequence's rows
+    def keys_of(pool):
+        both = [pool[torch.as_tensor(table.astype(np.int64), device="cuda")].double().transpose(0, 1).reshape(kv_heads, -1, dim) for table in (prefix.table[0], cache.table[0])]
+        return torch.cat([both[0][:, :length], both[1][:, :earlier + count]], 1)
+    key, value = keys_of(cache.key), keys_of(cache.value)
+    q = query[:count].double().view(count, kv_heads, heads // kv_heads, dim)
+    score = torch.einsum("nkgd,kjd->nkgj", q, key) * dim ** -0.5
+    hidden = torch.arange(key.shape[1], device="cuda")[None] > length + earlier + torch.arange(count, device="cuda")[:, None]
+    weight = torch.softmax(score.masked_fill(hidden[:, None, None], -float("inf")), -1)
+    mass = torch.einsum("nkgj,kjd->nkgd", weight, value.abs()).reshape(count, heads, dim).cpu().numpy()
+    size = torch.einsum("nkgd,kjd->nkgj", q.abs(), key.abs()).amax(-1).reshape(count, heads).cpu().numpy() * dim ** -0.5
+    bound = weight_bound(dict(dim=dim, dtype=dtype), mass, size, np.full(count, key.shape[1]))
+    (many, many_bf16), (alone, alone_bf16) = results
+    assert (np.abs(many - alone) <= 2 * bound).all()
+    assert np.mean(many_bf16 != alone_bf16) < 0.01
+
+
+@pytest.mark.parametrize("name", ["drafts", "many rows", "wide heads", "heads of 80", "f32", "heads of 256"])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf")])
+def test_infinite_values_of_a_prefix_reach_the_results(name, value):
+    """A value that everyone sees and that is infinite: so is its column of the results of the prefix's groups, whatever their form."""
+    state, cache, prefix, query, of = T.attention_state(name)
+    page, shared, where = prefix.key.shape[2], of["group_prefix"][0], 21
+    cache.value[prefix.table[shared, where // page], :, where % page, 3] = value
+    sees = np.zeros(state.rows, dtype=bool)
+    for g, number in enumerate(of["group_prefix"]):
+        if number == shared:
+            sees[state.first[of["group_first"][g]]:state.first[of["group_first"][g + 1]]] = True
+    call = T.Attention(state, cache, prefix, query, of)
+    out, one = torch.empty((state.rows, of["heads"], of["dim"]), device="cuda"), torch.empty((state.rows, of["heads"], of["dim"]), dtype=torch.bfloat16, device="cuda")
+    call(out)
+    call(None, one)
+    for got in (T.host(out), T.host(one)):
+        assert (got[sees][:, :, 3] == value).all() and np.isfinite(got[~sees]).all() and np.isfinite(np.delete(got, 3, axis=2)).all()
