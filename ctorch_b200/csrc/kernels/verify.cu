@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const VerifyPa
             if (begin < end) bulk_load(tile + begin, own.base - own.shift + 4 * begin, (end - begin) * 16, &full[piece]);
         }
     float most = -INFINITY;
+    bool gave_up = false;
     for (int v = kTileVectors + thread; v < own.vectors; v += kPieceVectors) {
         float4 x[kSweeps];
 #pragma unroll
@@ -164,7 +165,10 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const VerifyPa
     const int sweeps = max(0, tiled - 1) / kRowThreads;   // whole ones, before the part's last vector
     const float4* mine = tile + thread;
     for (int piece = 0; piece * kPieceVectors < tiled; ++piece) {
-        if (!mbar_wait(&full[piece], 0)) atomicExch(p.status, B200_DEVICE_TIMEOUT);
+        if (!mbar_wait(&full[piece], 0)) {
+            atomicExch(p.status, B200_DEVICE_TIMEOUT);
+            gave_up = true;
+        }
         if (piece == 0 && thread == 0 && own.shift) tile[0] = own.inside(tile[0], 0);
         if (kSweeps * (piece + 1) <= sweeps) {
 #pragma unroll
@@ -223,6 +227,8 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const VerifyPa
         p.row_sum[at * p.parts + part] = sum;
         if (part == 0) p.row_max[at] = most;
     }
+    if (gave_up)   // no copy is in flight when the CTA leaves
+        for (int piece = 0; piece * kPieceVectors < tiled; ++piece) mbar_wait(&full[piece], 0);
     if (p.parts > 1) cluster_sync_all();   // the peers have read this CTA's maximum
 }
 
