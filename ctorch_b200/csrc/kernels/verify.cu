@@ -107,6 +107,13 @@ __device__ __forceinline__ double load_cluster_double(uint32_t address) {
     return value;
 }
 
+// Of a peer whose candidate is on an 8-byte boundary.
+__device__ __forceinline__ Candidate load_cluster_candidate(uint32_t address) {
+    Candidate c;
+    asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=f"(c.value), "=r"(c.index) : "r"(address) : "memory");
+    return c;
+}
+
 __device__ __forceinline__ float most_of(float4 x) { return fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)); }
 
 // grid: clusters of `parts` CTAs, two (target, draft) or one per row.  A part's first kTileVectors come to shared memory with bulk copies and stay for the
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
     __shared__ int stop_row;
     __shared__ double part_total;
     __shared__ Candidate warp_best[kVerifyWarps];
-    __shared__ Candidate part_best;
+    __shared__ alignas(8) Candidate part_best;   // read by the peers as eight bytes
     const int part = cluster_part(), s = blockIdx.x / p.draw_parts;
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
     // The pass's arrays and the logits were complete before verify_rows_kernel began: what the first tests need is fetched while that still runs.
@@ -410,8 +417,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
         cluster_sync_all();
         if (part == 0 && thread == 0) {
             for (int c = 1; c < p.draw_parts; ++c) {
-                const float2 raw = load_cluster_float2(map_peer_shared(smem_u32(&part_best), static_cast<uint32_t>(c)));
-                const Candidate other{raw.x, __float_as_int(raw.y)};
+                const Candidate other = load_cluster_candidate(map_peer_shared(smem_u32(&part_best), static_cast<uint32_t>(c)));
                 if (preferred(other, best)) best = other;
             }
             p.next[s] = best.index;
