@@ -326,6 +326,12 @@ __device__ __forceinline__ Test fetch_test(const VerifyParams& p, int row) {
     return t;
 }
 
+// The rows of a sequence whose tokens stand: its slot's length moves on.  A slot below 0 is none.
+__device__ __forceinline__ void advance_slot(const VerifyParams& p, int s, int tokens) {
+    const int slot = __ldg(p.rows.slot + s);
+    if (p.advance && slot >= 0) atomicAdd(p.rows.lengths + slot, tokens);
+}
+
 // grid: a cluster of `draw_parts` CTAs per sequence.  Dynamic shared memory: the sums of the part's segments of 128 values.
 __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const VerifyParams p) {
     extern __shared__ double segment_sum[];
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_finish_kernel(const Ver
     }
     if (part == 0 && thread == 0) {
         p.accepted[s] = row - first;
-        if (p.advance) atomicAdd(p.rows.lengths + __ldg(p.rows.slot + s), row - first + 1);
+        advance_slot(p, s, row - first + 1);
     }
 }
 
@@ -572,7 +578,7 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyParams p
     if (lane == 0) {
         p.accepted[s] = last < first ? 0 : stop - first;
         p.next[s] = token;
-        if (p.advance && last >= first) atomicAdd(p.rows.lengths + __ldg(p.rows.slot + s), stop - first + 1);
+        if (last >= first) advance_slot(p, s, stop - first + 1);
     }
 }
 

@@ -719,7 +719,8 @@ typedef struct b200_verify_args {
     const double* draw;            /* [sequences] in [0, 1) */
     int32_t* accepted;             /* [sequences] drafts accepted */
     int64_t* next;                 /* [sequences] the token behind them; -1 for a sequence without rows */
-    int32_t advance;               /* 1: lengths[slot[s]] += accepted[s] + 1, the rows of the pass whose tokens stand */
+    int32_t advance;               /* 1: lengths[slot[s]] += accepted[s] + 1, the rows of the pass whose tokens stand; a slot below 0 is none, others have to
+                                    * lie inside lengths */
 } b200_verify_args;
 B200_API size_t b200_verify_scratch_bytes(const b200_verify_args* args, const b200_rows* pass);
 B200_API int b200_verify_drafts(const b200_verify_args* args, const b200_rows* pass, void* scratch, size_t scratch_bytes, void* stream);

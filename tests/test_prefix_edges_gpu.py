@@ -142,3 +142,24 @@ def test_infinite_values_of_a_prefix_reach_the_results(name, value):
     call(None, one)
     for got in (T.host(out), T.host(one)):
         assert (got[sees][:, :, 3] == value).all() and np.isfinite(got[~sees]).all() and np.isfinite(np.delete(got, 3, axis=2)).all()
+
+
+# ---- verification ------------------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_sequences_without_a_slot_do_not_move_on(temperature):
+    """Slot -1 is none, as for append and attention: the values around the lengths stay as they are."""
+    counts = [3, 1, 0, 4, 2]
+    state, logits, draft, ids, accept, draw = T.verify_state(counts, 600, temperature, True, 17)
+    call = T.Verify(state, logits, draft, ids, temperature, accept, draw, advance=1)
+    memory = torch.arange(100, 130, dtype=torch.int32, device="cuda")
+    slots = T.dev(np.array([-1, 2, -1, 0, -5], dtype=np.int32))
+    state.args.slot, state.args.lengths = slots.data_ptr(), memory[12:].data_ptr()
+    accepted, chosen = call()
+    want = O.verify(logits, draft, ids, [int(f) for f in state.first], temperature, accept, draw)
+    assert np.array_equal(accepted, want[0]) and np.array_equal(chosen, want[1])
+    moved = np.arange(100, 130)
+    moved[12 + 2] += accepted[1] + 1
+    moved[12 + 0] += accepted[3] + 1
+    assert np.array_equal(T.host(memory), moved)
