@@ -655,8 +655,10 @@ __global__ void rows_advance_kernel(const RowsView rows, const int64_t* ids, int
     grid_launch_dependents();
     const int s = blockIdx.x * blockDim.x + threadIdx.x;
     if (s >= rows.sequences) return;
-    rows.lengths[rows.slot[s]] += rows.first[s + 1] - rows.first[s];
-    if (last) last[rows.slot[s]] = static_cast<int32_t>(ids[rows.first[s + 1] - 1]);
+    const int slot = rows.slot[s], rows_of = rows.first[s + 1] - rows.first[s];
+    if (slot < 0 || rows_of <= 0) return;
+    rows.lengths[slot] += rows_of;
+    if (last) last[slot] = static_cast<int32_t>(ids[rows.first[s + 1] - 1]);
 }
 
 __global__ void __launch_bounds__(256) dynamic_tanh_kernel(const float* x, const float* add_rows, const float* add_vector, int width,

@@ -344,7 +344,7 @@ typedef struct b200_rows {
     int32_t* lengths;              /* [slots] */
 } b200_rows;
 
-/* lengths[slot[s]] += rows of s, for every sequence of the pass. */
+/* lengths[slot[s]] += rows of s, for every sequence of the pass; a slot below 0 is none. */
 B200_API int b200_rows_advance(const b200_rows* pass, void* stream);
 
 /* out[r, :] = f32(table[ids[r], :]) * scale */
@@ -600,7 +600,7 @@ typedef struct b200_pair_embedding {
     void* normed_lo;
 } b200_pair_embedding;
 B200_API int b200_embed_pairs(const b200_pair_embedding* args, const int64_t* ids, const b200_rows* pass, void* stream);
-/* b200_rows_advance that also leaves every sequence's last token in last[slot]. */
+/* b200_rows_advance that also leaves every sequence's last token in last[slot]; a sequence without rows leaves it as it was. */
 B200_API int b200_rows_advance_tokens(const b200_rows* pass, const int64_t* ids, int32_t* last, void* stream);
 /* x <- cap * tanh(x / cap) */
 B200_API int b200_soft_cap(float* x, int64_t count, float cap, void* stream);

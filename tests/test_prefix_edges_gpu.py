@@ -163,3 +163,23 @@ def test_sequences_without_a_slot_do_not_move_on(temperature):
     moved[12 + 2] += accepted[1] + 1
     moved[12 + 0] += accepted[3] + 1
     assert np.array_equal(T.host(memory), moved)
+
+
+@pytest.mark.parametrize("tokens", [False, True])
+def test_rows_of_no_slot_do_not_move_on(tokens):
+    """b200_rows_advance and its form that keeps the last tokens: slot -1 is none, a sequence without rows has no last token."""
+    state = T.Pass([0, 3, 1, 0, 4], [0, 1, 2, 3, 4], [0] * 5)
+    lengths, last = torch.arange(100, 130, dtype=torch.int32, device="cuda"), torch.arange(200, 230, dtype=torch.int32, device="cuda")
+    slots = T.dev(np.array([4, -1, 2, -1, 0], dtype=np.int32))
+    state.args.slot, state.args.lengths = slots.data_ptr(), lengths[12:].data_ptr()
+    ids = torch.arange(7, 7 + state.rows, device="cuda")
+    if tokens:
+        B.kcheck(B.lib().b200_rows_advance_tokens(C.byref(state.args), ids.data_ptr(), last[12:].data_ptr(), T.stream()))
+    else:
+        B.kcheck(B.lib().b200_rows_advance(C.byref(state.args), T.stream()))
+    want, want_last = np.arange(100, 130), np.arange(200, 230)
+    want[12 + 2] += 1
+    want[12 + 0] += 4
+    if tokens:
+        want_last[12 + 2], want_last[12 + 0] = 7 + 3, 7 + 7
+    assert np.array_equal(T.host(lengths), want) and np.array_equal(T.host(last), want_last)
