@@ -21,7 +21,7 @@ constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
 constexpr int kPieceVectors = 1024, kTilePieces = 4;
 constexpr int kTileVectors = kTilePieces * kPieceVectors;    // 16-byte vectors of a row that a CTA holds
 constexpr int kSweeps = kPieceVectors / kRowThreads;         // of the block's threads over a piece
-static_assert(kTileVectors / kRowThreads * 4 / 2 <= 64);     // see add_weights: values of a thread per half of a sum
+static_assert(kTileVectors / kRowThreads * 4 / 2 <= 64);     // see add_weights: values of a thread per half of its sums
 constexpr int kVerifyMostParts = 8;
 
 struct VerifyParams {
@@ -50,16 +50,31 @@ __device__ __forceinline__ double widen(float w) {
     return bits < 0x00800000u ? 0.0 : __hiloint2double(static_cast<int>((bits >> 3) + (bits < 0x7f800000u ? 0x38000000u : 0x70000000u)), static_cast<int>(bits << 29));
 }
 
-// Adds the weights of two values to a sum in two parts: multiples of 2^-17, of which the at most 64 that a thread adds are exact in f32, and what is left of each
-// weight, at most 2^-18, whose sum is off by 2^-36 at most: together as good as f64 sums, at four packed operations for two values (a conversion to
-// f64 for each value takes the exponential's unit).
-__device__ __forceinline__ void add_weights(Two x, Two minus_most, Two inverse, Two& coarse, Two& fine) {
+// Adds the weights of two values to a sum in three parts: multiples of 2^-17, of which the at most 64 that a thread adds are exact in f32; what is left of each
+// weight, at most 2^-18, in multiples of 2^-36, exact as well; and what is left of that, at most 2^-37, to a sum below 2^-31, off by 2^-56 for each value.
+// A row's sum is then off by 2^-38 for 2^18 values, as good as f64 sums of as many weights (2^-53 each), without conversions, which take the exponential's unit.
+// With two parts it was off by up to 1.4e-7 (10^5 weights of 2^-18).
+struct Parts { Two coarse, middle, fine; };
+__device__ __forceinline__ void add_weights(Two x, Two minus_most, Two inverse, Parts& sum) {
     float a, b;
     split(mul_two(add_two(x, minus_most), inverse), a, b);
-    const Two w = two(expf(a), expf(b));
+    const Two w = two(expf(a), expf(b)), minus_one = two(-1.0f, -1.0f);
     const Two high = add_two(add_two(w, two(96.0f, 96.0f)), two(-96.0f, -96.0f));
-    coarse = add_two(coarse, high);
-    fine = add_two(fine, fma_two(high, two(-1.0f, -1.0f), w));
+    const Two rest = fma_two(high, minus_one, w);
+    const Two middle = add_two(add_two(rest, two(0x1.8p-13f, 0x1.8p-13f)), two(-0x1.8p-13f, -0x1.8p-13f));
+    sum.coarse = add_two(sum.coarse, high);
+    sum.middle = add_two(sum.middle, middle);
+    sum.fine = add_two(sum.fine, fma_two(middle, minus_one, rest));
+}
+__device__ __forceinline__ double total_of(const Parts& sum) {
+    float a, b;
+    double total = 0.0;
+    split(sum.fine, a, b);
+    total += static_cast<double>(a) + static_cast<double>(b);
+    split(sum.middle, a, b);
+    total += static_cast<double>(a) + static_cast<double>(b);
+    split(sum.coarse, a, b);
+    return total + (static_cast<double>(a) + static_cast<double>(b));
 }
 
 // One CTA's part of a row, in vectors of four values on 16-byte boundaries: vector v holds the values 4 v - shift .. + 3 of the part.
@@ -197,31 +212,25 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const VerifyPa
         most = warp_max(lane < p.parts ? load_cluster_float(map_peer_shared(smem_u32(&part_max), static_cast<uint32_t>(lane))) : -INFINITY);
     }
     double sum = 0.0;
-    Two coarse = two(0.0f, 0.0f), fine = two(0.0f, 0.0f);
-    const Two minus_most = two(-most, -most), inverse = two(p.inverse, p.inverse);
-    auto fold = [&] {
-        float a, b, c, d;
-        split(coarse, a, b);
-        split(fine, c, d);
-        sum += (static_cast<double>(a) + static_cast<double>(b)) + (static_cast<double>(c) + static_cast<double>(d));
-    };
+    const Two zero = two(0.0f, 0.0f), minus_most = two(-most, -most), inverse = two(p.inverse, p.inverse);
+    Parts parts{zero, zero, zero};
     auto add = [&](float4 x) {
-        add_weights(two(x.x, x.y), minus_most, inverse, coarse, fine);
-        add_weights(two(x.z, x.w), minus_most, inverse, coarse, fine);
+        add_weights(two(x.x, x.y), minus_most, inverse, parts);
+        add_weights(two(x.z, x.w), minus_most, inverse, parts);
     };
     for (int sweep = 0; sweep + 4 <= sweeps; sweep += 4)
 #pragma unroll
         for (int j = 0; j < 4; ++j) add(mine[(sweep + j) * kRowThreads]);
     for (int v = sweeps / 4 * 4 * kRowThreads + thread; v < tiled; v += kRowThreads) add(tile[v]);
-    fold();
+    sum += total_of(parts);
     for (int v = kTileVectors + thread; v < own.vectors; v += kPieceVectors) {
         float4 x[kSweeps];
 #pragma unroll
         for (int j = 0; j < kSweeps; ++j) x[j] = own.load_or_none(v + j * kRowThreads);
-        coarse = fine = two(0.0f, 0.0f);
+        parts = {zero, zero, zero};
 #pragma unroll
         for (int j = 0; j < kSweeps; ++j) add(x[j]);
-        fold();
+        sum += total_of(parts);
     }
     // values outside the part weigh nothing; where the row's maximum is itself -inf every weight is NaN, as for the values inside
     sum = warp_sum(sum);

@@ -183,3 +183,37 @@ def test_rows_of_no_slot_do_not_move_on(tokens):
     if tokens:
         want_last[12 + 2], want_last[12 + 0] = 7 + 3, 7 + 7
     assert np.array_equal(T.host(lengths), want) and np.array_equal(T.host(last), want_last)
+
+
+@pytest.mark.parametrize("level", [-12.48, -6.3, -17.9])   # weights of about 2^-18, 2^-9, 2^-26
+@pytest.mark.parametrize("vocab", [1001, 5003, 50257, 100001, 300001])
+def test_sums_of_many_small_weights(vocab, level):
+    """Rows of one token of weight 1 and vocab - 1 of one weight w, at every alignment.  Bisection over `accept` finds the shares 1 / S and w / S that the
+    kernel holds to the last bit; their quotient is w, a value of f32, and S = 1 + (vocab - 1) w.  What the sum may be off by: a thread adds at most 64 values in
+    three f32 parts, of which two are exact and the third stays below 64 2^-37, so that each addition to it is off by 2^-56 at most; what is added in 64 bits is off
+    by 2^-53 of S for each of the less than 64 additions on a value's way."""
+    counts = [2, 2, 1, 2, 2]
+    state = T.Pass(counts, list(range(5)), [0] * 5)
+    logits = np.full((state.rows, vocab), level, dtype=np.float32)
+    judged = [int(state.first[s]) for s in range(5) if counts[s] == 2]
+    assert {r * vocab % 4 for r in judged} == {0, 1, 2, 3}
+    logits[:, 0] = 0.0
+    ids = np.zeros(state.rows, dtype=np.int64)
+
+    def shares(token):
+        ids[:] = token
+        call = T.Verify(state, logits, None, ids, 1.0, np.zeros(state.rows), np.zeros(5))
+        low, high = np.zeros(4, dtype=np.int64), np.full(4, np.float64(1.0).view(np.int64))   # bits of uniforms that are accepted, and that are not
+        while (high - low > 1).any():
+            middle = (low + high) // 2
+            u = np.zeros(state.rows)
+            u[judged] = middle.view(np.float64)
+            call.keep[3].copy_(torch.as_tensor(u))
+            accepted = call()[0][[0, 1, 3, 4]] == 1
+            low, high = np.where(accepted, middle, low), np.where(accepted, high, middle)
+        return high.view(np.float64)   # u < share holds up to the value before
+    one, small = shares(0), shares(1)
+    weight = (small / one).astype(np.float32)
+    assert (np.abs(small / one / weight - 1) < 2.0 ** -50).all() and (weight == weight[0]).all() and abs(np.log(weight[0]) / level - 1) < 1e-6
+    exact = 1 + (vocab - 1) * float(weight[0])
+    assert (np.abs(one * exact - 1) <= vocab * 2.0 ** -56 / exact + 64 * 2.0 ** -53).all(), np.abs(one * exact - 1).max()
