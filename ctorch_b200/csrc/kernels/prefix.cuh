@@ -13,6 +13,7 @@ struct PrefixParams {
     RowsView rows;
     PagesView own, prefix;
     int heads, group, dim, groups;
+    int row_begin, row_end;    // of this launch: the rows of the pass from row_begin on, whose partial results begin there
     Divider by_group;
     const int32_t *group_first, *group_prefix, *prefix_length;
     const void* query;
@@ -27,8 +28,8 @@ struct PrefixParams {
     int planes;                // 1: weights as two bf16 planes
     int wide_out;              // results on 16-byte boundaries
     int32_t* status;
-    float* part_o;             // [rows * heads][splits][dim]
-    float* part_ml;            // [rows * heads][splits][2]
+    float* part_o;             // [(row_end - row_begin) * heads][splits][dim]
+    float* part_ml;            // [(row_end - row_begin) * heads][splits][2]
     float* out;
     __nv_bfloat16 *out_hi, *out_lo;
     int64_t out_stride;
@@ -100,8 +101,8 @@ __device__ __forceinline__ Item find_prefix_item(const PrefixParams& p, int inde
         if (g < p.groups) {   // two rounds of loads that do not wait for one another
             const int from = __ldg(p.group_first + g), to = __ldg(p.group_first + g + 1);
             slot = __ldg(p.group_prefix + g);
-            begin = __ldg(p.rows.first + from);
-            rows = max(0, __ldg(p.rows.first + to) - begin);
+            begin = max(__ldg(p.rows.first + from), p.row_begin);
+            rows = max(0, min(__ldg(p.rows.first + to), p.row_end) - begin);
             keys = prefix_keys(p, slot);
             tiles = (rows * p.group + p.prefix_rows - 1) / p.prefix_rows;
         }
@@ -151,16 +152,16 @@ __device__ __forceinline__ Item find_own_item(const PrefixParams& p, int index) 
     rest /= p.own_tiles;
     const int s = rest % p.rows.sequences, split = rest / p.rows.sequences;
     it.split = p.prefix_splits + split;
-    it.row = __ldg(p.rows.first + s);
-    const int count = max(0, __ldg(p.rows.first + s + 1) - it.row);
-    it.m_count = count * p.group;
+    const int first = __ldg(p.rows.first + s), count = max(0, __ldg(p.rows.first + s + 1) - first);
+    it.row = max(first, p.row_begin);
+    it.m_count = max(0, min(first + count, p.row_end) - it.row) * p.group;
     it.m_begin = tile * p.own_rows;
     it.slot = __ldg(p.rows.slot + s);
     const int length = it.slot >= 0 && it.slot < p.own.sequences ? p.rows.lengths[it.slot] : INT32_MIN / 2;
     const int keys = max(0, min(length + count, p.own.capacity()));
     it.keys = split_span(keys, p.own_splits, split);
     it.causal = true;
-    it.visible = length + 1;
+    it.visible = length + 1 + it.row - first;
     // no further than the tile's last pair sees
     it.keys.end = min(it.keys.end, it.visible + divide(max(0, min(it.m_begin + p.own_rows, it.m_count) - 1), p.by_group));
     it.live = it.m_begin < it.m_count && it.keys.begin < it.keys.end;
@@ -207,7 +208,7 @@ __device__ __forceinline__ void end_items(const PrefixParams& p) {
 }
 __device__ __forceinline__ int first_item(const PrefixParams& p) { return p.beside ? prefix_items(p) : 0; }
 
-// Pair m of an item among the pass's rows * heads, and where it leaves its partial result, a row of [rows * heads][splits].
+// Pair m of an item among the pass's rows * heads, and where it leaves its partial result, a row of [(row_end - row_begin) * heads][splits].
 __device__ __forceinline__ int64_t pair_row(const PrefixParams& p, const Item& it, int m) {
     return static_cast<int64_t>(it.row) * p.heads + it.kv_head * p.group + static_cast<int64_t>(divide(m, p.by_group)) * (p.heads - p.group) + m;
 }
@@ -242,7 +243,7 @@ template <int N> __device__ __forceinline__ void store_results(const PrefixParam
     }
 }
 __device__ __forceinline__ int64_t partial_row(const PrefixParams& p, const Item& it, int m) {
-    return pair_row(p, it, m) * (p.prefix_splits + p.own_splits) + it.split;
+    return (pair_row(p, it, m) - static_cast<int64_t>(p.row_begin) * p.heads) * (p.prefix_splits + p.own_splits) + it.split;
 }
 
 }  // namespace b200

@@ -536,8 +536,9 @@ template <int V, bool SPREAD> __global__ void __launch_bounds__(kMergeWarps * 32
     __shared__ Lanes<V> shares[SPREAD ? kMergeWarps : 1][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t index = SPREAD ? blockIdx.x : blockIdx.x * static_cast<int64_t>(kMergeWarps) + warp;
-    const int row = static_cast<int>(index / p.heads);
-    if (row >= p.rows.rows || row >= __ldg(p.rows.first + p.rows.sequences)) {
+    const int64_t row_of = p.row_begin + index / p.heads;
+    const int row = static_cast<int>(min(row_of, static_cast<int64_t>(p.row_end)));
+    if (row >= p.row_end || row >= __ldg(p.rows.first + p.rows.sequences)) {
         grid_dependency_wait();
         return;
     }
@@ -645,6 +646,7 @@ constexpr int kMostDim = 256;
 enum class Form { plain, mma };
 struct Plan {
     Form form;
+    int rows;                  // rows per launch
     bool aligned;              // 16-byte addresses, head sizes of 4 n
     bool tensor;               // the prefix's items are the tcgen05 kernel's
     bool joined;               // one item per tile of own rows goes over prefix and own tokens: no partial results
@@ -667,12 +669,12 @@ double step_time(int rows, int dim) { return rows == 16 ? (dim > 64 ? 0.6 : 0.4)
 // leaves: few splits of the prefix leave more of them and fewer partial results, many shorten the prefix's own time.  Measured, in us: a CTA of the prefix takes
 // 10 and 0.75 (heads of 64: 0.6) per step; partial results go out and back at 5 MB per us.
 struct Share { int splits, own_ctas; double time; };   // own_ctas: 0: as many as there are items for
-Share share_sms(int64_t items, int max_prefix, int dim, int own_rows, double own_steps, double part_bytes, int sms) {
+Share share_sms(int64_t items, int max_prefix, int most_splits, int dim, int own_rows, double own_steps, double part_bytes, int sms) {
     const int steps = ceil_div(max_prefix, kTensorKeys);
     const double step = dim > 64 ? 0.75 : 0.6;
     const double own = own_steps * step_time(own_rows, dim);
     Share best{1, 0, 1e30};
-    for (int n = 1; n <= kMostSplits && n <= steps; ++n) {
+    for (int n = 1; n <= most_splits && n <= steps; ++n) {
         const int64_t ctas = items * n, waves = ceil_div64(ctas, sms);
         const double wave = 10.0 + step * ceil_div(steps, n);
         const double rest = static_cast<double>(waves * sms - ctas), prefix = static_cast<double>(waves) * wave;
@@ -683,8 +685,36 @@ Share share_sms(int64_t items, int max_prefix, int dim, int own_rows, double own
     return best;
 }
 
-Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length, int max_prefix) {
+// Partial results (a maximum, a sum and an accumulator of head_dim values for a row, head and split) that a call may leave, by sizes alone of which smaller ones
+// never need more: a program that asks with its largest pass and bounds has enough for all others.  Up to 64 splits each of prefix and own tokens, as many as they
+// have steps, in 2^16 partial results; four splits together in up to 2^19 (273 MB
+// with heads of 128), in which the parts of longer passes are run one after the other.
+constexpr int64_t kManySplits = 1 << 16, kMostPartial = 1 << 19;
+int64_t partial_results(const b200_prefix_args& a, int64_t rows, int max_length, int max_prefix) {
+    const int64_t pairs = rows * a.heads;
+    const int prefix = a.groups > 0 ? std::min(ceil_div(max_prefix, kUnit), kMostSplits) : 0;
+    const int64_t splits = prefix + std::min(ceil_div(max_length, kUnit), kMostSplits);
+    return std::max(std::min(pairs * splits, kManySplits), std::min<int64_t>(pairs * std::min<int64_t>(splits, 4), std::max<int64_t>(kMostPartial, 2 * a.heads)));
+}
+// Rows whose partial results, one of the prefix and one of the own tokens, find room, in whole waves of the tcgen05 kernel's tiles.
+int64_t rows_per_launch(const b200_prefix_args& a) {
+    const int64_t most = std::max<int64_t>(1, kMostPartial / 2 / a.heads), kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
+    const int64_t waves = most * group / kTensorRows * kv_heads / 148, tiles = waves * 148 / kv_heads;
+    return tiles > 0 ? tiles * kTensorRows / group : most;
+}
+
+Plan make_plan(const b200_prefix_args& a, const b200_rows& whole, int max_length, int max_prefix, bool may_join = true) {
     Plan plan{};
+    b200_rows pass = whole;
+    if (!may_join && pass.rows > rows_per_launch(a)) {   // a joined pass leaves no partial results
+        pass.rows = rows_per_launch(a);
+        pass.sequences = static_cast<int32_t>(std::min<int64_t>(pass.sequences, pass.rows));
+        pass.max_count = static_cast<int32_t>(std::min<int64_t>(pass.max_count, pass.rows));
+    }
+    plan.rows = static_cast<int>(pass.rows);
+    // splits of prefix and own tokens together
+    const int64_t most = partial_results(a, pass.rows, max_length, max_prefix) / (pass.rows * a.heads);
+    const int most_splits = static_cast<int>(std::clamp<int64_t>(most, 2, 2 * kMostSplits));
     const int kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
     uintptr_t bits = reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.cache.key) | reinterpret_cast<uintptr_t>(a.cache.value);
     if (a.groups) bits |= reinterpret_cast<uintptr_t>(a.prefix.key) | reinterpret_cast<uintptr_t>(a.prefix.value);
@@ -702,32 +732,31 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     plan.prefix_rows = plan.tensor ? kTensorRows : plan.own_rows;
     plan.prefix_tiles = prefix ? static_cast<int>(pairs / plan.prefix_rows) + groups : 0;
     plan.own_tiles = ceil_div(own_pairs, plan.own_rows);
-    auto splits = [&](int64_t items, int keys, int ctas) {
+    auto splits = [&](int64_t items, int keys, int ctas, int room) {
         const int most = ceil_div(keys, mma ? 4 * kUnit : kUnit);   // the plain kernel takes longer over a step than a partial result costs
-        int n = static_cast<int>(ctas / (items > 0 ? items : 1));
-        if (n > most) n = most;
-        if (n > kMostSplits) n = kMostSplits;
-        return n < 1 ? 1 : n;
+        const int64_t n = std::min<int64_t>(ctas / std::max<int64_t>(items, 1), std::min({most, room, kMostSplits}));
+        return static_cast<int>(std::max<int64_t>(n, 1));
     };
     const int64_t own_items = static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads;
-    plan.own_splits = splits(own_items, max_length, 2 * 148);
+    plan.own_splits = splits(own_items, max_length, 2 * 148, prefix ? most_splits / 2 : most_splits);
+    const int room = std::min(kMostSplits, most_splits - plan.own_splits);
     const int prefix_steps = prefix ? ceil_div(max_prefix, kUnit) : 0, length_steps = ceil_div(max_length, kUnit);
     // tiles that the rows fill: the last tile of every group is half empty
     const int64_t filled = prefix ? std::max<int64_t>(ceil_div(pairs, plan.prefix_rows), groups) * kv_heads : 0;
     const int64_t own_filled = plan.own_tiles == 1 ? own_items : (ceil_div64(pairs, plan.own_rows) + pass.sequences / 2) * kv_heads;
     double time;   // of the split work, its launches and merge, in us
     if (plan.tensor) {
-        const Share share = share_sms(filled, max_prefix, a.cache.head_dim, plan.own_rows, static_cast<double>(own_filled) * length_steps,
+        const Share share = share_sms(filled, max_prefix, room, a.cache.head_dim, plan.own_rows, static_cast<double>(own_filled) * length_steps,
                                       static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8, 148);
         plan.prefix_splits = share.splits;
         plan.own_ctas = share.own_ctas;
         time = 5.0 + share.time;
     } else {
-        if (prefix) plan.prefix_splits = splits(filled, max_prefix, 2 * 148);
+        if (prefix) plan.prefix_splits = splits(filled, max_prefix, 2 * 148, room);
         const double longest = std::max(prefix ? ceil_div(prefix_steps, plan.prefix_splits) : 0, ceil_div(length_steps, plan.own_splits));
         time = 10.0 + step_time(plan.own_rows, a.cache.head_dim) * std::max(longest, (static_cast<double>(filled) * prefix_steps + static_cast<double>(own_filled) * length_steps) / 148);
     }
-    if (!mma) return plan;
+    if (!mma || !may_join) return plan;
     // Short prefixes, whose keys come from L2 each time: one item per tile of own rows goes over both and leaves the result.  Measured: 34 sequences of up to 5 tokens
     // behind 221 and 329 keys 27 us joined, 29 split; 52 single tokens behind 165 8.8 and 14.9; 9 single tokens behind 5755 61 and 24.
     const int rows = own_pairs <= 16 ? 16 : own_pairs <= 32 ? 32 : 64, tiles = ceil_div(own_pairs, rows);
@@ -743,11 +772,8 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& pass, int max_length,
     return plan;
 }
 
-// Floats of the partial accumulators: the maxima and sums behind them are read eight bytes at a time, and rows * heads * splits * head_dim may be odd.
-size_t part_floats(const b200_prefix_args& a, const b200_rows& pass, const Plan& plan) {
-    const size_t floats = static_cast<size_t>(pass.rows) * a.heads * (plan.prefix_splits + plan.own_splits) * a.cache.head_dim;
-    return (floats + 3) / 4 * 4;
-}
+// Floats of the accumulators of `results` partial results: the maxima and sums behind them are read eight bytes at a time, and results * head_dim may be odd.
+int64_t part_floats(int64_t results, int dim) { return (results * dim + 3) / 4 * 4; }
 
 bool same_heads(const b200_kv_pages& a, const b200_kv_pages& b) { return a.dtype == b.dtype && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim; }
 
@@ -807,8 +833,8 @@ using namespace b200;
 extern "C" size_t b200_prefix_scratch_bytes(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix) {
     PrefixParams p{};
     if (check_prefix(a, pass, p) != B200_OK || max_length <= 0 || max_prefix < 0) return 0;
-    const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
-    return (part_floats(*a, *pass, plan) + static_cast<size_t>(pass->rows) * a->heads * (plan.prefix_splits + plan.own_splits) * 2) * sizeof(float) + 256;
+    const int64_t results = partial_results(*a, pass->rows, max_length, max_prefix);
+    return static_cast<size_t>(part_floats(results, a->cache.head_dim) + 2 * results) * sizeof(float) + 256;
 }
 
 extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows* pass, int32_t max_length, int32_t max_prefix, void* scratch, size_t scratch_bytes,
@@ -826,7 +852,8 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
         set_error("b200_prefix_attention: scratch of %zu bytes on a 32-byte boundary needed, %zu given", need, scratch_bytes);
         return B200_BAD_ARGUMENT;
     }
-    const Plan plan = make_plan(*a, *pass, max_length, max_prefix);
+    Plan plan = make_plan(*a, *pass, max_length, max_prefix);
+    if (!plan.joined) plan = make_plan(*a, *pass, max_length, max_prefix, false);
     p.heads = a->heads; p.group = a->heads / a->cache.kv_heads; p.by_group = divider(p.group); p.dim = a->cache.head_dim;
     p.groups = plan.prefix_splits || (plan.joined && max_prefix > 0) ? a->groups : 0;
     p.joined = plan.joined;
@@ -837,44 +864,52 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
     p.prefix_splits = plan.prefix_splits; p.own_splits = plan.own_splits; p.prefix_tiles = plan.prefix_tiles; p.own_tiles = plan.own_tiles;
     p.prefix_rows = plan.prefix_rows; p.own_rows = plan.own_rows;
     p.part_o = static_cast<float*>(scratch);
-    p.part_ml = p.part_o + part_floats(*a, *pass, plan);
+    p.part_ml = p.part_o + part_floats(static_cast<int64_t>(plan.rows) * a->heads * (plan.prefix_splits + plan.own_splits), p.dim);
     p.out = out; p.out_hi = static_cast<__nv_bfloat16*>(out_hi); p.out_lo = static_cast<__nv_bfloat16*>(out_lo);
     p.out_stride = out_stride ? out_stride : width;
     p.wide_out = (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_hi) | reinterpret_cast<uintptr_t>(out_lo)) % 16 == 0 && p.out_stride % 8 == 0 && p.dim % 8 == 0;
     const int64_t prefix_items = static_cast<int64_t>(plan.prefix_tiles) * plan.prefix_splits * a->cache.kv_heads;
     const int64_t own_items = static_cast<int64_t>(pass->sequences) * plan.own_tiles * plan.own_splits * a->cache.kv_heads;
-    const int64_t merges = (pass->rows * a->heads + kMergeWarps - 1) / kMergeWarps;
-    if (prefix_items + own_items > INT32_MAX || merges > INT32_MAX || static_cast<int64_t>(pass->rows) * p.group > INT32_MAX / 2) {
+    if (prefix_items + own_items > INT32_MAX || static_cast<int64_t>(pass->rows) * p.group > INT32_MAX / 2) {
         set_error("b200_prefix_attention: too many rows");
         return B200_UNSUPPORTED;
     }
     cudaStream_t s = as_stream(stream);
-    int status;
-    int ctas = 2 * 148;
+    int whole_ctas = 2 * 148;
     if (plan.form == Form::mma) {
         int device = 0;
         B200_CUDA(cudaGetDevice(&device));
-        ctas = 2 * sm_count(device);
+        whole_ctas = 2 * sm_count(device);
         p.status = device_status_word(device);
         if (!p.status) { set_error("b200_prefix_attention: the device status word could not be allocated"); return B200_NO_DEVICE; }
     }
-    if (plan.tensor) {
-        status = launch_prefix_tensor(p, static_cast<int>(prefix_items), s);
-        if (status != B200_OK) return status;
-        p.beside = 1;
-    }
-    p.items = static_cast<int>(plan.tensor ? own_items : prefix_items + own_items);
-    // beside the prefix: CTAs for the SMs that are free at once, or, where those do not suffice, two items per CTA, which begin as SMs become free
-    if (plan.tensor) ctas = plan.own_ctas ? plan.own_ctas : std::max(ctas, (p.items + 1) / 2);
-    const unsigned items = static_cast<unsigned>(p.items);
-    if (plan.form == Form::plain)
-        status = cuda_status(a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, plan.aligned, s) : launch_plain<float>(p, items, plan.aligned, s),
-                             "prefix_plain_kernel launch");
-    else
-        status = p.dim <= 64 ? launch_mma<64>(p, ctas, s) : p.dim <= 96 ? launch_mma<96>(p, ctas, s) : launch_mma<128>(p, ctas, s);
-    if (status != B200_OK || plan.joined) return status;
-    const bool spread = plan.prefix_splits + plan.own_splits > 8 && pass->rows * static_cast<int64_t>(a->heads) <= 8 * 148;
+    const bool spread = plan.prefix_splits + plan.own_splits > 8 && plan.rows * static_cast<int64_t>(a->heads) <= 8 * 148;
     auto merge = spread ? (p.dim % 4 == 0 ? prefix_merge_kernel<4, true> : prefix_merge_kernel<1, true>)
                         : (p.dim % 4 == 0 ? prefix_merge_kernel<4, false> : prefix_merge_kernel<1, false>);
-    return cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(spread ? pass->rows * a->heads : merges)), dim3(kMergeWarps * 32), 0, s, p), "prefix_merge_kernel launch");
+    for (int begin = 0; begin < p.rows.rows; begin += plan.rows) {
+        p.row_begin = begin;
+        p.row_end = std::min(p.rows.rows, begin + plan.rows);
+        p.beside = 0;
+        int ctas = whole_ctas, status;
+        if (plan.tensor) {
+            status = launch_prefix_tensor(p, static_cast<int>(prefix_items), s);
+            if (status != B200_OK) return status;
+            p.beside = 1;
+        }
+        p.items = static_cast<int>(plan.tensor ? own_items : prefix_items + own_items);
+        // beside the prefix: CTAs for the SMs that are free at once, or, where those do not suffice, two items per CTA, which begin as SMs become free
+        if (plan.tensor) ctas = plan.own_ctas ? plan.own_ctas : std::max(ctas, (p.items + 1) / 2);
+        const unsigned items = static_cast<unsigned>(p.items);
+        if (plan.form == Form::plain)
+            status = cuda_status(a->cache.dtype == B200_BF16 ? launch_plain<__nv_bfloat16>(p, items, plan.aligned, s) : launch_plain<float>(p, items, plan.aligned, s),
+                                 "prefix_plain_kernel launch");
+        else
+            status = p.dim <= 64 ? launch_mma<64>(p, ctas, s) : p.dim <= 96 ? launch_mma<96>(p, ctas, s) : launch_mma<128>(p, ctas, s);
+        if (status != B200_OK || plan.joined) return status;
+        const int64_t pairs = static_cast<int64_t>(p.row_end - begin) * a->heads;
+        status = cuda_status(launch_dependent(merge, dim3(static_cast<unsigned>(spread ? pairs : ceil_div64(pairs, kMergeWarps))), dim3(kMergeWarps * 32), 0, s, p),
+                             "prefix_merge_kernel launch");
+        if (status != B200_OK) return status;
+    }
+    return B200_OK;
 }

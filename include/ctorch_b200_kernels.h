@@ -691,7 +691,9 @@ typedef struct b200_prefix_args {
     const int32_t* prefix_length;  /* [prefixes] */
 } b200_prefix_args;
 /* max_length and max_prefix: upper bounds of lengths[slot] + rows of a sequence and of a prefix's length, by which the work is split (the pages
- * of a table bound what is read).  The result [rows, heads*dim] in f32 (out) and / or as planes, out_stride elements between rows (0: heads*dim).
+ * of a table bound what is read).  The scratch (32-byte boundary) grows with rows, max_length and max_prefix and hangs on nothing else but heads, head_dim and
+ * whether there are groups, up to 2^19 (head_dim + 2) floats; what is asked for with the largest pass and bounds is enough for all smaller ones.
+ * The result [rows, heads*dim] in f32 (out) and / or as planes, out_stride elements between rows (0: heads*dim).
  * bf16 caches: products of bf16 queries, keys and values with f32 sums.  Results in f32 or two planes take the softmax's weights with 15 bits (two bf16 planes),
  * results in one plane with 8, rounded in product and sum alike.  The work is split by the whole pass, and the split sets the order of the f32 sums: between
  * batches a sequence's f32 results differ by what f32 rounding gives, its bf16 results in the few that lie at a border.  Two equal calls give equal bits. */

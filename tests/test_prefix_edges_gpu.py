@@ -217,3 +217,63 @@ def test_sums_of_many_small_weights(vocab, level):
     assert (np.abs(small / one / weight - 1) < 2.0 ** -50).all() and (weight == weight[0]).all() and abs(np.log(weight[0]) / level - 1) < 1e-6
     exact = 1 + (vocab - 1) * float(weight[0])
     assert (np.abs(one * exact - 1) <= vocab * 2.0 ** -56 / exact + 64 * 2.0 ** -53).all(), np.abs(one * exact - 1).max()
+
+
+# ---- passes that run part after part -----------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,counts,lengths,prefixes,group_first,group_prefix", [
+    ("bf16", 128, 8, 64, 32, [1500, 1, 900, 3, 0, 2500, 40, 100], [10, 0, 70, 5, 3, 33, 64, 2], [300, 77], [0, 4, 8], [1, 0]),
+    ("bf16", 256, 4, 128, 16, [700, 700, 800], [0, 100, 3], [130], [1, 3], [0]),
+    ("bf16", 128, 128, 36, 10, [2100, 200], [20, 0], [50], [0, 2], [0]),
+    ("f32", 192, 16, 20, 16, [1, 1400, 1, 1700], [20, 0, 50, 31], [90, 10, 33], [0, 1, 2, 4], [2, 0, 1]),
+    ("bf16", 256, 2, 64, 64, [1] * 2600, [i % 90 for i in range(2600)], [500], [0, 2600], [0]),
+])
+def test_passes_of_more_rows_than_partial_results_find_room(dtype, heads, kv_heads, dim, page, counts, lengths, prefixes, group_first, group_prefix):
+    """2^18 pairs of a row and a head run at once; these passes have more, with sequences and groups across the borders of the parts."""
+    rng = np.random.default_rng(heads + dim)
+    n, rows = len(counts), sum(counts)
+    assert rows * heads > 1 << 18
+    span, prefix_span = -(-max(c + i for c, i in zip(counts, lengths)) // page), -(-max(prefixes) // page)
+    pages = n * span + len(prefixes) * prefix_span
+    order = rng.permutation(pages)
+    slots = rng.permutation(n)
+    of_slot = np.empty(n, dtype=np.int64)
+    of_slot[slots] = lengths
+    cache = T.Paged(dtype, kv_heads, page, dim, 1, order[:n * span].reshape(n, span))
+    prefix = T.Paged(dtype, kv_heads, page, dim, 1, order[n * span:].reshape(len(prefixes), prefix_span))
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    cache.key, cache.value = prefix.key, prefix.value = torch.randn((2, pages, kv_heads, page, dim), generator=g, device="cuda").to(T.TORCH[dtype])
+    state = T.Pass(counts, slots, of_slot, spare=5)
+    query = torch.randn((state.rows, heads, dim), generator=g, device="cuda").to(T.TORCH[dtype])
+    of = dict(heads=heads, dim=dim, prefixes=prefixes, group_first=group_first, group_prefix=group_prefix, dtype=dtype, max_length=1 << 14, max_prefix=1 << 16)
+    call = T.Attention(state, cache, prefix, query, of)
+    call.scratch = torch.full((call.need + 4096,), 0xff, dtype=torch.uint8, device="cuda")
+    out = torch.full((state.rows, heads, dim), 9.0, device="cuda")
+    call(out)
+    assert (call.scratch[call.need:] == 0xff).all() and (out[state.live:] == 9.0).all()
+    group = heads // kv_heads
+    for s in range(n):
+        if s >= 60 and s % 97:   # of very many sequences some
+            continue
+        begin, count = int(state.first[s]), counts[s]
+        if not count:
+            continue
+        owner = [i for i in range(len(group_prefix)) if group_first[i] <= s < group_first[i + 1]]
+        shared = prefixes[group_prefix[owner[0]]] if owner else 0
+
+        def keys_of(pool):
+            a = pool[torch.as_tensor(prefix.table[group_prefix[owner[0]]] if owner else prefix.table[0], device="cuda").long()].double().transpose(0, 1).reshape(kv_heads, -1, dim)
+            b = pool[torch.as_tensor(cache.table[slots[s]], device="cuda").long()].double().transpose(0, 1).reshape(kv_heads, -1, dim)
+            return torch.cat([a[:, :shared], b[:, :lengths[s] + count]], 1)
+        key, value = keys_of(cache.key), keys_of(cache.value)
+        for at in range(0, count, 256):
+            part = query[begin + at:begin + min(count, at + 256)].double().view(-1, kv_heads, group, dim)
+            m = len(part)
+            score = torch.einsum("nkgd,kjd->nkgj", part, key) * dim ** -0.5
+            hidden = torch.arange(key.shape[1], device="cuda")[None] > shared + lengths[s] + at + torch.arange(m, device="cuda")[:, None]
+            weight = torch.softmax(score.masked_fill(hidden[:, None, None], -float("inf")), -1)
+            want, mass = (torch.einsum("nkgj,kjd->nkgd", weight, v).reshape(m, heads, dim).cpu().numpy() for v in (value, value.abs()))
+            size = torch.einsum("nkgd,kjd->nkgj", part.abs(), key.abs()).amax(-1).reshape(m, heads).cpu().numpy() * dim ** -0.5
+            got = T.host(out[begin + at:begin + at + m])
+            assert (np.abs(got - want) <= weight_bound(of, mass, size, np.full(m, key.shape[1]))).all(), (s, at)
