@@ -796,12 +796,13 @@ int check_prefix(const b200_prefix_args* a, const b200_rows* pass, PrefixParams&
 
 template <class T, int ROWS> cudaError_t launch_plain(const PrefixParams& p, unsigned items, bool whole, cudaStream_t stream) {
     auto kernel = p.dim <= 64 ? prefix_plain_kernel<T, 2, ROWS> : p.dim <= 128 ? prefix_plain_kernel<T, 4, ROWS> : prefix_plain_kernel<T, 8, ROWS>;
-    const int smem = plain_smem(p.dim, 16 * ROWS);
-    if (smem > 48 * 1024) {
-        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the kernel's limit is the same whatever the head size: a call beside this one may be between setting it and launching
+    const int most = plain_smem(p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, 16 * ROWS);
+    if (most > 48 * 1024) {
+        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (status != cudaSuccess) return status;
     }
-    return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(smem), stream, p, whole);
+    return launch_dependent(kernel, dim3(items), dim3(kPlainThreads), static_cast<size_t>(plain_smem(p.dim, 16 * ROWS)), stream, p, whole);
 }
 template <class T> cudaError_t launch_plain(const PrefixParams& p, unsigned items, bool whole, cudaStream_t stream) {
     return p.own_rows == 16 ? launch_plain<T, 1>(p, items, whole, stream) : launch_plain<T, 2>(p, items, whole, stream);

@@ -22,7 +22,7 @@ constexpr int kPieceVectors = 1024, kTilePieces = 4;
 constexpr int kTileVectors = kTilePieces * kPieceVectors;    // 16-byte vectors of a row that a CTA holds
 constexpr int kSweeps = kPieceVectors / kRowThreads;         // of the block's threads over a piece
 static_assert(kTileVectors / kRowThreads * 4 / 2 <= 64);     // see add_weights: values of a thread per half of its sums
-constexpr int kVerifyMostParts = 8;
+constexpr int kVerifyMostParts = 8, kVerifyMostVocab = 1 << 23;
 
 struct VerifyParams {
     RowsView rows;
@@ -599,6 +599,8 @@ int split_rows(int64_t vocab, int64_t rows, int64_t ctas) {
     while (parts < kVerifyMostParts && (vocab > static_cast<int64_t>(parts) * (4 * kTileVectors - 8) || (rows * parts < ctas && vocab >= 2 * parts * kLeast))) parts *= 2;
     return parts;
 }
+// Shared memory of the drawing kernel for a part of `chunk` values.
+size_t segment_bytes(int chunk) { return static_cast<size_t>((chunk + 3) / 4 + 1 + 31) / 32 * sizeof(double); }
 int chunk_of(int vocab, int parts) { return ((vocab + parts - 1) / parts + 3) / 4 * 4; }
 
 }  // namespace
@@ -622,7 +624,7 @@ extern "C" int b200_verify_drafts(const b200_verify_args* a, const b200_rows* pa
     }
     const float inverse = a->temperature > 0.0 ? static_cast<float>(1.0 / a->temperature) : 1.0f;
     if (!std::isfinite(inverse) || inverse == 0.0f) { set_error("b200_verify_drafts: temperature %g is out of range", a->temperature); return B200_BAD_ARGUMENT; }
-    if (a->vocab > (1 << 23)) { set_error("b200_verify_drafts: more than 2^23 values per row are not supported"); return B200_UNSUPPORTED; }
+    if (a->vocab > kVerifyMostVocab) { set_error("b200_verify_drafts: more than 2^23 values per row are not supported"); return B200_UNSUPPORTED; }
     const size_t need = b200_verify_scratch_bytes(a, pass);
     if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 8) {
         set_error("b200_verify_drafts: scratch of %zu bytes on an 8-byte boundary needed, %zu given", need, scratch_bytes);
@@ -658,8 +660,9 @@ extern "C" int b200_verify_drafts(const b200_verify_args* a, const b200_rows* pa
     const int status = cuda_status(launch_dependent_cluster(verify_rows_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kRowThreads), held, st,
                                                             dim3(static_cast<unsigned>(p.parts), 1, 1), p), "verify_rows_kernel launch");
     if (status != B200_OK) return status;
-    const size_t smem = static_cast<size_t>((p.draw_chunk + 3) / 4 + 1 + 31) / 32 * sizeof(double);
-    if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(verify_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    const size_t smem = segment_bytes(p.draw_chunk);
+    // the same limit for all vocabularies: a call beside this one may be between setting it and launching
+    if (smem > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(verify_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(segment_bytes(kVerifyMostVocab / kVerifyMostParts))));
     return cuda_status(launch_dependent_cluster(verify_finish_kernel, dim3(static_cast<unsigned>(p.rows.sequences * p.draw_parts)), dim3(kVerifyThreads), smem, st,
                                                 dim3(static_cast<unsigned>(p.draw_parts), 1, 1), p), "verify_finish_kernel launch");
 }

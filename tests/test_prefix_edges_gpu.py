@@ -277,3 +277,62 @@ def test_passes_of_more_rows_than_partial_results_find_room(dtype, heads, kv_hea
             size = torch.einsum("nkgd,kjd->nkgj", part.abs(), key.abs()).amax(-1).reshape(m, heads).cpu().numpy() * dim ** -0.5
             got = T.host(out[begin + at:begin + at + m])
             assert (np.abs(got - want) <= weight_bound(of, mass, size, np.full(m, key.shape[1]))).all(), (s, at)
+
+
+# ---- two calls at once -------------------------------------------------------------------------------------------------------------------------------
+
+
+def at_once(calls, times=400):
+    """Every call again and again, each from a thread and on a stream of its own; what they return."""
+    import threading
+    failed, start = [], threading.Barrier(len(calls))
+
+    def loop(call, stream):
+        start.wait()
+        for _ in range(times):
+            status = call(stream.cuda_stream)
+            if status != 0:
+                failed.append((status, B.lib().b200_last_error().decode()))
+                return
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=loop, args=a) for a in zip(calls, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return failed
+
+
+def test_attention_of_different_head_sizes_at_once():
+    """The plain kernel's shared memory hangs on the head size: heads of 128 and of 116 share a kernel and need more than the default."""
+    calls, checks = [], []
+    for dim in (128, 116, 124):
+        T.ATTENTIONS["at once"] = ("f32", 16, 1, dim, 16, [40], [0, 3], [0], [2, 1, 2], [10, 0, 31])
+        state, cache, prefix, query, of = T.attention_state("at once")
+        del T.ATTENTIONS["at once"]
+        call, out = T.Attention(state, cache, prefix, query, of), torch.empty((state.rows, 16, dim), device="cuda")
+        calls.append(lambda stream, call=call, out=out: B.lib().b200_prefix_attention(C.byref(call.a), C.byref(call.rows), call.max_length, call.max_prefix,
+                                                                                        call.scratch.data_ptr(), call.need, out.data_ptr(), None, None, 0, stream))
+        checks.append((state, cache, prefix, query, of, out))
+    assert at_once(calls) == []
+    for state, cache, prefix, query, of, out in checks:
+        want, mass, size, keys = T.wanted(state, cache, prefix, query, of)
+        assert (np.abs(T.host(out).reshape(want.shape) - want) <= T.attention_bound(of, mass, size, keys)).all()
+
+
+def test_verification_of_different_vocabularies_at_once():
+    """The draw's shared memory hangs on the vocabulary; beyond 6 million values it is more than the default."""
+    calls, checks = [], []
+    for vocab in (1 << 23, 6_500_000, 7_300_001):
+        state = T.Pass([2], [0], [0])
+        logits = torch.full((2, vocab), -30.0, device="cuda")
+        logits[:, vocab - 5] = 0.0
+        check = T.Verify(state, np.zeros((2, 1), dtype=np.float32), None, np.array([3, vocab - 5]), 1.0, [0.5, 0.5], [0.5])
+        check.a.vocab, check.a.logits = vocab, logits.data_ptr()
+        calls.append(lambda stream, check=check: B.lib().b200_verify_drafts(C.byref(check.a), C.byref(check.state.args), check.scratch.data_ptr(), check.need, stream))
+        checks.append((check, logits, vocab))
+    assert at_once(calls) == []
+    for check, _, vocab in checks:
+        assert T.host(check.accepted).tolist() == [1] and T.host(check.next).tolist() == [vocab - 5]
