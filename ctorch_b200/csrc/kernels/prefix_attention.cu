@@ -662,6 +662,8 @@ int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+constexpr int kSms = 148;   // of a B200: plans are made from sizes alone, without asking a device, and so are the launches
+
 // us that a step of prefix_mma_kernel takes an SM, measured, and a CTA that has an SM to itself.
 double step_time(int rows, int dim) { return rows == 16 ? (dim > 64 ? 0.6 : 0.4) : rows == 32 ? (dim > 64 ? 1.0 : 0.65) : dim > 64 ? 1.7 : 0.9; }
 
@@ -669,16 +671,16 @@ double step_time(int rows, int dim) { return rows == 16 ? (dim > 64 ? 0.6 : 0.4)
 // leaves: few splits of the prefix leave more of them and fewer partial results, many shorten the prefix's own time.  Measured, in us: a CTA of the prefix takes
 // 10 and 0.75 (heads of 64: 0.6) per step; partial results go out and back at 5 MB per us.
 struct Share { int splits, own_ctas; double time; };   // own_ctas: 0: as many as there are items for
-Share share_sms(int64_t items, int max_prefix, int most_splits, int dim, int own_rows, double own_steps, double part_bytes, int sms) {
+Share share_sms(int64_t items, int max_prefix, int most_splits, int dim, int own_rows, double own_steps, double part_bytes) {
     const int steps = ceil_div(max_prefix, kTensorKeys);
     const double step = dim > 64 ? 0.75 : 0.6;
     const double own = own_steps * step_time(own_rows, dim);
     Share best{1, 0, 1e30};
     for (int n = 1; n <= most_splits && n <= steps; ++n) {
-        const int64_t ctas = items * n, waves = ceil_div64(ctas, sms);
+        const int64_t ctas = items * n, waves = ceil_div64(ctas, kSms);
         const double wave = 10.0 + step * ceil_div(steps, n);
-        const double rest = static_cast<double>(waves * sms - ctas), prefix = static_cast<double>(waves) * wave;
-        const double free_only = rest > 0 ? std::max(prefix, prefix - wave + own / rest) : 1e30, all = prefix + std::max(0.0, own - rest * wave) / sms;
+        const double rest = static_cast<double>(waves * kSms - ctas), prefix = static_cast<double>(waves) * wave;
+        const double free_only = rest > 0 ? std::max(prefix, prefix - wave + own / rest) : 1e30, all = prefix + std::max(0.0, own - rest * wave) / kSms;
         const double time = std::min(free_only, all) + n * part_bytes / 5e6;
         if (time < best.time) best = {n, free_only <= all ? static_cast<int>(2 * rest) : 0, time};
     }
@@ -699,7 +701,7 @@ int64_t partial_results(const b200_prefix_args& a, int64_t rows, int max_length,
 // Rows whose partial results, one of the prefix and one of the own tokens, find room, in whole waves of the tcgen05 kernel's tiles.
 int64_t rows_per_launch(const b200_prefix_args& a) {
     const int64_t most = std::max<int64_t>(1, kMostPartial / 2 / a.heads), kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
-    const int64_t waves = most * group / kTensorRows * kv_heads / 148, tiles = waves * 148 / kv_heads;
+    const int64_t waves = most * group / kTensorRows * kv_heads / kSms, tiles = waves * kSms / kv_heads;
     return tiles > 0 ? tiles * kTensorRows / group : most;
 }
 
@@ -738,7 +740,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& whole, int max_length
         return static_cast<int>(std::max<int64_t>(n, 1));
     };
     const int64_t own_items = static_cast<int64_t>(pass.sequences) * plan.own_tiles * kv_heads;
-    plan.own_splits = splits(own_items, max_length, 2 * 148, prefix ? most_splits / 2 : most_splits);
+    plan.own_splits = splits(own_items, max_length, 2 * kSms, prefix ? most_splits / 2 : most_splits);
     const int room = std::min(kMostSplits, most_splits - plan.own_splits);
     const int prefix_steps = prefix ? ceil_div(max_prefix, kUnit) : 0, length_steps = ceil_div(max_length, kUnit);
     // tiles that the rows fill: the last tile of every group is half empty
@@ -747,14 +749,14 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& whole, int max_length
     double time;   // of the split work, its launches and merge, in us
     if (plan.tensor) {
         const Share share = share_sms(filled, max_prefix, room, a.cache.head_dim, plan.own_rows, static_cast<double>(own_filled) * length_steps,
-                                      static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8, 148);
+                                      static_cast<double>(pairs) * kv_heads * a.cache.head_dim * 8);
         plan.prefix_splits = share.splits;
         plan.own_ctas = share.own_ctas;
         time = 5.0 + share.time;
     } else {
-        if (prefix) plan.prefix_splits = splits(filled, max_prefix, 2 * 148, room);
+        if (prefix) plan.prefix_splits = splits(filled, max_prefix, 2 * kSms, room);
         const double longest = std::max(prefix ? ceil_div(prefix_steps, plan.prefix_splits) : 0, ceil_div(length_steps, plan.own_splits));
-        time = 10.0 + step_time(plan.own_rows, a.cache.head_dim) * std::max(longest, (static_cast<double>(filled) * prefix_steps + static_cast<double>(own_filled) * length_steps) / 148);
+        time = 10.0 + step_time(plan.own_rows, a.cache.head_dim) * std::max(longest, (static_cast<double>(filled) * prefix_steps + static_cast<double>(own_filled) * length_steps) / kSms);
     }
     if (!mma || !may_join) return plan;
     // Short prefixes, whose keys come from L2 each time: one item per tile of own rows goes over both and leaves the result.  Measured: 34 sequences of up to 5 tokens
@@ -762,7 +764,7 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& whole, int max_length
     const int rows = own_pairs <= 16 ? 16 : own_pairs <= 32 ? 32 : 64, tiles = ceil_div(own_pairs, rows);
     const int64_t items = (tiles == 1 ? pass.sequences : ceil_div64(pairs, rows) + pass.sequences / 2) * kv_heads;
     const double step = step_time(rows, a.cache.head_dim);
-    if (6.0 + step * (2.5 + (prefix_steps + length_steps) * std::max(1.0, static_cast<double>(items) / 148)) > time) return plan;
+    if (6.0 + step * (2.5 + (prefix_steps + length_steps) * std::max(1.0, static_cast<double>(items) / kSms)) > time) return plan;
     plan.joined = true;
     plan.tensor = false;
     plan.own_rows = plan.prefix_rows = rows;
@@ -876,22 +878,20 @@ extern "C" int b200_prefix_attention(const b200_prefix_args* a, const b200_rows*
         return B200_UNSUPPORTED;
     }
     cudaStream_t s = as_stream(stream);
-    int whole_ctas = 2 * 148;
     if (plan.form == Form::mma) {
         int device = 0;
         B200_CUDA(cudaGetDevice(&device));
-        whole_ctas = 2 * sm_count(device);
         p.status = device_status_word(device);
         if (!p.status) { set_error("b200_prefix_attention: the device status word could not be allocated"); return B200_NO_DEVICE; }
     }
-    const bool spread = plan.prefix_splits + plan.own_splits > 8 && plan.rows * static_cast<int64_t>(a->heads) <= 8 * 148;
+    const bool spread = plan.prefix_splits + plan.own_splits > 8 && plan.rows * static_cast<int64_t>(a->heads) <= 8 * kSms;
     auto merge = spread ? (p.dim % 4 == 0 ? prefix_merge_kernel<4, true> : prefix_merge_kernel<1, true>)
                         : (p.dim % 4 == 0 ? prefix_merge_kernel<4, false> : prefix_merge_kernel<1, false>);
     for (int begin = 0; begin < p.rows.rows; begin += plan.rows) {
         p.row_begin = begin;
         p.row_end = std::min(p.rows.rows, begin + plan.rows);
         p.beside = 0;
-        int ctas = whole_ctas, status;
+        int ctas = 2 * kSms, status;
         if (plan.tensor) {
             status = launch_prefix_tensor(p, static_cast<int>(prefix_items), s);
             if (status != B200_OK) return status;
