@@ -31,6 +31,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Adds a packed pair to two f32 sums, without unpacking it first.
+__device__ __forceinline__ void add_bf16(uint32_t pair, float& low, float& high) {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.rn.f32.bf16 %0, l, %0;\n add.rn.f32.bf16 %1, h, %1;\n}" : "+f"(low), "+f"(high) : "r"(pair));
+}
 // hi and lo planes of an adjacent pair
 __device__ __forceinline__ void pack_planes(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
