@@ -336,3 +336,76 @@ def test_verification_of_different_vocabularies_at_once():
     assert at_once(calls) == []
     for check, _, vocab in checks:
         assert T.host(check.accepted).tolist() == [1] and T.host(check.next).tolist() == [vocab - 5]
+
+
+# ---- long contexts, lengths that the pages do not hold -----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,length,sequences,count,earlier", [
+    ("bf16", 8, 2, 64, 64, 131072, 1, 1, 30),        # few rows: tiles of 16 pairs
+    ("bf16", 4, 1, 128, 32, 100003, 40, 3, 100),     # many: the tcgen05 kernel
+    ("bf16", 4, 1, 128, 64, 70, 2, 3, 70001),        # own tokens that are long
+    ("bf16", 2, 1, 36, 10, 65537, 3, 2, 50),         # plain
+    ("f32", 4, 2, 64, 16, 70001, 5, 2, 33000),
+])
+def test_long_contexts(dtype, heads, kv_heads, dim, page, length, sequences, count, earlier):
+    prefix_span, span = -(-length // page), -(-(earlier + count) // page)
+    pages = prefix_span + span * sequences
+    order = np.random.default_rng(dim).permutation(pages)
+    cache, prefix = T.Paged(dtype, kv_heads, page, dim, 1, order[:span * sequences].reshape(sequences, span)), T.Paged(dtype, kv_heads, page, dim, 1, order[span * sequences:].reshape(1, -1))
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    cache.key, cache.value = prefix.key, prefix.value = torch.randn((2, pages, kv_heads, page, dim), generator=g, device="cuda").to(T.TORCH[dtype])
+    query = (2.0 * torch.randn((sequences * count, heads, dim), generator=g, device="cuda")).to(T.TORCH[dtype])
+    state = T.Pass([count] * sequences, list(range(sequences)), [earlier] * sequences)
+    of = dict(heads=heads, dim=dim, prefixes=[length], group_first=[0, sequences], group_prefix=[0], dtype=dtype, max_length=earlier + count, max_prefix=length)
+    out = torch.empty((sequences * count, heads, dim), device="cuda")
+    T.Attention(state, cache, prefix, query, of)(out)
+    for s in range(0, sequences, 7):
+        def keys_of(pool):
+            both = [pool[torch.as_tensor(t.astype(np.int64), device="cuda")].double().transpose(0, 1).reshape(kv_heads, -1, dim) for t in (prefix.table[0], cache.table[s])]
+            return torch.cat([both[0][:, :length], both[1][:, :earlier + count]], 1)
+        key, value = keys_of(cache.key), keys_of(cache.value)
+        q = query[s * count:(s + 1) * count].double().view(count, kv_heads, heads // kv_heads, dim)
+        hidden = torch.arange(key.shape[1], device="cuda")[None] > length + earlier + torch.arange(count, device="cuda")[:, None]
+        weight = torch.softmax((torch.einsum("nkgd,kjd->nkgj", q, key) * dim ** -0.5).masked_fill(hidden[:, None, None], -float("inf")), -1)
+        want, mass = (torch.einsum("nkgj,kjd->nkgd", weight, v).reshape(count, heads, dim).cpu().numpy() for v in (value, value.abs()))
+        size = torch.einsum("nkgd,kjd->nkgj", q.abs(), key.abs()).amax(-1).reshape(count, heads).cpu().numpy() * dim ** -0.5
+        got = T.host(out[s * count:(s + 1) * count])
+        assert (np.abs(got - want) <= weight_bound(of, mass, size, np.full(count, key.shape[1]))).all(), s
+
+
+@pytest.mark.parametrize("loose", [False, True])
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,counts", [
+    ("bf16", 8, 2, 64, 16, [1, 2, 1, 3]), ("bf16", 16, 1, 128, 64, [9, 7, 20, 11]), ("bf16", 4, 2, 33, 10, [1, 9, 2, 2]), ("f32", 4, 2, 64, 16, [3, 1, 2, 2]),
+])
+def test_lengths_that_the_pages_do_not_hold(dtype, heads, kv_heads, dim, page, counts, loose):
+    """Prefix lengths below 0 and past the table, lengths past the slot's pages: what the pages hold is what there is."""
+    rng = np.random.default_rng(page)
+    cache, prefix = (T.Paged(dtype, kv_heads, page, dim, 24, t, rng) for t in (rng.permutation(24)[:12].reshape(4, 3), rng.permutation(24)[:12].reshape(4, 3)))
+    prefix.key, prefix.value = cache.key, cache.value
+    state = T.Pass(counts, [2, 0, 3, 1], [3 * page - 1, 5 * page, 0, 3 * page])
+    query = T.dev(rng.standard_normal((state.rows, heads, dim), dtype=np.float32), T.TORCH[dtype])
+    of = dict(heads=heads, dim=dim, prefixes=[-5, 10 * page, 3 * page, 1], group_first=[0, 1, 2, 3, 4], group_prefix=[1, 0, 2, 3], dtype=dtype,
+              max_length=1 << 16 if loose else 6 * page, max_prefix=1 << 16 if loose else 10 * page)
+    out = torch.empty((state.rows, heads, dim), device="cuda")
+    T.Attention(state, cache, prefix, query, of)(out)
+    want, mass, size, keys = T.wanted(state, cache, prefix, query, of)
+    assert (np.abs(T.host(out) - want) <= weight_bound(of, mass, size, keys)).all()
+
+
+@pytest.mark.parametrize("vocab", [300, 40000])
+def test_temperatures_at_their_ends(vocab):
+    """Towards 0 sampling becomes the argmax; towards infinity all tokens have the same share."""
+    counts = [4, 1, 3]
+    state, logits, draft, ids, accept, draw = T.verify_state(counts, vocab, 0.0, True, vocab)
+    want = O.verify(logits, None, ids, [int(f) for f in state.first], 0.0, accept, draw)
+    for temperature in (1e-6, 1e-36):
+        accepted, chosen = T.Verify(state, logits, None, ids, temperature, np.full(state.rows, 0.5), [0.5] * 3)()
+        assert np.array_equal(accepted, want[0]) and np.array_equal(chosen, want[1])
+    # no draft is taken by uniforms above 1 / vocab; the residual leaves the refused token out, so vocab - 1 tokens share the draw (and vocab of them behind no draft)
+    accepted, chosen = T.Verify(state, logits, None, ids, 1e36, np.full(state.rows, 0.5), [0.25 + 0.5 / vocab] * 3)()
+    assert accepted.tolist() == [0, 0, 0]
+    for s in range(3):
+        left = [x for x in range(vocab) if counts[s] == 1 or x != ids[state.first[s] + 1]]
+        at = (0.25 + 0.5 / vocab) * len(left)
+        assert abs(at - round(at)) > 1e-3 and chosen[s] == left[int(at)]
