@@ -177,6 +177,8 @@ __device__ __forceinline__ void tma_prefetch_descriptor(const CUtensorMap* map) 
 // execute grid_dependency_wait() before it touches anything the predecessor writes (and before it writes anything
 // the predecessor reads); everything before that point may only read constants such as weights.  A kernel calls
 // grid_launch_dependents() to let its successor start early.
+// One kernel waits late, that of own tokens beside a shared prefix's (begin_items in prefix.cuh): its predecessor in the stream lets it start only after it
+// has waited itself, writes nothing that this one touches, and is waited for before this one ends.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

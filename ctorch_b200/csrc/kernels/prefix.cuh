@@ -54,7 +54,7 @@ __device__ __forceinline__ int used_splits(int total, int splits, int seen) {
 // the batch, so it is a whole number of powers of two (whole_maximum): another one shifts a weight's exponent and leaves its rounding alone.  (Rounded relative to
 // the maximum itself, f32 results of peaked rows moved by up to 9e-3 from batch to batch, and a third of all bf16 results by a step.)
 //   PLANES, for results in f32 or two planes: two bf16 planes, 15 bits.  The first is cut off, not rounded, and the second larger by 2^-23 of the weight, so that
-//   both are positive where the weight is and an infinite value stays one.
+//   both are positive where the weight is (down to 2^-109) and an infinite value stays one.
 //   Otherwise, for bf16 results, one plane of 8 bits, and the sum is that of the rounded weights: rounding the largest ones cancels.  Half the products.
 __device__ __forceinline__ float whole_maximum(float top) { return top == -INFINITY ? 0.0f : ceilf(top); }
 __device__ __forceinline__ uint32_t first_plane(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
@@ -198,7 +198,8 @@ __device__ __forceinline__ Item item_of_lane(const Item& it, int lane) {
 }
 
 // A kernel that runs beside the prefix's: that one let it start when everything before both was complete, so it need not wait to begin; its first CTA waits
-// before it ends, so that the kernel is complete no earlier than the other and the merge can wait for this one alone.
+// before it ends, so that the kernel is complete no earlier than the other and the merge can wait for this one alone.  This holds because the prefix's kernel is
+// launched just before it on the same stream, and all its CTAs wait before they let it start.
 __device__ __forceinline__ void begin_items(const PrefixParams& p) {
     if (!p.beside) grid_dependency_wait();
     grid_launch_dependents();

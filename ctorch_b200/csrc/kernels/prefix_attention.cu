@@ -759,8 +759,8 @@ Plan make_plan(const b200_prefix_args& a, const b200_rows& whole, int max_length
         time = 10.0 + step_time(plan.own_rows, a.cache.head_dim) * std::max(longest, (static_cast<double>(filled) * prefix_steps + static_cast<double>(own_filled) * length_steps) / kSms);
     }
     if (!mma || !may_join) return plan;
-    // Short prefixes, whose keys come from L2 each time: one item per tile of own rows goes over both and leaves the result.  Measured: 34 sequences of up to 5 tokens
-    // behind 221 and 329 keys 27 us joined, 29 split; 52 single tokens behind 165 8.8 and 14.9; 9 single tokens behind 5755 61 and 24.
+    // Short prefixes, whose keys come from L2 each time: one item per tile of own rows goes over both and leaves the result.  Measured, 32 heads
+    // of 64 over 8: 34 sequences of up to 5 tokens behind 329 keys 13.7 us joined, 16.4 split; 52 single tokens behind 165 12.5 and 13.0; 9 behind 5755 49 and 27.
     const int rows = own_pairs <= 16 ? 16 : own_pairs <= 32 ? 32 : 64, tiles = ceil_div(own_pairs, rows);
     const int64_t items = (tiles == 1 ? pass.sequences : ceil_div64(pairs, rows) + pass.sequences / 2) * kv_heads;
     const double step = step_time(rows, a.cache.head_dim);

@@ -160,7 +160,7 @@ template <int V> __device__ __forceinline__ void finish_item(const AppendParams&
 
 // An item is 2 V values of one head of one row.  grid (rows, blocks of items): a block has one or more whole rows where there are rows for every SM, since it
 // walks from the row to its page (four dependent loads); it asks for the row's values before that, and before it knows whether the row is one of a sequence.
-// Bound by this chain with few rows, by memory with many: 670 MB (18 k rows of 48 heads of 128 to bf16) at 5.8 TB/s.
+// Bound by this chain with few rows, by memory with many: 670 MB (18 k rows of 48 heads of 128 to bf16) in 118 - 125 us, 5.4 - 5.7 TB/s.
 constexpr int kItemsHeld = 4;
 template <int V> __global__ void __launch_bounds__(256) rotary_append_kernel(const AppendParams p) {
     grid_dependency_wait();
@@ -265,8 +265,8 @@ extern "C" int b200_rotary_append(const b200_rotary_append_args* a, const b200_r
     p.by_head = divider(dim / (wide ? 8 : 2));
     const int64_t items = width / (wide ? 8 : 2);
     // Many rows: four items per thread and no thread without, so that as many rows as there is room for have their values on the way.  18 k rows of 48 heads
-    // of 128 (of 64, 10 heads of 128): 116 us (62, 30), with 256 threads whatever the row's length 121 (82, 46).  Short rows share blocks of up to 128 threads:
-    // with rows of 3 heads of 64 10 us, with a block each 20.
+    // of 128 (of 64, 10 heads of 128): 119 us (64, 31), with 256 threads for every 256 items of a row 197 (109, 52).  Short rows share blocks of up to 128 threads:
+    // with rows of 3 heads of 64 11 us, with a block each 20.
     int64_t threads = 256, blocks = (items + 255) / 256, rows = 1;
     if (p.rows.rows >= 148) {
         threads = std::clamp<int64_t>((items + 32 * kItemsHeld - 1) / (32 * kItemsHeld) * 32, 32, 256);

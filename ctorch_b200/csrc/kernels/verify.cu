@@ -3,7 +3,7 @@
 // Two launches.  verify_rows_kernel: for every row of target and draft logits the maximum and the sum of its weights exp((x - max) / T); a row is
 // split over a cluster of CTAs that hold their part in shared memory, so the row is read once although the weights need the maximum first.
 // verify_finish_kernel: one cluster per sequence walks the acceptance tests, then draws from the residual of the row that refused: running sums
-// over segments of 128 values, in index order.  All sums are as good as f64 and added in a fixed order.
+// over segments of 128 values, in index order.  Sums are as good as f64 and added in an order that the row's alignment and the pass's sizes set.
 #include "linear_common.cuh"
 #include "mma.cuh"
 #include "rows.cuh"
@@ -132,8 +132,8 @@ __device__ __forceinline__ Candidate load_cluster_candidate(uint32_t address) {
 __device__ __forceinline__ float most_of(float4 x) { return fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)); }
 
 // grid: clusters of `parts` CTAs, two (target, draft) or one per row.  A part's first kTileVectors come to shared memory with bulk copies and stay for the
-// second pass; longer parts are read twice.  Bound by the chain of a CTA (9 us: launch of the cluster, its row's place, copy, the cluster's barrier, 14 instructions
-// per value), of which an SM holds three with 64 KB each: 825 rows of 128256 take 124 us, 3 TB/s.  What did not help: several rows per cluster with the next one's
+// second pass; longer parts are read twice.  Bound by the chain of a CTA (9 us: launch of the cluster, its row's place, copy, the cluster's barrier, 16 instructions
+// per value), of which an SM holds three with 64 KB each: 710 rows of 128256 take 130 us, 2.8 TB/s.  What did not help: several rows per cluster with the next one's
 // copies under way (+15%), a cluster per sequence that stops at the first refusal (+50%), 512 threads (+10%).
 __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const VerifyParams p) {
     extern __shared__ __align__(128) float4 tile[];
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyParams p
 }
 
 // CTAs per row: parts that a CTA can hold, and more, of 2048 values at least, where there are fewer CTAs than wanted.  Parts of a size cost a cluster's launch and
-// barriers each: 64 x 7 rows of 32000 take 43 us with two parts per row, 60 with eight; 15 rows of 50257 take 31 us with four parts and 29 with eight.
+// barriers each: a batch of 358 rows of 32000 takes 42 us with two parts per row, 50 with eight; 15 rows of 50257 take 18 us with four parts and 14 with eight.
 int split_rows(int64_t vocab, int64_t rows, int64_t ctas) {
     constexpr int kLeast = 2048;
     int parts = 1;

@@ -620,7 +620,7 @@ B200_API int32_t b200_experts_takes_grouped(const b200_experts* args);
  *
  * What a server needs that answers many packed sequences (b200_rows) over one or a few long prompts, with tokens drafted ahead: a view of
  * paged keys and values that several sequences may share pages of, the rotation that is applied while rows are appended, attention that
- * reads a shared prompt once for all its sequences, and the verification of the drafts.  Rows behind the last sequence (from
+ * reads a shared prompt for many sequences at once, and the verification of the drafts.  Rows behind the last sequence (from
  * first[sequences] on, as in a pass of fixed size that is not full) are left as they were. */
 
 /* Paged keys and values in the caller's memory, or those of a cache (b200_kv_cache_pages): pools [pages][kv_heads][page_size][head_dim] and a
@@ -640,7 +640,8 @@ B200_API int b200_kv_cache_pages(const b200_kv_cache* cache, b200_kv_pages* out)
  * cos(position * f_i), i < rot_dims / 2.  PLAIN: f_i = base^(-2 i / rot_dims).  LINEAR: f_i / factor.  BASE: base * factor^(rot_dims /
  * (rot_dims - 2)) in place of base, which leaves f_0 and divides the last f_i by the factor.  PARTS: with turns = original * f_i / (2 pi), the
  * turns that entry i makes in the `original` positions of the training, f_i stays where turns >= high, becomes f_i / factor where turns <=
- * low, and is mixed linearly in between. */
+ * low, and is mixed linearly in the turns in between.  Models that were trained with a ramp over the entry's index i in place of its turns have
+ * other angles, which no kind gives.  An angle is good to 2^-46 of itself: to f32's last bit for angles up to 2^21. */
 enum b200_rotary_kind { B200_ROTARY_PLAIN = 0, B200_ROTARY_LINEAR = 1, B200_ROTARY_BASE = 2, B200_ROTARY_PARTS = 3 };
 typedef struct b200_rotary_scaling {
     int32_t kind;
@@ -675,10 +676,11 @@ B200_API int b200_rotary_append(const b200_rotary_append_args* args, const b200_
 
 /* Grouped-query attention of a pass over a prefix that the sequences of a group share and over each sequence's own tokens: row r of
  * sequence s in group g sees the first prefix_length[group_prefix[g]] positions of that prefix and, in slot[s] of the cache, the positions 0 ..
- * lengths[slot[s]] + r - first[s], which the cache must already hold.  One softmax(scale q.k) over both.  A prefix's keys and values are read
- * once for all rows of a group (short ones once per sequence, from L2, where that takes less time).  Group g owns the sequences group_first[g] .. group_first[g + 1] - 1 of the pass; a sequence in no group has no
- * prefix, a prefix or slot number outside its table no positions; a row that sees nothing gives zeros.  Prefix and cache may be tables over the
- * same pools. */
+ * lengths[slot[s]] + r - first[s], which the cache must already hold.  One softmax(scale q.k) over both.  With heads / kv_heads pairs for every
+ * row, a prefix's keys and values are read once per 256 pairs of a group in bf16 passes with heads of 8 n up to 128, once per 16 to 64 pairs in
+ * others, and, where that takes less time, once per 16 to 64 pairs of a sequence (short prefixes, from L2).  Group g owns the sequences
+ * group_first[g] .. group_first[g + 1] - 1 of the pass; a sequence in no group has no prefix, a prefix or slot number outside its table no positions;
+ * a row that sees nothing gives zeros.  Prefix and cache may be tables over the same pools. */
 typedef struct b200_prefix_args {
     int32_t heads;
     float scale;
@@ -708,8 +710,8 @@ B200_API int b200_prefix_attention(const b200_prefix_args* args, const b200_rows
  * running sum exceeds draw[s] times the total.  Tokens so chosen are distributed as if drawn from p one by one.  Without draft_logits the
  * drafts count as certain (q(x) = 1): what a lookup in the text gives.  temperature 0: a draft is accepted if it is the argmax (b200_argmax's
  * rule), the next token is the argmax; no random numbers are read.  A draft outside [0, vocab) is refused, with p as the residual; so is one
- * whose row of draft_logits has no finite weights.  A row of logits without finite weights (NaN or +inf in it, or nothing but -inf) accepts
- * nothing and gives its argmax.  Weights are exp((x - max) * (1 / temperature)) in f32; a row's sum is off by
+ * whose row of draft_logits has no finite weights.  At temperatures above 0 a row of logits without finite weights (NaN or +inf in it, or nothing but
+ * -inf) accepts nothing and gives its argmax.  Weights are exp((x - max) * (1 / temperature)) in f32; a row's sum is off by
  * 2^-56 for each value, as sums in f64 are. */
 typedef struct b200_verify_args {
     int64_t vocab;                 /* up to 2^23 */
