@@ -711,8 +711,8 @@ B200_API int b200_prefix_attention(const b200_prefix_args* args, const b200_rows
  * drafts count as certain (q(x) = 1): what a lookup in the text gives.  temperature 0: a draft is accepted if it is the argmax (b200_argmax's
  * rule), the next token is the argmax; no random numbers are read.  A draft outside [0, vocab) is refused, with p as the residual; so is one
  * whose row of draft_logits has no finite weights.  At temperatures above 0 a row of logits without finite weights (NaN or +inf in it, or nothing but
- * -inf) accepts nothing and gives its argmax.  Weights are exp((x - max) * (1 / temperature)) in f32; a row's sum is off by
- * 2^-56 for each value, as sums in f64 are. */
+ * -inf) accepts nothing and gives its argmax.  Weights are exp((x - max) * (1 / temperature)) in f32, those below 2^-126
+ * count as 0; a row's sum is off by 2^-56 for each value, as sums in f64 are. */
 typedef struct b200_verify_args {
     int64_t vocab;                 /* up to 2^23 */
     int64_t stride;                /* floats between rows of logits and draft_logits; 0: vocab */
