@@ -409,3 +409,39 @@ def test_temperatures_at_their_ends(vocab):
         left = [x for x in range(vocab) if counts[s] == 1 or x != ids[state.first[s] + 1]]
         at = (0.25 + 0.5 / vocab) * len(left)
         assert abs(at - round(at)) > 1e-3 and chosen[s] == left[int(at)]
+
+
+def test_a_pass_in_parts_is_captured_and_replayed():
+    """Three launches for every part in one graph: the same bits as by the call itself, with other queries and lengths."""
+    rng = np.random.default_rng(1)
+    heads, kv_heads, dim, page, counts = 256, 4, 64, 64, [500, 1, 700, 30]
+    table, prefix_table = np.arange(60).reshape(4, 15), np.arange(60, 64).reshape(1, 4)
+    cache, prefix = T.Paged("bf16", kv_heads, page, dim, 64, table, rng), T.Paged("bf16", kv_heads, page, dim, 1, prefix_table)
+    prefix.key, prefix.value = cache.key, cache.value
+    state = T.Pass(counts, [2, 0, 3, 1], [0, 7, 64, 100])
+    assert state.rows * heads > 1 << 18
+    query = T.dev(rng.standard_normal((state.rows, heads, dim), dtype=np.float32), torch.bfloat16)
+    of = dict(heads=heads, dim=dim, prefixes=[250], group_first=[0, 3], group_prefix=[0], dtype="bf16", max_length=1 << 14, max_prefix=1 << 16)
+    call = T.Attention(state, cache, prefix, query, of)
+    out, one = torch.empty((state.rows, heads, dim), device="cuda"), torch.empty((state.rows, heads, dim), dtype=torch.bfloat16, device="cuda")
+
+    def both():
+        call(out)
+        call(None, one)
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for _ in range(3):
+        query.copy_(torch.randn_like(query, dtype=torch.float32))
+        state.d[3].copy_(T.dev(rng.integers(0, 200, 4).astype(np.int32)))
+        got = []
+        for how in (graph.replay, both):
+            call.scratch.fill_(0xff)
+            out.zero_()
+            one.zero_()
+            how()
+            torch.cuda.synchronize()
+            got.append((out.clone(), one.clone()))
+        assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(*got))
